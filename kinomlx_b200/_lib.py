@@ -248,6 +248,51 @@ class IpcHandle(ctypes.Structure):
     _fields_ = [("bytes", ctypes.c_ubyte * 64)]
 
 
+Q8_INT8 = 0
+Q8_E4M3 = 1
+
+
+class Q8Cache(ctypes.Structure):
+    """kino_q8_cache."""
+
+    _fields_ = [
+        ("k_codes", c_void_p),
+        ("v_codes", c_void_p),
+        ("k_scales", c_void_p),
+        ("v_scales", c_void_p),
+        ("num_blocks", c_int64),
+        ("heads", c_int64),
+        ("dim", c_int64),
+        ("block", c_int64),
+        ("format", c_int),
+        ("table", c_void_p),
+        ("ld_table", c_int64),
+        ("table_blocks", c_int64),
+        ("lengths", c_void_p),
+        ("batch", c_int64),
+    ]
+
+
+class Q8AttentionArgs(ctypes.Structure):
+    """kino_q8_attention_args."""
+
+    _fields_ = [
+        ("q", c_void_p),
+        ("ld_q", c_int64),
+        ("hs_q", c_int64),
+        ("out", c_void_p),
+        ("ld_out", c_int64),
+        ("hs_out", c_int64),
+        ("token_starts", c_void_p),
+        ("rows", c_int64),
+        ("q_heads", c_int64),
+        ("scale", c_float),
+        ("causal", c_int),
+        ("workspace", c_void_p),
+        ("workspace_bytes", c_int64),
+    ]
+
+
 I64 = c_int64
 P = c_void_p
 F = c_float
@@ -364,6 +409,20 @@ SIGNATURES: dict[str, tuple[object, list[object]]] = {
     "kino_peer_barrier": (c_int, [P, I64, I64, I64, P]),
 }
 
+# The 8-bit serving entry points, in include/kino_q8.h order.
+SIGNATURES_Q8: dict[str, tuple[object, list[object]]] = {
+    "kino_q8_abi_version": (c_int, []),
+    "kino_q8_rows": (
+        c_int,
+        [P, I64, P, I64, P, F, F, c_int, P, I64, P, P, c_int, I64, I64, P],
+    ),
+    "kino_q8_linear": (c_int, [P, I64, P, P, I64, P, P, P, I64, I64, I64, I64, P]),
+    "kino_q8_cache_write": (c_int, [POINTER(Q8Cache), P, I64, I64, P, I64, I64, P, I64, P]),
+    "kino_q8_cache_read": (c_int, [POINTER(Q8Cache), P, P, I64, P]),
+    "kino_q8_attention_workspace_size": (I64, [POINTER(Q8Cache), POINTER(Q8AttentionArgs)]),
+    "kino_q8_attention": (c_int, [POINTER(Q8Cache), POINTER(Q8AttentionArgs), P]),
+}
+
 _LIB: ctypes.CDLL | None = None
 
 
@@ -378,7 +437,7 @@ def load() -> ctypes.CDLL:
             "(the sm_100a kernels have no fallback)"
         )
     lib = ctypes.CDLL(str(LIBRARY_PATH))
-    for name, (restype, argtypes) in SIGNATURES.items():
+    for name, (restype, argtypes) in (*SIGNATURES.items(), *SIGNATURES_Q8.items()):
         fn = getattr(lib, name)
         fn.restype = restype
         fn.argtypes = argtypes

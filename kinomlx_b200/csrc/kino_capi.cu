@@ -9,6 +9,7 @@
 #include <utility>
 
 #include "../../include/kino.h"
+#include "../../include/kino_q8.h"
 #include "kino_attention.cuh"
 #include "kino_common.cuh"
 #include "kino_gemm.cuh"
@@ -21,6 +22,9 @@
 #include "kino_vae.cuh"
 #include "kino_quant.cuh"
 #include "kino_f32.cuh"
+#include "kino_q8_attention.cuh"
+#include "kino_q8_gemm.cuh"
+#include "kino_q8_quant.cuh"
 
 // Scratch of kino_group_norm_noalloc: a fixed device array that every GPU loading this library
 // holds until the process exits. Host code only sees a stand-in symbol for it, so its device
@@ -2183,3 +2187,5 @@ kino_status kino_tile_blend_f32(const float* decoded, int64_t frames, int64_t he
 }  // extern "C"
 
 #include "kino_blocks.cuh"
+
+#include "kino_q8_capi.cuh"

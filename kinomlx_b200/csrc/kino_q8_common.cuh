@@ -1,0 +1,132 @@
+// Shared pieces of the 8-bit serving kernels: the two code formats, their scales, and the
+// conversions between codes and floating values.
+//
+// A group of values (a token's row, a weight's output channel, the tokens of one cache block and
+// head) is held as codes times one fp32 scale:
+//   scale = amax / top (top 127 for int8, 448 for e4m3), codes = round-to-even(x * (1 / scale)).
+// The reciprocal is taken once a group (IEEE) and multiplied, so that a code is one fp32 product
+// and one rounding: the same two operations in any implementation give the same code. A group
+// whose scale would fall below 2^-126 (1 / scale would overflow) is a group of zeros with scale 0;
+// one that holds an infinity or a NaN gets the scale NaN and codes 0, so that it reads back as
+// NaN wherever it is used and no code is ever a NaN pattern.
+#pragma once
+#include <cuda_fp8.h>
+
+#include "kino_common.cuh"
+
+namespace kino {
+
+constexpr int Q8_INT8 = 0;
+constexpr int Q8_E4M3 = 1;
+constexpr float Q8_LEAST_SCALE = 1.1754943508222875e-38f;  // 2^-126
+
+template <int FMT>
+__device__ __forceinline__ float q8_top() {
+  return FMT == Q8_INT8 ? 127.0f : 448.0f;
+}
+
+// Records an error for kino_device_status; the first one stays.
+__device__ __forceinline__ void q8_flag(int code) { atomicCAS(&g_device_error, 0, code); }
+
+// Scale of a group from the bit pattern of its largest magnitude. Patterns of non-negative floats
+// order like the floats, with NaN above infinity, so an integer maximum keeps what is not finite.
+template <int FMT>
+__device__ __forceinline__ float q8_scale(uint32_t amax_bits) {
+  if (amax_bits >= 0x7F800000u) return __uint_as_float(0x7FC00000u);
+  const float s = __fdiv_rn(__uint_as_float(amax_bits), q8_top<FMT>());
+  return s < Q8_LEAST_SCALE ? 0.0f : s;
+}
+
+// What a group's values are multiplied by; 0 for scales 0 and NaN.
+__device__ __forceinline__ float q8_inverse(float scale) {
+  return scale > 0.0f ? __frcp_rn(scale) : 0.0f;
+}
+
+__device__ __forceinline__ uint32_t abs_bits(float x) { return __float_as_uint(x) & 0x7FFFFFFFu; }
+
+// Four codes, lowest byte first, of already scaled values. A NaN becomes 0 in both formats: int8
+// through the conversion to integer, e4m3 by the comparison.
+template <int FMT>
+__device__ __forceinline__ uint32_t q8_encode4(float a, float b, float c, float d) {
+  if constexpr (FMT == Q8_INT8) {
+    // the low bytes of four integers that are within [-127, 127] after the clamp
+    const int ia = max(-127, min(127, __float2int_rn(a))), ib = max(-127, min(127, __float2int_rn(b)));
+    const int ic = max(-127, min(127, __float2int_rn(c))), id = max(-127, min(127, __float2int_rn(d)));
+    return __byte_perm(__byte_perm(ia, ib, 0x0040), __byte_perm(ic, id, 0x0040), 0x5410);
+  } else {
+    a = a == a ? a : 0.0f;
+    b = b == b ? b : 0.0f;
+    c = c == c ? c : 0.0f;
+    d = d == d ? d : 0.0f;
+    const uint32_t lo = __nv_cvt_float2_to_fp8x2(make_float2(a, b), __NV_SATFINITE, __NV_E4M3);
+    const uint32_t hi = __nv_cvt_float2_to_fp8x2(make_float2(c, d), __NV_SATFINITE, __NV_E4M3);
+    return lo | (hi << 16);
+  }
+}
+
+// Two codes as exact bf16 values, from a register that holds them in the byte positions given
+// below; the other two bytes may hold anything.
+//
+// int8, codes in the low byte of each half: with u = the low 7 bits, 0x4300 | u is the bf16
+// 128 + u, and 0x4300 | sign bit is 128 or 256 (the sign bit is the exponent's lowest), so their
+// difference is u - 128 * sign, the code.
+// e4m3, codes in the high byte of each half: sign, exponent and mantissa moved to their bf16
+// places are the value times 2^(7 - 127), subnormals included; times 2^120 restores it. (The NaN
+// pattern, which no kernel here writes, reads as 480.)
+__device__ __forceinline__ uint32_t q8_int8_pair(uint32_t spread) {
+  const uint32_t lo = (spread & 0x007F007Fu) | 0x43004300u;
+  const uint32_t hi = (spread & 0x00800080u) | 0x43004300u;
+  uint32_t r;
+  asm("sub.rn.bf16x2 %0, %1, %2;" : "=r"(r) : "r"(lo), "r"(hi));
+  return r;
+}
+__device__ __forceinline__ uint32_t q8_e4m3_pair(uint32_t spread) {
+  const uint32_t t = ((spread >> 4) & 0x07F007F0u) | (spread & 0x80008000u);
+  uint32_t r;
+  asm("mul.rn.bf16x2 %0, %1, %2;" : "=r"(r) : "r"(t), "r"(0x7B807B80u));  // 2^120
+  return r;
+}
+
+// Bytes i and j (0..3 of a, 4..7 of b) as a bf16 pair (i low).
+template <int FMT>
+__device__ __forceinline__ uint32_t q8_pair(uint32_t a, uint32_t b, int i, int j) {
+  if constexpr (FMT == Q8_INT8) {
+    return q8_int8_pair(__byte_perm(a, b, i | (j << 8)));
+  } else {
+    return q8_e4m3_pair(__byte_perm(a, b, (i << 4) | (j << 12)));
+  }
+}
+
+// Four consecutive codes as fp32 values.
+template <int FMT>
+__device__ __forceinline__ void q8_decode4(uint32_t w, float (&f)[4]) {
+  const float2 lo = unpack_bf16x2(q8_pair<FMT>(w, 0u, 0, 1));
+  const float2 hi = unpack_bf16x2(q8_pair<FMT>(w, 0u, 2, 3));
+  f[0] = lo.x;
+  f[1] = lo.y;
+  f[2] = hi.x;
+  f[3] = hi.y;
+}
+
+// Where sequence b's rows are: given starts, or the same number for each.
+struct Q8Rows {
+  const int32_t* starts;  // [batch + 1] or null
+  int each;
+  int64_t rows;
+  __device__ __forceinline__ void of(int b, int64_t& first, int& count) const {
+    if (starts != nullptr) {
+      const int s0 = starts[b], s1 = starts[b + 1];
+      first = s0;
+      count = s1 - s0;
+      if (s0 < 0 || s1 < s0 || s1 > rows) {  // not the rows of this call: nothing to do
+        count = 0;
+        q8_flag(1);
+      }
+    } else {
+      first = static_cast<int64_t>(b) * each;
+      count = each;
+    }
+  }
+};
+
+}  // namespace kino

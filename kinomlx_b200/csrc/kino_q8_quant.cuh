@@ -1,0 +1,346 @@
+// Quantising kernels of the 8-bit serving path: token rows (with the residual's addition and the
+// RMS norm in front), the K/V cache as it is written, and the cache back to bf16.
+#pragma once
+#include "kino_q8_common.cuh"
+
+namespace kino {
+
+__device__ __forceinline__ void q8_unpack8(const uint4& raw, float (&f)[8]) {
+  const uint32_t w[4] = {raw.x, raw.y, raw.z, raw.w};
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const float2 t = unpack_bf16x2(w[i]);
+    f[2 * i] = t.x;
+    f[2 * i + 1] = t.y;
+  }
+}
+
+// ---------------------------------------------------------------- token rows
+// One CTA a row: h = bf16(x + residual), y = h * rsqrt(mean h^2 + eps) * (weight + offset) in
+// fp32, then codes and a scale for the row. The row is read once and stays in registers over the
+// two reductions (sum of squares, largest magnitude), so the kernel moves 2 bytes of x, 2 of the
+// residual in, 2 of the sum out and 1 of code per element: it is bound by HBM. The statistics are
+// taken from the rounded sum, which is what the next layer reads, so that the fused form equals
+// an addition followed by the norm.
+constexpr int Q8_ROW_MAX_THREADS = 512;
+
+struct Q8RowArgs {
+  const __nv_bfloat16* x;
+  int64_t ldx;
+  const __nv_bfloat16* residual;  // or null
+  int64_t ld_residual;
+  const __nv_bfloat16* weight;  // or null
+  float weight_offset;
+  float eps;
+  int norm;
+  __nv_bfloat16* hidden;  // or null
+  int64_t ld_hidden;
+  uint8_t* codes;  // contiguous rows
+  float* scales;
+  int dim;
+};
+
+template <int FMT, int NV>
+__global__ void __launch_bounds__(Q8_ROW_MAX_THREADS) q8_rows_kernel(const Q8RowArgs a) {
+  griddep_wait();
+  griddep_launch();
+  __shared__ float s_sum[16];
+  __shared__ uint32_t s_max[16];
+  const int64_t row = blockIdx.x;
+  const int warps = blockDim.x >> 5;
+  const int nvec = a.dim >> 3;
+  const uint4* xr = reinterpret_cast<const uint4*>(a.x + row * a.ldx);
+  uint4 raw[NV], rres[NV];
+#pragma unroll
+  for (int i = 0; i < NV; ++i) {
+    const int c = threadIdx.x + i * blockDim.x;
+    raw[i] = c < nvec ? __ldcs(xr + c) : make_uint4(0, 0, 0, 0);
+  }
+  if (a.residual != nullptr) {
+    const uint4* rr = reinterpret_cast<const uint4*>(a.residual + row * a.ld_residual);
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+      const int c = threadIdx.x + i * blockDim.x;
+      rres[i] = c < nvec ? __ldcs(rr + c) : make_uint4(0, 0, 0, 0);
+    }
+  }
+  float v[NV][8];
+  float sum = 0.0f;
+#pragma unroll
+  for (int i = 0; i < NV; ++i) {
+    q8_unpack8(raw[i], v[i]);
+    if (a.residual != nullptr) {
+      float r[8];
+      q8_unpack8(rres[i], r);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) v[i][j] = bf16_round(v[i][j] + r[j]);
+    }
+#pragma unroll
+    for (int j = 0; j < 8; ++j) sum = fmaf(v[i][j], v[i][j], sum);
+  }
+  if (a.hidden != nullptr) {
+    uint4* hr = reinterpret_cast<uint4*>(a.hidden + row * a.ld_hidden);
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+      const int c = threadIdx.x + i * blockDim.x;
+      if (c < nvec)
+        hr[c] = make_uint4(pack_bf16x2(v[i][0], v[i][1]), pack_bf16x2(v[i][2], v[i][3]),
+                           pack_bf16x2(v[i][4], v[i][5]), pack_bf16x2(v[i][6], v[i][7]));
+    }
+  }
+  if (a.norm) {
+    sum = warp_sum_f(sum);
+    if (warps > 1) {
+      if ((threadIdx.x & 31) == 0) s_sum[threadIdx.x >> 5] = sum;
+      __syncthreads();
+      sum = (threadIdx.x & 31) < warps ? s_sum[threadIdx.x & 31] : 0.0f;
+      sum = warp_sum_f(sum);
+    }
+    const float inv = rsqrtf(sum / static_cast<float>(a.dim) + a.eps);
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+      const int c = threadIdx.x + i * blockDim.x;
+      if (a.weight != nullptr && c < nvec) {
+        float w[8];
+        q8_unpack8(__ldg(reinterpret_cast<const uint4*>(a.weight) + c), w);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) v[i][j] = v[i][j] * inv * (w[j] + a.weight_offset);
+      } else {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) v[i][j] *= inv;
+      }
+    }
+  }
+  uint32_t top = 0;
+#pragma unroll
+  for (int i = 0; i < NV; ++i)
+#pragma unroll
+    for (int j = 0; j < 8; ++j) top = max(top, abs_bits(v[i][j]));
+  top = __reduce_max_sync(0xffffffffu, top);
+  if (warps > 1) {
+    if ((threadIdx.x & 31) == 0) s_max[threadIdx.x >> 5] = top;
+    __syncthreads();
+    top = (threadIdx.x & 31) < warps ? s_max[threadIdx.x & 31] : 0u;
+    top = __reduce_max_sync(0xffffffffu, top);
+  }
+  const float scale = q8_scale<FMT>(top);
+  const float inv = q8_inverse(scale);
+  if (threadIdx.x == 0) a.scales[row] = scale;
+  uint2* cr = reinterpret_cast<uint2*>(a.codes + row * a.dim);
+#pragma unroll
+  for (int i = 0; i < NV; ++i) {
+    const int c = threadIdx.x + i * blockDim.x;
+    if (c < nvec)
+      cr[c] = make_uint2(
+          q8_encode4<FMT>(v[i][0] * inv, v[i][1] * inv, v[i][2] * inv, v[i][3] * inv),
+          q8_encode4<FMT>(v[i][4] * inv, v[i][5] * inv, v[i][6] * inv, v[i][7] * inv));
+  }
+}
+
+// ---------------------------------------------------------------- cache write
+// Codes live as (block, head, slot, dim): the tokens of one block and head are contiguous, which
+// is the unit every kernel here reads. Sequence b's new tokens take positions lengths[b] on.
+//
+// One CTA per (cache block that gets new tokens, head, K or V). The new tokens' values stay in
+// registers between the maximum and the rounding. A block that holds earlier tokens keeps the
+// larger of its scale and the new tokens': where it grows, the earlier codes are rounded again to
+// the new scale (at most a half step of the new scale each time).
+constexpr int Q8_WRITE_THREADS = 128;
+
+struct Q8WriteArgs {
+  const __nv_bfloat16* x[2];  // k, v
+  int64_t ld[2], head_stride[2];
+  uint8_t* codes[2];
+  float* scales[2];
+  const int32_t* table;
+  int64_t ld_table;
+  int table_blocks;
+  const int32_t* lengths;  // tokens held before this call
+  Q8Rows rows;
+  int batch, heads, dim, block, num_blocks;
+};
+
+// The item-th cache block that gets new tokens, in order of sequences; false past the last one.
+// The same scan in every thread of a warp: each lane counts one sequence's blocks.
+__device__ __forceinline__ bool q8_write_item(const Q8WriteArgs& a, int item, int& b, int& index,
+                                              int& held, int64_t& first, int& count) {
+  int before = 0;
+  for (int b0 = 0; b0 < a.batch; b0 += 32) {
+    const int mine = b0 + static_cast<int>(lane_id());
+    int n = 0;
+    if (mine < a.batch) {
+      int64_t f;
+      int c;
+      a.rows.of(mine, f, c);
+      const int len = a.lengths[mine];
+      if (len < 0) q8_flag(1);
+      if (c > 0 && len >= 0) n = static_cast<int>((static_cast<int64_t>(len) + c - 1) / a.block - len / a.block + 1);
+    }
+    int upto = n;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int up = __shfl_up_sync(0xffffffffu, upto, o);
+      if (static_cast<int>(lane_id()) >= o) upto += up;
+    }
+    const unsigned hit = __ballot_sync(0xffffffffu, before + upto > item);
+    if (hit != 0) {
+      const int l = __ffs(hit) - 1;
+      b = b0 + l;
+      const int skipped = before + __shfl_sync(0xffffffffu, upto - n, l);
+      held = a.lengths[b];
+      a.rows.of(b, first, count);
+      index = held / a.block + (item - skipped);
+      return true;
+    }
+    before += __shfl_sync(0xffffffffu, upto, 31);
+  }
+  return false;
+}
+
+template <int FMT, int NV>
+__global__ void __launch_bounds__(Q8_WRITE_THREADS) q8_cache_write_kernel(const Q8WriteArgs a) {
+  griddep_wait();
+  griddep_launch();
+  __shared__ uint32_t s_max[Q8_WRITE_THREADS / 32];
+  int b, index, held, count;
+  int64_t first;
+  if (!q8_write_item(a, blockIdx.x, b, index, held, first, count)) return;
+  const int page = index < a.table_blocks ? a.table[b * a.ld_table + index] : -1;
+  if (page < 0 || page >= a.num_blocks) {  // past the table, or no block of this cache
+    if (threadIdx.x == 0) q8_flag(1);
+    return;
+  }
+  const int head = blockIdx.y, kv = blockIdx.z;
+  const int64_t unit = static_cast<int64_t>(page) * a.heads + head;
+  uint8_t* codes = a.codes[kv] + unit * a.block * a.dim;
+  const int chunks = a.dim >> 3;  // 8-value chunks of a token: 8 or 16
+  const int64_t at0 = static_cast<int64_t>(index) * a.block;  // position of slot 0
+  const __nv_bfloat16* src = a.x[kv] + head * a.head_stride[kv];
+  uint4 raw[NV];
+  bool fresh[NV];
+  uint32_t top = 0;
+#pragma unroll
+  for (int i = 0; i < NV; ++i) {
+    const int e = threadIdx.x + i * Q8_WRITE_THREADS;
+    const int slot = e / chunks, c = e % chunks;
+    const int64_t t = at0 + slot - held;
+    fresh[i] = t >= 0 && t < count;
+    raw[i] = make_uint4(0, 0, 0, 0);
+    if (fresh[i]) raw[i] = __ldcs(reinterpret_cast<const uint4*>(src + (first + t) * a.ld[kv]) + c);
+  }
+#pragma unroll
+  for (int i = 0; i < NV; ++i) {
+    const uint32_t w[4] = {raw[i].x, raw[i].y, raw[i].z, raw[i].w};
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+      top = max(top, max((w[j] & 0x7FFFu) << 16, w[j] & 0x7FFF0000u));
+  }
+  top = __reduce_max_sync(0xffffffffu, top);
+  if ((threadIdx.x & 31) == 0) s_max[threadIdx.x >> 5] = top;
+  const bool earlier = held > at0;
+  const float before = earlier ? a.scales[kv][unit] : 0.0f;
+  __syncthreads();  // every thread has read the old scale
+#pragma unroll
+  for (int i = 0; i < Q8_WRITE_THREADS / 32; ++i) top = max(top, s_max[i]);
+  float scale = q8_scale<FMT>(top);
+  if (!(before <= scale)) scale = before == before && scale == scale ? before : __uint_as_float(0x7FC00000u);
+  const float inv = q8_inverse(scale);
+  if (threadIdx.x == 0) a.scales[kv][unit] = scale;
+  const bool grown = earlier && scale > before;
+  const float ratio = before * inv;
+#pragma unroll
+  for (int i = 0; i < NV; ++i) {
+    const int e = threadIdx.x + i * Q8_WRITE_THREADS;
+    uint2* dst = reinterpret_cast<uint2*>(codes) + e;
+    float f[8];
+    if (fresh[i]) {
+      q8_unpack8(raw[i], f);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) f[j] *= inv;
+    } else if (grown && at0 + e / chunks < held) {
+      const uint2 old = *dst;
+      float lo[4], hi[4];
+      q8_decode4<FMT>(old.x, lo);
+      q8_decode4<FMT>(old.y, hi);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        f[j] = lo[j] * ratio;
+        f[4 + j] = hi[j] * ratio;
+      }
+    } else {
+      continue;
+    }
+    *dst = make_uint2(q8_encode4<FMT>(f[0], f[1], f[2], f[3]),
+                      q8_encode4<FMT>(f[4], f[5], f[6], f[7]));
+  }
+}
+
+// ---------------------------------------------------------------- cache read
+// The tokens [0, tokens) of every sequence as (batch, tokens, heads, dim) bf16, zeros past a
+// sequence's length: one thread takes 16 codes of K and of V (one scale each) and writes two
+// 32-byte runs; threads follow the output, so stores are contiguous and a head's 64 or 128 codes
+// are read as whole lines. 1 byte in, 2 out per value, bound by HBM.
+struct Q8ReadArgs {
+  const uint8_t* codes[2];
+  const float* scales[2];
+  __nv_bfloat16* out[2];  // contiguous
+  const int32_t* table;
+  int64_t ld_table;
+  int table_blocks;
+  const int32_t* lengths;
+  int64_t tokens;
+  int heads, dim, block, num_blocks;
+};
+
+template <int FMT>
+__global__ void __launch_bounds__(256) q8_cache_read_kernel(const Q8ReadArgs a) {
+  griddep_wait();
+  griddep_launch();
+  const int b = blockIdx.y;
+  const int chunks = a.dim >> 4;
+  const int64_t per_token = static_cast<int64_t>(a.heads) * chunks;
+  const int64_t total = a.tokens * per_token;
+  const int64_t e = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x;
+  if (e >= total) return;
+  const int64_t t = e / per_token;
+  const int rest = static_cast<int>(e - t * per_token);
+  const int head = rest / chunks, c = rest % chunks;
+  const int64_t capacity = static_cast<int64_t>(a.table_blocks) * a.block;
+  const int64_t length = a.lengths[b];
+  if (length < 0 || length > capacity) q8_flag(1);
+  int page = -1;
+  if (t < length && t < capacity) {
+    page = a.table[b * a.ld_table + t / a.block];
+    if (page < 0 || page >= a.num_blocks) {
+      q8_flag(1);
+      page = -1;
+    }
+  }
+  const int64_t dst = ((b * a.tokens + t) * a.heads + head) * a.dim + c * 16;
+  uint4 raw[2] = {make_uint4(0, 0, 0, 0), make_uint4(0, 0, 0, 0)};
+  float scale[2] = {0.0f, 0.0f};
+  if (page >= 0) {
+    const int64_t unit = static_cast<int64_t>(page) * a.heads + head;
+    const int64_t src = (unit * a.block + t % a.block) * a.dim + c * 16;
+#pragma unroll
+    for (int kv = 0; kv < 2; ++kv) {
+      raw[kv] = __ldcs(reinterpret_cast<const uint4*>(a.codes[kv] + src));
+      scale[kv] = a.scales[kv][unit];
+    }
+  }
+#pragma unroll
+  for (int kv = 0; kv < 2; ++kv) {
+    const uint32_t w[4] = {raw[kv].x, raw[kv].y, raw[kv].z, raw[kv].w};
+    uint32_t o[8];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      float f[4];
+      q8_decode4<FMT>(w[i], f);
+      o[2 * i] = pack_bf16x2(f[0] * scale[kv], f[1] * scale[kv]);
+      o[2 * i + 1] = pack_bf16x2(f[2] * scale[kv], f[3] * scale[kv]);
+    }
+    store_16(a.out[kv] + dst, o);
+  }
+}
+
+}  // namespace kino

@@ -1,0 +1,369 @@
+"""8-bit serving operators: torch front end of include/kino_q8.h.
+
+Values are held as 8-bit codes (int8 or float8_e4m3fn) times an fp32 scale for each group: a
+token's row, a weight's output channel, or the tokens of one cache block and head. A group's scale
+is its largest magnitude over 127 (int8) or 448 (e4m3); a group of zeros (or of magnitudes below
+about 1e-36) has scale 0; one that holds an infinity or a NaN has the scale NaN and reads back as
+NaN.
+
+    codes, scales, hidden = rms_norm_quantize(x, weight, residual=hidden)
+    y = linear_int8(codes, scales, w_codes, w_scales)      # w from quantize_tokens(weight)
+    kv_cache_write(cache, k, v, table, lengths)
+    out = kv_cache_attention(q, cache, table, lengths + 1)
+
+Like `ops`, these have no CPU path: a tensor of the wrong device, type or shape is a ValueError, a
+refusal by the library a RuntimeError. Lengths, token starts and block tables are read on the
+device; entries that do not fit are skipped there and `ops.device_status` raises.
+"""
+
+from __future__ import annotations
+
+from typing import NamedTuple
+
+import torch
+
+from . import _lib
+from .ops import _need, _ptr, _stream, _timed
+
+BF16 = torch.bfloat16
+I32 = torch.int32
+F32 = torch.float32
+FORMATS = {torch.int8: _lib.Q8_INT8, torch.float8_e4m3fn: _lib.Q8_E4M3}
+
+__all__ = [
+    "KVCache",
+    "kv_cache_attention",
+    "kv_cache_read",
+    "kv_cache_write",
+    "linear_int8",
+    "new_kv_cache",
+    "quantize_tokens",
+    "rms_norm_quantize",
+]
+
+
+def _format(dtype: torch.dtype) -> int:
+    if dtype not in FORMATS:
+        raise ValueError(f"codes are int8 or float8_e4m3fn, not {dtype}")
+    return FORMATS[dtype]
+
+
+def _same_device(t: torch.Tensor, name: str, device: torch.device) -> None:
+    if t.device != device:
+        raise ValueError(f"{name} is on {t.device}, not on {device}")
+
+
+class _on:
+    """Makes a tensor's GPU the current one for a call (and its stream the one launched on)."""
+
+    __slots__ = ("guard",)
+
+    def __init__(self, device: torch.device):
+        other = device.index is not None and device.index != torch.cuda.current_device()
+        self.guard = torch.cuda.device(device) if other else None
+
+    def __enter__(self):
+        if self.guard is not None:
+            self.guard.__enter__()
+
+    def __exit__(self, *exc):
+        if self.guard is not None:
+            self.guard.__exit__(*exc)
+        return False
+
+
+def _rows(t: torch.Tensor, name: str) -> torch.Tensor:
+    """(..., dim) as (rows, dim) without a copy."""
+    if t.dim() == 2:
+        return t
+    if t.dim() == 0:
+        raise ValueError(f"{name} needs rows")
+    try:
+        return t.view(-1, t.shape[-1])
+    except RuntimeError:
+        raise ValueError(f"{name}: rows of {tuple(t.shape)} are not at one stride") from None
+
+
+def _quantize_rows(x, weight, eps, residual, dtype, weight_offset, norm, hidden, label):
+    fmt = _format(dtype)
+    _need(x, "x")
+    x2 = _rows(x, "x")
+    rows, dim = x2.shape
+    device = x.device
+    codes = torch.empty(x.shape, device=device, dtype=dtype)
+    scales = torch.empty(x.shape[:-1], device=device, dtype=F32)
+    r2 = h2 = None
+    if residual is not None:
+        _need(residual, "residual")
+        _same_device(residual, "residual", device)
+        if residual.shape != x.shape:
+            raise ValueError(f"residual {tuple(residual.shape)} does not match {tuple(x.shape)}")
+        if hidden is None:
+            hidden = torch.empty(x.shape, device=device, dtype=BF16)
+        _need(hidden, "hidden")
+        _same_device(hidden, "hidden", device)
+        if hidden.shape != x.shape:
+            raise ValueError(f"hidden {tuple(hidden.shape)} does not match {tuple(x.shape)}")
+        r2, h2 = _rows(residual, "residual"), _rows(hidden, "hidden")
+    elif hidden is not None:
+        raise ValueError("hidden is the sum with a residual: give one")
+    if weight is not None:
+        _need(weight, "weight")
+        _same_device(weight, "weight", device)
+        if tuple(weight.shape) != (dim,):
+            raise ValueError(f"weight {tuple(weight.shape)} does not match width {dim}")
+    if rows and dim:
+        with _on(device), _timed(label, 0.0, (3.0 if r2 is None else 7.0) * rows * dim):
+            _lib.call(
+                "kino_q8_rows", x2.data_ptr(), x2.stride(0), _ptr(r2),
+                0 if r2 is None else r2.stride(0), _ptr(weight), weight_offset, eps, norm,
+                _ptr(h2), 0 if h2 is None else h2.stride(0), codes.data_ptr(), scales.data_ptr(),
+                fmt, rows, dim, _stream())
+    return codes, scales, x if hidden is None else hidden
+
+
+def quantize_tokens(x: torch.Tensor, dtype: torch.dtype = torch.int8):
+    """Codes like x and a scale for each row of x (..., dim) bf16: activations by token, or a
+    weight (out, in) by output channel. dim a multiple of 8, at most 16384."""
+    codes, scales, _ = _quantize_rows(x, None, 0.0, None, dtype, 0.0, 0, None, "quantize_tokens")
+    return codes, scales
+
+
+def rms_norm_quantize(
+    x: torch.Tensor,
+    weight: torch.Tensor | None = None,
+    eps: float = 1e-6,
+    *,
+    residual: torch.Tensor | None = None,
+    dtype: torch.dtype = torch.int8,
+    weight_offset: float = 0.0,
+    hidden: torch.Tensor | None = None,
+):
+    """(codes, scales, hidden): hidden = bf16(x + residual) (x itself without a residual), and the
+    codes and row scales of its RMS norm times (weight + weight_offset), which stays in fp32 until
+    it is rounded to a code. `hidden` may be given, also as x or residual (in place)."""
+    return _quantize_rows(x, weight, eps, residual, dtype, weight_offset, 1, hidden,
+                          "rms_norm_quantize")
+
+
+def linear_int8(
+    codes: torch.Tensor,
+    scales: torch.Tensor,
+    w_codes: torch.Tensor,
+    w_scales: torch.Tensor,
+    bias: torch.Tensor | None = None,
+    out: torch.Tensor | None = None,
+) -> torch.Tensor:
+    """bf16(codes @ w_codes.T * scales[:, None] * w_scales + bias) for int8 codes (..., k) with a
+    scale for each row and an int8 weight (n, k) with one for each channel; the sum over k is
+    exact. k a multiple of 16, n of 8."""
+    _need(codes, "codes", torch.int8)
+    _need(w_codes, "w_codes", torch.int8)
+    _need(scales, "scales", F32)
+    _need(w_scales, "w_scales", F32)
+    x2 = _rows(codes, "codes")
+    m, k = x2.shape
+    if w_codes.dim() != 2 or w_codes.shape[1] != k:
+        raise ValueError(f"weight {tuple(w_codes.shape)} does not match input width {k}")
+    n = w_codes.shape[0]
+    device = codes.device
+    if scales.shape != codes.shape[:-1] or not scales.is_contiguous():
+        raise ValueError(f"scales {tuple(scales.shape)} are not one for each row, contiguous")
+    if w_scales.shape != (n,):
+        raise ValueError(f"w_scales {tuple(w_scales.shape)} are not one for each of {n} channels")
+    for t, name in ((scales, "scales"), (w_codes, "w_codes"), (w_scales, "w_scales")):
+        _same_device(t, name, device)
+    if bias is not None:
+        _need(bias, "bias")
+        _same_device(bias, "bias", device)
+        if bias.shape != (n,):
+            raise ValueError(f"bias {tuple(bias.shape)} is not one for each of {n} channels")
+    if out is None:
+        out = torch.empty((*codes.shape[:-1], n), device=device, dtype=BF16)
+    else:
+        _need(out, "out")
+        _same_device(out, "out", device)
+        if out.shape != (*codes.shape[:-1], n):
+            raise ValueError(f"out {tuple(out.shape)} does not match ({m}, {n})")
+    o2 = _rows(out, "out")
+    if m and n:
+        with _on(device), _timed("linear_int8", 2.0 * m * n * k, 1.0 * m * k + n * k + 2 * m * n):
+            _lib.call(
+                "kino_q8_linear", x2.data_ptr(), x2.stride(0) if m > 1 else k, scales.data_ptr(),
+                w_codes.data_ptr(), w_codes.stride(0) if n > 1 else k, w_scales.data_ptr(),
+                _ptr(bias), out.data_ptr(), o2.stride(0) if m > 1 else n, m, n, k, _stream())
+    return out
+
+
+class KVCache(NamedTuple):
+    """Keys and values in 8 bits: codes (blocks, heads, block tokens, dim), int8 or float8_e4m3fn,
+    with a scale for each block and head, (blocks, heads) fp32. All contiguous; dim 64 or 128,
+    block tokens 16, 32, 64 or 128. Token t of sequence b is slot t % block of the block
+    table[b, t // block]."""
+
+    k_codes: torch.Tensor
+    v_codes: torch.Tensor
+    k_scales: torch.Tensor
+    v_scales: torch.Tensor
+
+
+def new_kv_cache(blocks: int, heads: int, dim: int, *, block_tokens: int = 64,
+                 dtype: torch.dtype = torch.int8, device: torch.device | str = "cuda") -> KVCache:
+    """An empty cache (zeros)."""
+    _format(dtype)
+    if dim not in (64, 128) or block_tokens not in (16, 32, 64, 128):
+        raise ValueError(f"heads of 64 or 128 and blocks of 16, 32, 64 or 128 tokens, not {dim} "
+                         f"and {block_tokens}")
+    if blocks < 1 or heads < 1:
+        raise ValueError(f"a cache of {blocks} blocks and {heads} heads")
+    codes = [torch.zeros((blocks, heads, block_tokens, dim), device=device, dtype=torch.int8)
+             .view(dtype) for _ in range(2)]
+    scales = [torch.zeros((blocks, heads), device=device, dtype=F32) for _ in range(2)]
+    return KVCache(*codes, *scales)
+
+
+def _cache_args(cache: KVCache, table: torch.Tensor, lengths: torch.Tensor) -> _lib.Q8Cache:
+    k, v, ks, vs = cache
+    device = k.device
+    fmt = _format(k.dtype)
+    if k.dim() != 4 or v.shape != k.shape or v.dtype != k.dtype:
+        raise ValueError(f"codes of keys {tuple(k.shape)} and values {tuple(v.shape)} are not one "
+                         "(blocks, heads, tokens, dim) type and shape")
+    blocks, heads, block, dim = k.shape
+    if ks.shape != (blocks, heads) or vs.shape != (blocks, heads):
+        raise ValueError(f"scales {tuple(ks.shape)}, {tuple(vs.shape)} are not (blocks, heads)")
+    if not (k.is_cuda and k.is_contiguous() and v.is_contiguous() and ks.is_contiguous()
+            and vs.is_contiguous() and ks.dtype == F32 and vs.dtype == F32):
+        raise ValueError("a cache is contiguous CUDA tensors with fp32 scales")
+    if table.dtype != I32 or lengths.dtype != I32:
+        raise ValueError("block table and lengths are int32")
+    if table.dim() != 2 or lengths.shape != table.shape[:1]:
+        raise ValueError(f"table {tuple(table.shape)} and lengths {tuple(lengths.shape)} are not "
+                         "(batch, blocks) and (batch,)")
+    if table.stride(1) != 1 and table.shape[1] > 1 or not lengths.is_contiguous():
+        raise ValueError("block table rows and lengths need unit strides")
+    for t in (v, ks, vs, table, lengths):
+        if t.device != device:
+            raise ValueError(f"cache, table and lengths on {t.device} and {device}")
+    batch, wide = table.shape
+    return _lib.Q8Cache(k.data_ptr(), v.data_ptr(), ks.data_ptr(), vs.data_ptr(), blocks, heads,
+                        dim, block, fmt, table.data_ptr(),
+                        table.stride(0) if batch > 1 else max(wide, 1), wide, lengths.data_ptr(),
+                        batch)
+
+
+def _starts(token_starts: torch.Tensor | None, batch: int, rows: int,
+            device: torch.device) -> int | None:
+    if token_starts is None:
+        if rows % batch:
+            raise ValueError(f"{rows} rows do not divide over {batch} sequences")
+        return None
+    if token_starts.dtype != I32 or token_starts.shape != (batch + 1,) \
+            or not token_starts.is_contiguous():
+        raise ValueError(f"token_starts are batch + 1 = {batch + 1} int32, contiguous")
+    _same_device(token_starts, "token_starts", device)
+    return token_starts.data_ptr()
+
+
+def _heads(t: torch.Tensor, name: str, dim: int, device: torch.device) -> None:
+    _need(t, name)
+    _same_device(t, name, device)
+    if t.dim() != 3 or t.shape[2] != dim:
+        raise ValueError(f"{name} {tuple(t.shape)} is not (rows, heads, {dim})")
+
+
+def kv_cache_write(
+    cache: KVCache,
+    k: torch.Tensor,
+    v: torch.Tensor,
+    block_table: torch.Tensor,
+    lengths: torch.Tensor,
+    token_starts: torch.Tensor | None = None,
+) -> None:
+    """Quantise new tokens into the cache, in place. k, v (rows, heads, dim) bf16 (any row and
+    head strides that are multiples of 8); block_table (batch, blocks) int32; lengths (batch,)
+    int32, the tokens each sequence holds before. Sequence b's rows are token_starts[b] to
+    token_starts[b + 1], or rows / batch each; they take positions lengths[b] on. Where a block
+    already holds tokens, its scale only grows, and its codes are rounded again when it does.
+
+    A cache block may belong to one sequence of a call only (sequences that share blocks write
+    behind them)."""
+    args = _cache_args(cache, block_table, lengths)
+    device = cache[0].device
+    _heads(k, "k", args.dim, device)
+    _heads(v, "v", args.dim, device)
+    rows = k.shape[0]
+    if k.shape != v.shape or k.shape[1] != args.heads:
+        raise ValueError(f"k {tuple(k.shape)} and v {tuple(v.shape)} are not (rows, {args.heads}, "
+                         f"{args.dim})")
+    if not rows or not args.batch:
+        return
+    starts = _starts(token_starts, args.batch, rows, device)
+    with _on(device), _timed("kv_cache_write", 0.0, 6.0 * k.numel()):
+        _lib.call("kino_q8_cache_write", args, k.data_ptr(), k.stride(0), k.stride(1),
+                  v.data_ptr(), v.stride(0), v.stride(1), starts, rows, _stream())
+
+
+def kv_cache_read(
+    cache: KVCache,
+    block_table: torch.Tensor,
+    lengths: torch.Tensor,
+    tokens: int,
+) -> tuple[torch.Tensor, torch.Tensor]:
+    """Keys and values of tokens [0, tokens) of every sequence as (batch, tokens, heads, dim)
+    bf16, zeros from a sequence's length on."""
+    args = _cache_args(cache, block_table, lengths)
+    device = cache[0].device
+    if tokens < 0:
+        raise ValueError(f"{tokens} tokens")
+    shape = (args.batch, tokens, args.heads, args.dim)
+    k, v = (torch.empty(shape, device=device, dtype=BF16) for _ in range(2))
+    if k.numel():
+        with _on(device), _timed("kv_cache_read", 0.0, 6.0 * k.numel()):
+            _lib.call("kino_q8_cache_read", args, k.data_ptr(), v.data_ptr(), tokens, _stream())
+    return k, v
+
+
+def kv_cache_attention(
+    q: torch.Tensor,
+    cache: KVCache,
+    block_table: torch.Tensor,
+    lengths: torch.Tensor,
+    token_starts: torch.Tensor | None = None,
+    *,
+    causal: bool = True,
+    scale: float | None = None,
+    out: torch.Tensor | None = None,
+) -> torch.Tensor:
+    """softmax(q k^T * scale) v over the cached tokens of each sequence. q (rows, query heads,
+    dim) bf16, query heads a multiple of the cache's heads (head h reads cache head h // group);
+    lengths (batch,) int32, the tokens in the cache, among them the sequence's queries, which are
+    its last tokens: with `causal` query i of n sees keys up to position lengths - n + i. Rows go
+    to sequences as in `kv_cache_write`. A query that sees no key gives zeros. Rows of `out`
+    outside every sequence are left as they were (uninitialised where `out` is not given)."""
+    args = _cache_args(cache, block_table, lengths)
+    device = cache[0].device
+    _heads(q, "q", args.dim, device)
+    rows, heads = q.shape[:2]
+    if heads % args.heads:
+        raise ValueError(f"{heads} query heads on {args.heads} cache heads")
+    if out is None:
+        out = torch.empty(q.shape, device=device, dtype=BF16)
+    else:
+        _heads(out, "out", args.dim, device)
+        if out.shape != q.shape:
+            raise ValueError(f"out {tuple(out.shape)} does not match q {tuple(q.shape)}")
+    if not rows or not heads or not args.batch:
+        return out
+    starts = _starts(token_starts, args.batch, rows, device)
+    with _on(device), _timed("kv_cache_attention"):
+        call = _lib.Q8AttentionArgs(
+            q.data_ptr(), q.stride(0), q.stride(1), out.data_ptr(), out.stride(0), out.stride(1),
+            starts, rows, heads, args.dim**-0.5 if scale is None else scale, int(causal))
+        size = _lib.load().kino_q8_attention_workspace_size(args, call)
+        if size < 0:
+            raise RuntimeError(f"kino_q8_attention: {_lib.last_error()}")
+        space = torch.empty(size, device=device, dtype=torch.uint8)
+        call.workspace, call.workspace_bytes = space.data_ptr(), size
+        _lib.call("kino_q8_attention", args, call, _stream())
+    return out

@@ -1,0 +1,130 @@
+"""The 8-bit serving operators from their definitions in 64 bits, on the CPU.
+
+Codes are whole numbers (int8) or the values of e4m3 codes, as float64. The quantisation of bf16
+values is also given in fp32 steps (`scale_f32`, `codes_f32`): one correctly rounded quotient, one
+reciprocal, one product and one rounding, so that another implementation of the same steps has to
+give the same codes bit for bit.
+"""
+
+from __future__ import annotations
+
+import math
+
+import torch
+
+TOP = {torch.int8: 127.0, torch.float8_e4m3fn: 448.0}
+F64 = torch.float64
+
+
+def scale_f32(amax: torch.Tensor, dtype: torch.dtype) -> torch.Tensor:
+    """fp32 scale of groups with these largest magnitudes (NaN where not finite)."""
+    s = amax.float() / torch.tensor(TOP[dtype], dtype=torch.float32)
+    s = torch.where(s < 2.0**-126, torch.zeros_like(s), s)
+    return torch.where(torch.isfinite(amax), s, torch.full_like(s, math.nan))
+
+
+def inverse_f32(scale: torch.Tensor) -> torch.Tensor:
+    return torch.where(scale > 0, 1.0 / scale, torch.zeros_like(scale))
+
+
+def codes_f32(scaled: torch.Tensor, dtype: torch.dtype) -> torch.Tensor:
+    """Codes of already scaled fp32 values; NaN gives 0."""
+    x = torch.nan_to_num(scaled, nan=0.0, posinf=TOP[dtype], neginf=-TOP[dtype])
+    if dtype == torch.int8:
+        return x.round().clamp(-127, 127).to(torch.int8)
+    return x.clamp(-448, 448).to(torch.float8_e4m3fn)
+
+
+def quantize_rows(x: torch.Tensor, dtype: torch.dtype):
+    """(codes, scales) of the last dimension, in fp32 steps."""
+    x = x.float()
+    bad = ~torch.isfinite(x).all(-1)
+    amax = torch.nan_to_num(x, nan=0.0, posinf=0.0, neginf=0.0).abs().amax(-1)
+    scale = scale_f32(torch.where(bad, torch.full_like(amax, math.nan), amax), dtype)
+    codes = codes_f32(x * inverse_f32(scale)[..., None], dtype)
+    return torch.where(bad[..., None], torch.zeros_like(codes.float()), codes.float()).to(dtype), scale
+
+
+def rms_norm(x, weight=None, eps=1e-6, residual=None, offset=0.0):
+    """(hidden bf16, normed float64)."""
+    h = x if residual is None else (x.float() + residual.float()).to(torch.bfloat16)
+    y = h.to(F64)
+    y = y / torch.sqrt(y.square().mean(-1, keepdim=True) + eps)
+    return h, y if weight is None else y * (weight.to(F64) + offset)
+
+
+def linear(codes, scales, w_codes, w_scales, bias=None):
+    y = (codes.to(F64) @ w_codes.to(F64).T) * scales.to(F64)[..., None] * w_scales.to(F64)
+    return y if bias is None else y + bias.to(F64)
+
+
+def rows_of(starts, batch: int, rows: int) -> list[tuple[int, int]]:
+    if starts is None:
+        n = rows // batch
+        return [(b * n, n) for b in range(batch)]
+    s = starts.tolist()
+    return [(s[b], s[b + 1] - s[b]) for b in range(batch)]
+
+
+def cache_write(codes, scales, x, table, lengths, starts=None):
+    """New (codes, scales) of one of keys or values, in fp32 steps; x (rows, heads, dim)."""
+    dtype, block = codes.dtype, codes.shape[2]
+    codes, scales = codes.float().clone(), scales.clone()
+    for b, (first, n) in enumerate(rows_of(starts, len(lengths), x.shape[0])):
+        held = int(lengths[b])
+        for j in range(held // block, (held + n - 1) // block + 1 if n else 0):
+            page = int(table[b, j])
+            t0, t1 = max(held, j * block), min(held + n, (j + 1) * block)
+            new = x[first + t0 - held : first + t1 - held].float().transpose(0, 1)
+            earlier = max(0, held - j * block)
+            bad = ~torch.isfinite(new).all(-1).all(-1)
+            amax = torch.nan_to_num(new, nan=0.0, posinf=0.0, neginf=0.0).abs().amax((1, 2))
+            scale = scale_f32(torch.where(bad, torch.full_like(amax, math.nan), amax), dtype)
+            if earlier:
+                before = scales[page]
+                scale = torch.maximum(scale, before)  # NaN wins
+                ratio = torch.where(scale > before, before * inverse_f32(scale), torch.ones_like(scale))
+                old = codes[page, :, :earlier]
+                again = codes_f32(old * ratio[:, None, None], dtype).float()
+                codes[page, :, :earlier] = torch.where((scale > before)[:, None, None], again, old)
+            codes[page, :, t0 - j * block : t1 - j * block] = codes_f32(
+                new * inverse_f32(scale)[:, None, None], dtype).float()
+            scales[page] = scale
+    return codes.to(dtype), scales
+
+
+def cached(codes, scales, table_row, length: int) -> torch.Tensor:
+    """(heads, length, dim) float64 values of one sequence."""
+    block = codes.shape[2]
+    pages = [codes[int(p)].to(F64) * scales[int(p)].to(F64)[:, None, None]
+             for p in table_row[: -(-length // block)]]
+    if not pages:
+        return torch.zeros((codes.shape[1], 0, codes.shape[3]), dtype=F64)
+    return torch.cat(pages, 1)[:, :length]
+
+
+def attention(q, k_codes, v_codes, k_scales, v_scales, table, lengths, starts=None, *, causal=True,
+              scale=None):
+    """(out, weight, reach) float64 like q: softmax attention, zeros for rows without keys; weight
+    = softmax @ |v|, and reach = the largest sum of |q k| * scale a row meets: what the rounding
+    errors of an implementation in shorter types scale with."""
+    rows, heads, dim = q.shape
+    group = heads // k_codes.shape[1]
+    scale = dim**-0.5 if scale is None else scale
+    out, weight = (torch.zeros(q.shape, dtype=F64) for _ in range(2))
+    reach = torch.zeros((rows, heads, 1), dtype=F64)
+    for b, (first, n) in enumerate(rows_of(starts, len(lengths), rows)):
+        length = int(lengths[b])
+        k = cached(k_codes, k_scales, table[b], length)
+        v = cached(v_codes, v_scales, table[b], length)
+        for i in range(n):
+            seen = min(length, max(0, length - n + i + 1)) if causal else length
+            if seen == 0:
+                continue
+            for h in range(heads):
+                x, kk, vv = q[first + i, h].to(F64), k[h // group, :seen], v[h // group, :seen]
+                p = torch.softmax(kk @ x * scale, 0)
+                out[first + i, h] = p @ vv
+                weight[first + i, h] = p @ vv.abs()
+                reach[first + i, h] = (kk.abs() @ x.abs()).max() * scale
+    return out, weight, reach

@@ -1,0 +1,317 @@
+"""8-bit serving operators on the GPU against their definitions in 64 bits.
+
+Where a kernel takes the same fp32 steps as the oracle (quantising bf16 values, the cache) codes and
+scales are equal bit for bit. Elsewhere a bound counts the roundings: fp32 2^-24, bf16 2^-8 of the
+value each, half a code step for a code.
+"""
+
+from __future__ import annotations
+
+import math
+
+import pytest
+import torch
+
+from kinomlx_b200 import ops, ops_q8
+from oracle import serving_q8 as ref
+
+pytestmark = pytest.mark.gpu
+
+BF16 = torch.bfloat16
+INT8, E4M3 = torch.int8, torch.float8_e4m3fn
+DTYPES = [INT8, E4M3]
+
+
+def _gen(seed):
+    return torch.Generator().manual_seed(seed)
+
+
+def _normal(shape, seed, std=1.0):
+    return (torch.randn(shape, generator=_gen(seed)) * std).to(BF16)
+
+
+def _same(a, b):
+    a, b = a.cpu().float(), b.cpu().float()
+    return bool(((a == b) | (a.isnan() & b.isnan())).all())
+
+
+# ---------------------------------------------------------------- rows
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize(("rows", "dim"), [(1, 8), (3, 64), (5, 504), (17, 1032), (2, 4096),
+                                           (3, 8200), (2, 16384)])
+def test_quantize_tokens_is_exact(cuda_device, dtype, rows, dim):
+    x = _normal((rows, dim), rows + dim)
+    x[0] *= 1e-3
+    codes, scales = ops_q8.quantize_tokens(x.to(cuda_device), dtype)
+    want, want_scales = ref.quantize_rows(x, dtype)
+    assert codes.dtype == dtype and torch.equal(scales.cpu(), want_scales)
+    assert _same(codes, want)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_quantize_tokens_special_rows(cuda_device, dtype):
+    x = _normal((7, 128), 3)
+    x[0] = 0
+    x[1] = 1e-37  # scale below 2^-126
+    x[2, 5] = math.inf
+    x[3, 77] = math.nan
+    x[4] = 3.3e38
+    x[5] = 1e-34
+    codes, scales = ops_q8.quantize_tokens(x.to(cuda_device), dtype)
+    want, want_scales = ref.quantize_rows(x, dtype)
+    assert _same(scales, want_scales) and _same(codes, want)
+    assert scales[:2].tolist() == [0.0, 0.0] and scales[2:4].isnan().all()
+    assert not codes[:4].float().any() and scales[4:].isfinite().all()
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize(("rows", "dim"), [(1, 8), (3, 264), (9, 2048), (2, 5000), (2, 16384)])
+@pytest.mark.parametrize("residual", [False, True])
+@pytest.mark.parametrize("weight", [False, True])
+def test_rms_norm_quantize(cuda_device, dtype, rows, dim, residual, weight):
+    x = _normal((rows, dim), dim, 2.0)
+    r = _normal((rows, dim), dim + 1, 3.0) if residual else None
+    w = _normal((dim,), dim + 2, 0.3) if weight else None
+    codes, scales, hidden = ops_q8.rms_norm_quantize(
+        x.to(cuda_device), None if w is None else w.to(cuda_device), 1e-5,
+        residual=None if r is None else r.to(cuda_device), dtype=dtype,
+        weight_offset=1.0 if weight else 0.0)
+    h, y = ref.rms_norm(x, w, 1e-5, r, 1.0)
+    assert torch.equal(hidden.cpu(), h)
+    # sum of squares: up to 42 fp32 additions in a row, halved by the root; rsqrtf 2 ulp; three
+    # products and the weight's sum: below 2e-6 of the value
+    want = y.abs().amax(-1) / ref.TOP[dtype]
+    assert bool(((scales.cpu().double() - want).abs() <= 3e-6 * want).all())
+    c = codes.cpu().double()
+    off = (c - y / want[:, None]).abs()
+    half = 0.5 if dtype == INT8 else torch.clamp((y / want[:, None]).abs() * 2.0**-4, min=2.0**-10)
+    assert bool((off <= half + 6e-6 * c.abs() + 1e-6).all())
+
+
+def test_rms_norm_quantize_in_place_and_strided(cuda_device):
+    wide = _normal((6, 3 * 256), 5).to(cuda_device)
+    x, r = wide[:, 256:512], _normal((6, 256), 6).to(cuda_device)
+    expect = ops_q8.rms_norm_quantize(x.contiguous(), residual=r.clone())
+    before = wide.clone()
+    codes, scales, hidden = ops_q8.rms_norm_quantize(x, residual=r, hidden=r)
+    assert hidden is r
+    for got, want in zip((codes, scales, hidden), expect):
+        assert torch.equal(got, want)
+    assert torch.equal(wide, before)
+    three = ops_q8.quantize_tokens(r.view(2, 3, 256))
+    two = ops_q8.quantize_tokens(r)
+    assert three[0].shape == (2, 3, 256) and three[1].shape == (2, 3)
+    assert torch.equal(three[0].view(6, 256), two[0]) and torch.equal(three[1].view(6), two[1])
+
+
+# ---------------------------------------------------------------- product
+def _product(m, n, k, seed, bias, device):
+    g = _gen(seed)
+    x = torch.randint(-127, 128, (m, k), generator=g, dtype=torch.int8)
+    w = torch.randint(-127, 128, (n, k), generator=g, dtype=torch.int8)
+    sx = torch.rand(m, generator=g) * 0.1
+    sw = torch.rand(n, generator=g) * 0.01
+    b = _normal((n,), seed, 3.0) if bias else None
+    return [t if t is None else t.to(device) for t in (x, sx, w, sw, b)], ref.linear(x, sx, w, sw, b)
+
+
+def _check_product(out, exact, bias):
+    # three fp32 roundings of the scaled sum, one of the sum with the bias, one to bf16
+    top = exact.abs() + (0 if bias is None else 2 * bias.cpu().double().abs())
+    off = (out.cpu().double() - exact).abs()
+    assert bool((off <= 2.0**-8 * exact.abs() + 4 * 2.0**-24 * top * (1 + 2.0**-8)).all()), float(off.max())
+
+
+@pytest.mark.parametrize(("m", "n", "k"), [
+    (1, 8, 16), (1, 4096, 4096), (2, 136, 128), (7, 1000, 272), (16, 640, 2064), (17, 384, 1040),
+    (33, 256, 512), (64, 128, 144), (65, 264, 384), (126, 520, 1024), (129, 128, 256),
+    (256, 512, 768), (257, 256, 128), (300, 1000, 400), (513, 264, 2048), (1025, 768, 640),
+])
+@pytest.mark.parametrize("bias", [False, True])
+def test_linear_int8(cuda_device, m, n, k, bias):
+    args, exact = _product(m, n, k, m + n + k, bias, cuda_device)
+    _check_product(ops_q8.linear_int8(*args), exact, args[4])
+    ops.device_status()
+
+
+def test_linear_int8_extremes_and_strides(cuda_device):
+    # the largest sums that 16384 codes give, beyond fp32's whole numbers
+    k = 16384
+    x = torch.full((3, k), 127, dtype=torch.int8, device=cuda_device)
+    w = torch.full((8, k), -127, dtype=torch.int8, device=cuda_device)
+    one = torch.ones(8, device=cuda_device)
+    out = ops_q8.linear_int8(x, one[:3].contiguous(), w, one)
+    assert bool((out.float() == torch.tensor(-127.0 * 127 * k).to(BF16).float()).all())
+    # a slice of wider codes, weights and outputs
+    for m in (5, 300):
+        args, exact = _product(m, 264, 512, m, True, cuda_device)
+        xw = torch.zeros((m, 1024), dtype=torch.int8, device=cuda_device)
+        ww = torch.zeros((264, 528), dtype=torch.int8, device=cuda_device)
+        xw[:, 512:] = args[0]
+        ww[:, 16:] = args[2]
+        wide = torch.full((m, 800), 7.0, dtype=BF16, device=cuda_device)
+        ops_q8.linear_int8(xw[:, 512:], args[1], ww[:, 16:], args[3], args[4], wide[:, 8:272])
+        _check_product(wide[:, 8:272], exact, args[4])
+        assert bool((wide[:, :8] == 7).all()) and bool((wide[:, 272:] == 7).all())
+    # scales of NaN and 0 stay in their rows and columns
+    args, _ = _product(20, 128, 128, 1, False, cuda_device)
+    args[1][3], args[1][4], args[3][7] = math.nan, 0.0, math.nan
+    out = ops_q8.linear_int8(*args)
+    assert out[3].isnan().all() and out[:, 7].isnan().all()
+    rest = torch.ones(out.shape, dtype=torch.bool, device=cuda_device)
+    rest[3] = False
+    rest[:, 7] = False
+    assert out[rest].isfinite().all() and not out[4, :7].any()
+
+
+# ---------------------------------------------------------------- cache
+def _cache(batch, most, heads, dim, block, dtype, seed, device, pool=0):
+    """A cache with random codes and scales everywhere, and a table of distinct blocks."""
+    g = _gen(seed)
+    per = max(1, -(-most // block))
+    blocks = batch * per + 1 + pool
+    table = torch.randperm(blocks, generator=g)[: batch * per].view(batch, per).to(torch.int32)
+    codes = [torch.randint(-127, 128, (blocks, heads, block, dim), generator=g) for _ in range(2)]
+    if dtype == INT8:
+        codes = [c.to(INT8) for c in codes]
+    else:
+        codes = [(c * 3.5).clamp(-448, 448).to(E4M3) for c in codes]
+    scales = [(torch.rand((blocks, heads), generator=g) + 0.5) * 0.02 for _ in range(2)]
+    cpu = ops_q8.KVCache(*codes, *scales)
+    return cpu, ops_q8.KVCache(*(t.to(device) for t in cpu)), table
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("block", [16, 32, 64, 128])
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize(("held", "new"), [
+    ([0], [1]), ([5, 64, 127], [1, 1, 1]), ([0, 63, 130, 17], [200, 1, 0, 47]),
+    ([128, 1], [128, 129]),
+])
+def test_cache_write_and_read(cuda_device, dtype, block, dim, held, new):
+    heads, batch = 3, len(held)
+    most = max(h + n for h, n in zip(held, new))
+    cpu, cache, table = _cache(batch, most, heads, dim, block, dtype, block + dim, cuda_device)
+    rows = sum(new)
+    k, v = _normal((rows + 2, heads, dim), 1, 0.5), _normal((rows + 2, heads, dim), 2, 3.0)
+    k[0] *= 20  # a token that makes the scales of its block grow
+    starts = torch.tensor([0] + [sum(new[: i + 1]) for i in range(batch)], dtype=torch.int32)
+    lengths = torch.tensor(held, dtype=torch.int32)
+    uniform = len(set(new)) == 1
+    if uniform:
+        k, v, dev_starts = k[:rows], v[:rows], None
+    else:
+        dev_starts = starts.to(cuda_device)  # two rows behind the last sequence
+    ops_q8.kv_cache_write(cache, k.to(cuda_device), v.to(cuda_device), table.to(cuda_device),
+                          lengths.to(cuda_device), dev_starts)
+    ops.device_status()
+    want = []
+    for c, s, x in ((cpu.k_codes, cpu.k_scales, k), (cpu.v_codes, cpu.v_scales, v)):
+        want.append(ref.cache_write(c, s, x[:rows], table, lengths, starts))
+    for i in range(2):
+        assert torch.equal(cache[2 + i].cpu(), want[i][1])
+        assert _same(cache[i], want[i][0])  # every block, the untouched ones too
+    after = lengths + torch.tensor(new, dtype=torch.int32)
+    tokens = most + 3
+    got = ops_q8.kv_cache_read(cache, table.to(cuda_device), after.to(cuda_device), tokens)
+    ops.device_status()
+    for i in range(2):
+        for b in range(batch):
+            n = int(after[b])
+            y = ref.cached(want[i][0], want[i][1], table[b], n).transpose(0, 1)
+            assert torch.equal(got[i][b, :n].cpu(), y.float().to(BF16))
+            assert not got[i][b, n:].any()
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_cache_write_not_finite_and_zero(cuda_device, dtype):
+    cpu, cache, table = _cache(2, 64, 2, 64, 32, dtype, 9, cuda_device)
+    k, v = _normal((2, 2, 64), 1), torch.zeros((2, 2, 64), dtype=BF16)
+    k[0, 1, 3] = math.nan
+    k[1, 0, 9] = -math.inf
+    lengths = torch.tensor([0, 40], dtype=torch.int32)
+    args = (table.to(cuda_device), lengths.to(cuda_device))
+    ops_q8.kv_cache_write(cache, k.to(cuda_device), v.to(cuda_device), *args)
+    for i, x in enumerate((k, v)):
+        codes, scales = ref.cache_write(cpu[i], cpu[2 + i], x, table, lengths)
+        assert _same(cache[2 + i], scales) and _same(cache[i], codes)
+    assert cache.k_scales[table[0, 0].long(), 1].isnan() and cache.k_scales[table[1, 1].long(), 0].isnan()
+    assert float(cache.v_scales[table[0, 0].long(), 0]) == 0.0
+    # a block that held a NaN stays one
+    ops_q8.kv_cache_write(cache, _normal((2, 2, 64), 5).to(cuda_device), v.to(cuda_device),
+                          args[0], args[1] + 1)
+    assert cache.k_scales[table[0, 0].long(), 1].isnan()
+
+
+def test_cache_write_strides(cuda_device):
+    cpu, cache, table = _cache(2, 100, 4, 128, 64, INT8, 4, cuda_device)
+    qkv = _normal((20, 3, 4, 128), 8)
+    lengths = torch.tensor([60, 3], dtype=torch.int32)
+    dev = qkv.to(cuda_device)
+    ops_q8.kv_cache_write(cache, dev[:, 1], dev[:, 2], table.to(cuda_device), lengths.to(cuda_device))
+    for i in range(2):
+        codes, scales = ref.cache_write(cpu[i], cpu[2 + i], qkv[:, 1 + i], table, lengths)
+        assert torch.equal(cache[2 + i].cpu(), scales) and _same(cache[i], codes)
+
+
+# ---------------------------------------------------------------- attention
+def _attend(cuda_device, held, new, heads, group, dim, block, dtype, *, causal=True, seed=0,
+            scale=None, spread=1.0, packed=None):
+    batch = len(held)
+    cpu, cache, table = _cache(batch, max(max(held), 1), heads, dim, block, dtype, seed, cuda_device)
+    if spread != 1.0:  # scales that differ between blocks by powers of `spread`
+        power = torch.randint(-2, 3, cpu.v_scales.shape, generator=_gen(seed + 7)).float()
+        cpu.v_scales.mul_(spread**power)
+        cache.v_scales.copy_(cpu.v_scales)
+    packed = len(set(new)) > 1 if packed is None else packed
+    extra = 3 if packed else 0
+    rows = sum(new)
+    q = _normal((rows + extra, heads * group, dim), seed + 1, 2.0)
+    starts = torch.tensor([0] + [sum(new[: i + 1]) for i in range(batch)], dtype=torch.int32)
+    lengths = torch.tensor(held, dtype=torch.int32)
+    out = torch.full(q.shape, 5.0, dtype=BF16, device=cuda_device)
+    got = ops_q8.kv_cache_attention(
+        q.to(cuda_device), cache, table.to(cuda_device), lengths.to(cuda_device),
+        starts.to(cuda_device) if packed else None, causal=causal, scale=scale, out=out)
+    ops.device_status()
+    assert got is out and bool((out[rows:] == 5).all())
+    want, weight, reach = ref.attention(q[:rows], cpu.k_codes, cpu.v_codes, cpu.k_scales,
+                                        cpu.v_scales, table, lengths, starts, causal=causal,
+                                        scale=scale)
+    return out[:rows].cpu(), want, weight, reach
+
+
+def _check_attention(got, want, weight, reach):
+    # probabilities and the result are rounded to bf16 (2^-8 of each term); a score's fp32 sum of
+    # up to 128 products and its scaling move it by at most 132 * 2^-24 of the sum of magnitudes,
+    # numerator and denominator alike; exponentials 2^-21
+    dim = want.shape[-1]
+    per = 2.0**-8 * 1.01 + 2 * ((dim + 4) * 2.0**-24 * reach + 2.0**-20)
+    off = (got.double() - want).abs()
+    limit = per * weight + 2.0**-8 * (want.abs() + per * weight) + 1e-30
+    assert got.isfinite().all()
+    assert bool((off <= limit).all()), float((off / limit).max())
+
+
+SMALL = [  # held (with the new tokens), new, cache heads, group
+    ([1], [1], 1, 1),
+    ([1, 64, 65, 300], [1, 1, 1, 1], 2, 4),
+    ([37, 129], [1, 1], 3, 5),
+    ([500], [1], 1, 8),
+    ([0, 70], [1, 1], 2, 2),
+    ([260, 33], [2, 2], 2, 8),
+    ([90, 200, 1], [3, 5, 1], 2, 3),
+    ([40, 0, 513], [1, 0, 2], 2, 7),
+    ([700], [1], 1, 16),
+    ([2, 90], [4, 4], 2, 2),
+]
+
+
+@pytest.mark.parametrize("case", SMALL, ids=range(len(SMALL)))
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize(("dim", "block"), [(128, 64), (128, 16), (64, 128), (64, 16), (128, 128),
+                                            (64, 32)])
+def test_attention_few_rows(cuda_device, case, dtype, dim, block):
+    held, new, heads, group = case
+    _check_attention(*_attend(cuda_device, held, new, heads, group, dim, block, dtype,
+                              causal=block != 32, seed=dim + block))
