@@ -559,6 +559,558 @@ __global__ void __launch_bounds__(Q8D_THREADS, 1)
   }
 }
 
+// ---------------------------------------------------------------- many query rows
+// tcgen05: an item is up to two tiles of 128 query rows (128 / group tokens x group heads each, so
+// that grouped heads share the keys' tile), in ping-pong over blocks of 128 keys as in the dense
+// kernel; the ring's K and V blocks are written by a warpgroup that reads codes and stores exact
+// bf16 in the layout TMA would (128-byte swizzle). Bound by the exponentials and the conversion.
+//   warp 0        Q tiles by TMA, one item ahead of the first product that needs them
+//   warp 1        tensor memory, products
+//   warps 2..9    softmax (two warps a lane quarter, 64 of the block's keys each)
+//   warps 10..13  codes -> bf16: each thread keeps the next block's codes in registers
+// Tensor memory as in the dense kernel: S_A, S_B, O_A, O_B. All roles walk the same run of items;
+// the pipelines' phases go on over items.
+constexpr int Q8P_BN = 128;
+constexpr int Q8P_THREADS = 448;
+
+struct Q8PrefillSmem {
+  static constexpr int HALF = 128 * 64 * 2;  // 128 rows x 64 dims
+  static constexpr int Q_OFF = 0;            // tile t at t * 2 * HALF
+  static constexpr int KV_OFF = 4 * HALF;    // per stage: K 2 halves, V 2 halves
+  static constexpr int STAGE = 4 * HALF;
+  static constexpr int STAGES = 2;
+  static constexpr int X_OFF = KV_OFF + STAGES * STAGE;  // maxima [tile][parity][half][128]
+  static constexpr int L_OFF = X_OFF + 2 * 2 * 2 * 128 * 4;  // sums [tile][half][128]
+  static constexpr int SC_OFF = L_OFF + 2 * 2 * 128 * 4;
+  static constexpr int SC = 80;  // a stage's scales of 8 groups of 16 keys, K then V, and a mask
+  static constexpr int BAR_OFF = SC_OFF + STAGES * SC;
+  // q_full, q_empty, kv_full[2], kv_empty[2], s_full[2], p_full[2], o_full, o_empty,
+  // xbar[4][2][2], lbar[4]
+  static constexpr int NBAR = 2 + 2 * STAGES + 2 + 2 + 2 + 16 + 4;
+  static constexpr int TOTAL = BAR_OFF + NBAR * 8 + 64 + 1024;
+};
+
+template <int D, int FMT>
+__global__ void __launch_bounds__(Q8P_THREADS, 1)
+    attention_q8_prefill_kernel(const __grid_constant__ CUtensorMap map_q, const Q8Attn a) {
+  using L = Q8PrefillSmem;
+  using Work = Q8Work<Q8P_BN>;
+  constexpr int NH = D / 64;
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) &
+                                             ~static_cast<uintptr_t>(1023));
+  uint64_t* bars = reinterpret_cast<uint64_t*>(smem + L::BAR_OFF);
+  uint64_t* q_full = bars;
+  uint64_t* q_empty = bars + 1;
+  uint64_t* kv_full = bars + 2;
+  uint64_t* kv_empty = kv_full + L::STAGES;
+  uint64_t* s_full = kv_empty + L::STAGES;
+  uint64_t* p_full = s_full + 2;
+  uint64_t* o_full = p_full + 2;
+  uint64_t* o_empty = o_full + 1;
+  uint64_t* xbar = o_empty + 1;  // [quarter][tile][parity]
+  uint64_t* lbar = xbar + 16;    // [quarter]
+  int64_t* s_run = reinterpret_cast<int64_t*>(bars + L::NBAR);  // u0, u1, at
+  int* s_item = reinterpret_cast<int*>(s_run + 3);              // b, tile, head
+  volatile int* abort_flag = s_item + 3;
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(s_item + 4);
+  float* xmax = reinterpret_cast<float*>(smem + L::X_OFF);
+  float* xsum = reinterpret_cast<float*>(smem + L::L_OFF);
+
+  const int warp = warp_id();
+  const int lane = static_cast<int>(lane_id());
+  griddep_wait();
+  Work w(a);
+  if (warp == 0) {
+    const int64_t total = w.total();
+    const int64_t run = q8_run_units(a, total);
+    const int64_t u0 = blockIdx.x * run;
+    int64_t in = 0;
+    if (u0 < total) in = w.seek(u0);
+    if (lane == 0) {
+      s_run[0] = u0;
+      s_run[1] = u0 + run < total ? u0 + run : total;
+      s_run[2] = in;
+      s_item[0] = w.b;
+      s_item[1] = w.tile;
+      s_item[2] = w.head;
+      *abort_flag = 0;
+    }
+  } else if (warp == 1) {
+    if (lane == 0) {
+      mbar_init(q_full, 1);
+      mbar_init(q_empty, 1);
+      for (int i = 0; i < L::STAGES; ++i) {
+        mbar_init(&kv_full[i], 4);
+        mbar_init(&kv_empty[i], 1);
+      }
+      for (int t = 0; t < 2; ++t) {
+        mbar_init(&s_full[t], 1);
+        mbar_init(&p_full[t], 8);
+      }
+      mbar_init(o_full, 1);
+      mbar_init(o_empty, 8);
+      for (int i = 0; i < 16; ++i) mbar_init(&xbar[i], 64);
+      for (int i = 0; i < 4; ++i) mbar_init(&lbar[i], 64);
+      fence_barrier_init();
+    }
+    __syncwarp();
+    tmem_alloc(tmem_slot, 512);
+    tmem_relinquish();
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = *tmem_slot;
+  griddep_launch();
+  int64_t left = s_run[1] - s_run[0];
+  int at = static_cast<int>(s_run[2]);
+  if (left > 0) {
+    w.enter(s_item[0]);
+    w.tile = s_item[1];
+    w.head = s_item[2];
+    w.units = Work::units_of(a, w.count, w.len, w.tile);
+  }
+  const int tile_q = a.tile_tokens >> 1;  // tokens of a 128-row tile
+
+  if (warp < 2) {
+    if (warp == 0 && lane == 0) {
+      // ---- queries
+      int items = 0;
+      while (left > 0) {
+        const int n = static_cast<int>(left < w.units - at ? left : w.units - at);
+        if (Work::keys(a, w.count, w.len, w.tile) > 0) {
+          const int tok0 = w.tile * a.tile_tokens;
+          const int ntile = w.count - tok0 > tile_q ? 2 : 1;
+          if (!mbar_wait(q_empty, (items & 1) ^ 1u, abort_flag)) break;
+          mbar_expect_tx(q_full, static_cast<uint32_t>(ntile * D * 2 * a.group * tile_q));
+          for (int t = 0; t < ntile; ++t)
+            for (int h = 0; h < NH; ++h)
+              tma_load_3d(smem + L::Q_OFF + (t * 2 + h) * L::HALF, &map_q, q_full, h * 64,
+                          w.head * a.group, static_cast<int>(w.first) + tok0 + t * tile_q);
+          ++items;
+        }
+        left -= n;
+        at = 0;
+        if (left > 0) w.next();
+      }
+      if (*abort_flag && items > 0) {  // copies in flight land (bounded)
+        const uint64_t t0 = global_ns();
+        while (!mbar_try_wait(q_full, (items - 1) & 1) && global_ns() - t0 < 200000000ull) {
+        }
+      }
+    } else if (warp == 1 && lane == 0) {
+      // ---- products
+      constexpr uint32_t idesc_s = idesc_bf16(128, 128);
+      constexpr uint32_t idesc_o = idesc_bf16(128, D) | (1u << 16);  // V: MN-major
+      auto s_mma = [&](int t, int jb) {
+        const uint32_t sq = smem_u32(smem + L::Q_OFF + t * 2 * L::HALF);
+        const uint32_t sk = smem_u32(smem + L::KV_OFF + (jb % L::STAGES) * L::STAGE);
+#pragma unroll
+        for (int kk = 0; kk < D / 16; ++kk) {
+          const uint32_t off = (kk >> 2) * L::HALF + (kk & 3) * 32;
+          umma_bf16(tmem + t * 128, sdesc_k128(sq + off), sdesc_k128(sk + off), idesc_s,
+                    kk > 0 ? 1u : 0u);
+        }
+        umma_commit(&s_full[t]);
+      };
+      auto pv_mma = [&](int t, int jb, bool first) {
+        const uint32_t sv =
+            smem_u32(smem + L::KV_OFF + (jb % L::STAGES) * L::STAGE + 2 * L::HALF);
+#pragma unroll
+        for (int kk = 0; kk < Q8P_BN / 16; ++kk)
+          umma_bf16_ts(tmem + 256 + t * 128, tmem + t * 128 + kk * 8 + (kk >= 4 ? 32 : 0),
+                       sdesc_mn128(sv + kk * 2048, L::HALF), idesc_o,
+                       (!first || kk > 0) ? 1u : 0u);
+      };
+      int items = 0, jb = 0;
+      int cnt[2] = {0, 0};  // blocks that a tile has been given
+      bool ok = true;
+      while (left > 0 && ok) {
+        const int n = static_cast<int>(left < w.units - at ? left : w.units - at);
+        if (Work::keys(a, w.count, w.len, w.tile) > 0) {
+          const int ntile = w.count - w.tile * a.tile_tokens > tile_q ? 2 : 1;
+          ok = mbar_wait(q_full, items & 1, abort_flag) &&
+               mbar_wait(&kv_full[jb % L::STAGES], (jb / L::STAGES) & 1, abort_flag);
+          if (!ok) break;
+          tc_fence_after();
+          for (int t = 0; t < ntile; ++t) s_mma(t, jb);
+          for (int j = 0; j < n && ok; ++j, ++jb) {
+            const bool more = j + 1 < n;
+            for (int t = 0; t < ntile; ++t) {
+              ok = mbar_wait(&p_full[t], cnt[t] & 1, abort_flag);
+              // the previous item's output has been read
+              if (ok && j == 0 && t == 0) ok = mbar_wait(o_empty, (items & 1) ^ 1u, abort_flag);
+              if (!ok) break;
+              ++cnt[t];
+              tc_fence_after();
+              pv_mma(t, jb, j == 0);
+              if (t == ntile - 1) umma_commit(&kv_empty[jb % L::STAGES]);
+              if (more) {
+                if (t == 0) {
+                  ok = mbar_wait(&kv_full[(jb + 1) % L::STAGES], ((jb + 1) / L::STAGES) & 1,
+                                 abort_flag);
+                  if (!ok) break;
+                  tc_fence_after();
+                }
+                s_mma(t, jb + 1);
+              }
+            }
+          }
+          if (!ok) break;
+          umma_commit(q_empty);
+          umma_commit(o_full);
+          ++items;
+        }
+        left -= n;
+        at = 0;
+        if (left > 0) w.next();
+      }
+      // all issued products end before tensor memory is released (bounded)
+      if (!ok) {
+        umma_commit(o_full);
+        const uint64_t t0 = global_ns();
+        while (!mbar_try_wait(o_full, items & 1) && global_ns() - t0 < 200000000ull) {
+        }
+      }
+    }
+    __syncwarp();
+  } else if (warp >= 10) {
+    // ---- codes to bf16
+    constexpr int PER_ROW = D / 16;                 // 16-code runs of a token
+    constexpr int ROWS = 32 / PER_ROW;              // tokens a warp reads at once
+    constexpr int NV = Q8P_BN / (4 * ROWS);         // its reads of K (and of V) a block
+    const int cw = warp - 10;
+    // a quarter warp's 16-byte stores fall on even chunks of one token and odd ones of the next
+    const int run16 = D == 128 ? (lane & 3) + ((lane >> 3) & 1) * 4 : lane & 3;
+    const int row = cw * ROWS + (D == 128 ? ((lane >> 2) & 1) + (lane >> 4) * 2 : lane >> 2);
+    uint32_t dst0 = smem_u32(smem + L::KV_OFF) + (run16 >> 2) * L::HALF + row * 128;
+    const uint32_t c0 = dst0 + ((((run16 & 3) * 2) ^ (row & 7)) << 4);
+    const uint32_t c1 = dst0 + ((((run16 & 3) * 2 + 1) ^ (row & 7)) << 4);
+    int n = 0;        // units of the item that are left to look up
+    bool none = false;  // an item without keys has one unit and no block
+    auto settle = [&]() {
+      // the cursor stands on a block that has keys, or left == 0
+      while (left > 0) {
+        n = static_cast<int>(left < w.units - at ? left : w.units - at);
+        none = Work::keys(a, w.count, w.len, w.tile) == 0;
+        if (!none) return;
+        left -= n;
+        at = 0;
+        if (left > 0) w.next();
+      }
+    };
+    auto step = [&]() {
+      ++at;
+      --left;
+      if (--n == 0) {
+        at = 0;
+        if (left > 0) {
+          w.next();
+          settle();
+        }
+      }
+    };
+    // lanes 0..7: where the cursor's 16-key groups are, and their scales
+    int there = -1;
+    float ks = 0.0f, vs = 0.0f;
+    auto look = [&]() {
+      there = -1;
+      ks = vs = 0.0f;
+      if (left > 0 && lane < 8) {
+        const int key = at * Q8P_BN + lane * 16;
+        if (key < Work::keys(a, w.count, w.len, w.tile)) {
+          const int page = a.table[static_cast<int64_t>(w.b) * a.ld_table + key / a.block];
+          if (page >= 0 && page < a.num_blocks) {
+            const int unit = page * a.heads + w.head;
+            there = unit * a.block + key % a.block;
+            ks = a.scales[0][unit] * a.scale_log2;
+            vs = a.scales[1][unit];
+          } else {
+            q8_flag(1);
+          }
+        }
+      }
+    };
+    uint4 raw[2][NV];
+    auto fetch = [&](int kv, int i) {
+      // rows of read i: group (i * 4 * ROWS + row) / 16, the same for the whole warp
+      const int r = i * 4 * ROWS + row;
+      const int base = __shfl_sync(0xffffffffu, there, r >> 4);
+      raw[kv][i] = make_uint4(0, 0, 0, 0);
+      if (base >= 0)
+        raw[kv][i] = __ldg(reinterpret_cast<const uint4*>(
+            a.codes[kv] + static_cast<int64_t>(base + (r & 15)) * D + run16 * 16));
+    };
+    settle();
+    look();
+    int todo = left > 0;
+    if (todo) {
+#pragma unroll
+      for (int i = 0; i < NV; ++i) {
+        fetch(0, i);
+        fetch(1, i);
+      }
+    }
+    int jb = 0;
+    while (todo) {
+      const float ks_now = ks, vs_now = vs;
+      const unsigned groups = __ballot_sync(0xffffffffu, there >= 0) & 0xFFu;
+      step();
+      look();
+      todo = left > 0;
+      const int stage = jb % L::STAGES;
+      if (!__all_sync(0xffffffffu, mbar_wait(&kv_empty[stage], ((jb / L::STAGES) & 1) ^ 1u,
+                                             abort_flag)))
+        break;
+#pragma unroll
+      for (int kv = 0; kv < 2; ++kv)
+#pragma unroll
+        for (int i = 0; i < NV; ++i) {
+          const uint32_t off = stage * L::STAGE + kv * 2 * L::HALF + i * 4 * ROWS * 128;
+          const uint4 v = raw[kv][i];
+          asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(c0 + off),
+                       "r"(q8_pair<FMT>(v.x, 0u, 0, 1)), "r"(q8_pair<FMT>(v.x, 0u, 2, 3)),
+                       "r"(q8_pair<FMT>(v.y, 0u, 0, 1)), "r"(q8_pair<FMT>(v.y, 0u, 2, 3))
+                       : "memory");
+          asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(c1 + off),
+                       "r"(q8_pair<FMT>(v.z, 0u, 0, 1)), "r"(q8_pair<FMT>(v.z, 0u, 2, 3)),
+                       "r"(q8_pair<FMT>(v.w, 0u, 0, 1)), "r"(q8_pair<FMT>(v.w, 0u, 2, 3))
+                       : "memory");
+          if (todo) fetch(kv, i);
+        }
+      if (cw == 0) {
+        float* sc = reinterpret_cast<float*>(smem + L::SC_OFF + stage * L::SC);
+        if (lane < 8) {
+          sc[lane] = ks_now;
+          sc[8 + lane] = vs_now;
+        }
+        if (lane == 0) reinterpret_cast<unsigned*>(sc)[16] = groups;
+      }
+      fence_proxy_async_smem();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&kv_full[stage]);
+      ++jb;
+    }
+  } else {
+    // ---- softmax
+    const int quarter = warp & 3;
+    const int half = (warp - 2) >> 2;
+    const int row = quarter * 32 + lane;
+    const uint32_t lane_base = static_cast<uint32_t>(quarter * 32) << 16;
+    const int row_tok = row / a.group, row_head = row % a.group;
+    const bool in_row = row < tile_q * a.group;
+    int items = 0, jb = 0, piece = 0;
+    int cnt[2] = {0, 0};
+    bool ok = true;
+    while (left > 0 && ok) {
+      const int n = static_cast<int>(left < w.units - at ? left : w.units - at);
+      const bool whole = n == w.units;
+      const int keys = Work::keys(a, w.count, w.len, w.tile);
+      const int tok0 = w.tile * a.tile_tokens;
+      const int ntile = w.count - tok0 > tile_q ? 2 : 1;
+      int limit[2], least[2];  // keys that this row sees; the least of the warp's rows
+#pragma unroll
+      for (int t = 0; t < 2; ++t) {
+        const int tok = tok0 + t * tile_q + row_tok;
+        const bool live = in_row && tok < w.count;
+        // rows of no query are computed with whatever is there and not stored
+        limit[t] = !live ? 0x7fffffff
+                         : a.causal ? max(0, min(keys, w.len - w.count + tok + 1)) : keys;
+        least[t] = __reduce_min_sync(0xffffffffu, limit[t]);
+      }
+      float m_run[2] = {-INFINITY, -INFINITY};
+      float l_run[2] = {0.0f, 0.0f};
+      const int blocks = keys > 0 ? n : 0;
+      for (int j = 0; j < blocks && ok; ++j, ++jb) {
+        const int stage = jb % L::STAGES;
+        const float* sc = reinterpret_cast<const float*>(smem + L::SC_OFF + stage * L::SC);
+        const int key0 = (at + j) * Q8P_BN + half * 64;
+        ok = __all_sync(0xffffffffu,
+                        mbar_wait(&kv_full[stage], (jb / L::STAGES) & 1, abort_flag));
+        if (!ok) break;
+        const volatile float* ks = sc + half * 4;  // of the half's four groups of 16 keys
+        const volatile float* vs = ks + 8;
+        const unsigned groups = (reinterpret_cast<const unsigned*>(sc)[16] >> (half * 4)) & 15u;
+        for (int t = 0; t < ntile; ++t) {
+          ok = __all_sync(0xffffffffu, mbar_wait(&s_full[t], cnt[t] & 1, abort_flag));
+          if (!ok) break;
+          tc_fence_after();
+          const uint32_t s_col = tmem + lane_base + t * 128 + half * 64;
+          uint32_t sr[2][32];
+          tmem_ld32(s_col, sr[0]);
+          tmem_ld32(s_col + 32, sr[1]);
+          tmem_wait_ld();
+          const bool masked = key0 + 64 > least[t] || groups != 15u;  // warp-uniform
+          if (masked) {
+            const int valid = limit[t] - key0;
+#pragma unroll
+            for (int i = 0; i < 64; ++i)
+              if (i >= valid || !((groups >> (i >> 4)) & 1))
+                sr[i >> 5][i & 31] = __float_as_uint(-INFINITY);
+          }
+          float mine = -INFINITY;
+#pragma unroll
+          for (int q = 0; q < 4; ++q) {
+            const uint32_t* v = sr[q >> 1] + (q & 1) * 16;
+            float x = max3f(__uint_as_float(v[0]), __uint_as_float(v[1]), __uint_as_float(v[2]));
+            x = max3f(x, __uint_as_float(v[3]), __uint_as_float(v[4]));
+            x = max3f(x, __uint_as_float(v[5]), __uint_as_float(v[6]));
+            x = max3f(x, __uint_as_float(v[7]), __uint_as_float(v[8]));
+            x = max3f(x, __uint_as_float(v[9]), __uint_as_float(v[10]));
+            x = max3f(x, __uint_as_float(v[11]), __uint_as_float(v[12]));
+            x = max3f(x, __uint_as_float(v[13]), __uint_as_float(v[14]));
+            x = fmaxf(x, __uint_as_float(v[15]));
+            // scales are not negative; a masked group stays at -inf whatever its scale is
+            mine = fmaxf(mine, x == -INFINITY ? x : x * ks[q]);
+          }
+          float* xm = xmax + (t * 2 + (cnt[t] & 1)) * 256;
+          xm[half * 128 + row] = mine;
+          uint64_t* xb = &xbar[(quarter * 2 + t) * 2 + (cnt[t] & 1)];
+          mbar_arrive(xb);
+          ok = __all_sync(0xffffffffu, mbar_wait(xb, (cnt[t] >> 1) & 1, abort_flag));
+          if (!ok) break;
+          const float m_blk = fmaxf(mine, xm[(1 - half) * 128 + row]);
+          float alpha = 1.0f;
+          bool rescale = false;
+          if (j > 0) {
+            const bool need = m_blk > m_run[t] + 8.0f;
+            rescale = __any_sync(0xffffffffu, need);
+            if (need) {
+              alpha = ex2_approx(m_run[t] - m_blk);
+              m_run[t] = m_blk;
+              l_run[t] *= alpha;
+            }
+          } else {
+            m_run[t] = m_blk;
+          }
+          const float ref = m_run[t] == -INFINITY ? 0.0f : m_run[t];
+          const uint64_t negm = f2_pack(-ref, -ref);
+          uint64_t lsum2[2] = {f2_pack(0.0f, 0.0f), f2_pack(0.0f, 0.0f)};
+#pragma unroll
+          for (int q8 = 0; q8 < 4; ++q8) {
+            uint32_t packed[8];
+            const uint64_t k2 = f2_pack(ks[q8], ks[q8]), v2 = f2_pack(vs[q8], vs[q8]);
+#pragma unroll
+            for (int u = 0; u < 8; ++u) {
+              const int i = q8 * 8 + u;
+              const uint32_t* v = sr[i >> 4];
+              const int e = (2 * i) & 31;
+              const uint64_t xs =
+                  f2_fma(f2_pack(__uint_as_float(v[e]), __uint_as_float(v[e + 1])), k2, negm);
+              uint64_t ev;
+              if ((ATT_EMU_MASK >> (i & 7)) & 1) {
+                ev = exp2_poly_x2(xs);
+              } else {
+                const float2 xv = f2_unpack(xs);
+                ev = f2_pack(ex2_approx(xv.x), ex2_approx(xv.y));
+              }
+              float2 p2;
+              if (masked) {  // a masked key counts for nothing, also where its scales are NaN
+                const float2 e2 = f2_unpack(ev);
+                const bool in0 = v[e] != __float_as_uint(-INFINITY);
+                const bool in1 = v[e + 1] != __float_as_uint(-INFINITY);
+                ev = f2_pack(in0 ? e2.x : 0.0f, in1 ? e2.y : 0.0f);
+                p2 = f2_unpack(f2_mul(ev, v2));
+                p2.x = in0 ? p2.x : 0.0f;
+                p2.y = in1 ? p2.y : 0.0f;
+              } else {
+                p2 = f2_unpack(f2_mul(ev, v2));
+              }
+              lsum2[u & 1] = f2_add(lsum2[u & 1], ev);
+              packed[u] = pack_bf16x2(p2.x, p2.y);
+            }
+            tmem_st8(s_col + q8 * 8, packed);
+          }
+          const float2 ls = f2_unpack(f2_add(lsum2[0], lsum2[1]));
+          l_run[t] += ls.x + ls.y;
+          if (rescale) {
+            const uint32_t o_col = tmem + lane_base + 256 + t * 128 + half * (D / 2);
+#pragma unroll 1
+            for (int c = 0; c < D / 64; ++c) {
+              uint32_t o[32];
+              tmem_ld32(o_col + c * 32, o);
+              tmem_wait_ld();
+#pragma unroll
+              for (int i = 0; i < 32; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * alpha);
+              tmem_st32(o_col + c * 32, o);
+            }
+          }
+          tmem_wait_st();
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&p_full[t]);
+          ++cnt[t];
+        }
+      }
+      if (!ok) break;
+      if (blocks > 0) {
+        for (int t = 0; t < ntile; ++t) xsum[(t * 2 + half) * 128 + row] = l_run[t];
+        mbar_arrive(&lbar[quarter]);
+        ok = __all_sync(0xffffffffu, mbar_wait(&lbar[quarter], items & 1, abort_flag) &&
+                                         mbar_wait(o_full, items & 1, abort_flag));
+        if (!ok) break;
+        tc_fence_after();
+      }
+      const int slot = 2 * static_cast<int>(blockIdx.x) + (piece > 0 ? 1 : 0);
+      for (int t = 0; t < ntile; ++t) {
+        const int tok = tok0 + t * tile_q + row_tok;
+        const bool store = in_row && tok < w.count;
+        const float sum = blocks > 0 ? l_run[t] + xsum[(t * 2 + 1 - half) * 128 + row] : 0.0f;
+        const float inv = m_run[t] == -INFINITY ? 1.0f : 1.0f / sum;
+        const int64_t part = static_cast<int64_t>(slot) * a.tile_rows + t * tile_q * a.group + row;
+        if (!whole && store && half == 0) {
+          a.part_ml[part * 2] = m_run[t];
+          a.part_ml[part * 2 + 1] = sum;
+        }
+        const uint32_t o_col = tmem + lane_base + 256 + t * 128 + half * (D / 2);
+#pragma unroll 1
+        for (int c = 0; c < D / 64; ++c) {
+          uint32_t o[32];
+          if (blocks > 0) {
+            tmem_ld32(o_col + c * 32, o);
+            tmem_wait_ld();
+          } else {
+#pragma unroll
+            for (int i = 0; i < 32; ++i) o[i] = 0;
+          }
+          const int col = half * (D / 2) + c * 32;
+          if (store && whole) {
+            uint32_t w16[16];
+#pragma unroll
+            for (int i = 0; i < 16; ++i)
+              w16[i] = pack_bf16x2(__uint_as_float(o[2 * i]) * inv, __uint_as_float(o[2 * i + 1]) * inv);
+            store_row32(a.out + (w.first + tok) * a.ld_out +
+                            static_cast<int64_t>(w.head * a.group + row_head) * a.hs_out + col,
+                        w16, 32);
+          } else if (store) {
+            uint4* dst = reinterpret_cast<uint4*>(a.part_o + part * D + col);
+#pragma unroll
+            for (int i = 0; i < 8; ++i)
+              dst[i] = make_uint4(o[4 * i], o[4 * i + 1], o[4 * i + 2], o[4 * i + 3]);
+          }
+        }
+      }
+      if (blocks > 0) {
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(o_empty);
+        ++items;
+      }
+      left -= n;
+      at = 0;
+      ++piece;
+      if (left > 0) w.next();
+    }
+  }
+  tc_fence_before();
+  __syncthreads();
+  if (warp == 1) {
+    tc_fence_after();
+    tmem_dealloc(tmem, 512);
+  }
+}
+
 // ---------------------------------------------------------------- cut items
 // CTA c looks at the border between the runs c and c + 1. Where it is the first border inside an
 // item, it adds that item's pieces: the last piece of run c, then the first piece of each run up

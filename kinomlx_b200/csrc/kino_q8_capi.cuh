@@ -178,7 +178,24 @@ kino_status launch_q8_attention(const kino_q8_cache* c, kino::Q8Attn& a, int dec
                                 cudaStream_t stream) {
   if (decode_tiles == 1) return launch_q8_decode<D, 1, FMT>(c, a, stream);
   if (decode_tiles == 2) return launch_q8_decode<D, 2, FMT>(c, a, stream);
-  return fail(KINO_ENOTSUPPORTED, "kino_q8_attention: too many query rows");
+  // queries as (rows, heads, dim): a box is 64 dims of the group's heads of 128 / group tokens
+  CUtensorMap mq;
+  const uint64_t dims[3] = {D, static_cast<uint64_t>(a.heads) * a.group,
+                            static_cast<uint64_t>(a.rows.rows)};
+  const uint64_t strides[2] = {static_cast<uint64_t>(a.hs_q), static_cast<uint64_t>(a.ld_q)};
+  const uint32_t box[3] = {64, static_cast<uint32_t>(a.group),
+                           static_cast<uint32_t>(a.tile_tokens / 2)};
+  kino_status st = make_map(&mq, a.q, 3, dims, strides, box);
+  if (st != KINO_OK) return st;
+  using L = kino::Q8PrefillSmem;
+  constexpr auto kernel = kino::attention_q8_prefill_kernel<D, FMT>;
+  st = q8_smem<kernel>(L::TOTAL);
+  if (st != KINO_OK) return st;
+  launch_pdl(kernel, dim3(a.runs), dim3(kino::Q8P_THREADS), L::TOTAL, stream, mq, a);
+  if (a.runs > 1)
+    launch_pdl(kino::attention_q8_combine_kernel<D, kino::Q8P_BN>, dim3(a.runs - 1, 16), dim3(256),
+               0, stream, a);
+  return check_launch("kino_q8_attention");
 }
 
 }  // namespace

@@ -315,3 +315,28 @@ def test_attention_few_rows(cuda_device, case, dtype, dim, block):
     held, new, heads, group = case
     _check_attention(*_attend(cuda_device, held, new, heads, group, dim, block, dtype,
                               causal=block != 32, seed=dim + block))
+
+
+MANY = [  # held (with the new tokens), new, cache heads, group
+    ([17], [17], 1, 1),
+    ([130], [130], 2, 1),
+    ([400], [129], 1, 1),
+    ([300, 70], [40, 40], 2, 3),
+    ([600, 40, 0, 129], [33, 40, 0, 65], 2, 4),
+    ([257], [257], 1, 8),
+    ([1000, 5], [9, 1], 1, 7),
+    ([64, 200], [70, 20], 1, 5),  # more queries than keys: the first see none
+    ([350], [3], 1, 100),
+    ([300], [270], 3, 1),
+]
+
+
+@pytest.mark.parametrize("case", MANY, ids=range(len(MANY)))
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize(("dim", "block", "causal"), [(128, 64, True), (128, 16, True),
+                                                      (64, 128, True), (64, 16, False),
+                                                      (128, 128, False), (64, 32, True)])
+def test_attention_many_rows(cuda_device, case, dtype, dim, block, causal):
+    held, new, heads, group = case
+    _check_attention(*_attend(cuda_device, held, new, heads, group, dim, block, dtype,
+                              causal=causal, seed=dim + block))
