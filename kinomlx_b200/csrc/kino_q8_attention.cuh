@@ -2,9 +2,13 @@
 // for each cache block and head, fp32 scores, statistics and accumulation, G query heads on each
 // K/V head.
 //
-// Codes are exact as bf16, so the products run on bf16 operands that are converted from the codes
-// in registers; a block's K scale multiplies its columns of the scores, its V scale its columns of
-// the probabilities (in fp32, before they are rounded to bf16 for the second product).
+// Codes are exact as bf16 and as f16, so the products run on 16-bit operands converted from the
+// codes in registers. A block's K scale multiplies its columns of the scores. Its V scale vs goes
+// into the exponent: with one reference m for a query row that follows the largest
+// s + log2(vs), the second product's operand is P = exp2(s + log2(vs) - m) = vs exp2(s - m), at
+// most 2^8 whatever the scales are, so it is rounded to f16 (2^-11 of its value; bf16 would give
+// 2^-8), and the row sum takes each group's sum of P over vs. V scales up to
+// 2^-90 count as 0.
 //
 // Work is cut by units of BN keys of one (sequence, query tile, K/V head), the items in that
 // order; every CTA of one resident wave takes an equal run of units, whatever the lengths are
@@ -12,8 +16,11 @@
 // unnormalised partial result with its row maxima and sums; attention_q8_combine adds the pieces
 // of each cut item in a fixed order.
 #pragma once
+#include <type_traits>
+
 #include "kino_attention.cuh"
 #include "kino_q8_common.cuh"
+#include "kino_sol.cuh"
 
 namespace kino {
 
@@ -35,7 +42,7 @@ struct Q8Attn {
   int tile_tokens;  // query tokens of an item
   int tile_rows;    // rows of its partial results (tile_tokens * group, padded)
   int least_units;  // units of a run, at least
-  int runs;         // CTAs
+  int runs;         // CTAs (or CTA pairs)
   float* part_o;    // [2 * runs][tile_rows][D]
   float* part_ml;   // [2 * runs][tile_rows][2]: row maximum (log2 units), row sum
 };
@@ -144,6 +151,8 @@ struct Q8Work {
   }
 };
 
+constexpr float Q8_LEAST_V = 8.0779356694631609e-28f;  // 2^-90
+
 // Units of a run.
 __device__ __forceinline__ int64_t q8_run_units(const Q8Attn& a, int64_t total) {
   const int64_t even = (total + a.runs - 1) / a.runs;
@@ -175,8 +184,9 @@ struct Q8DecodeSmem {
   static constexpr int MERGE = Q8D_WARPS * 8 * NT * LDO * 4;
   static constexpr int ML_OFF = MERGE_OFF + MERGE;      // [warp][8 NT][2]
   static constexpr int SC_OFF = ML_OFF + Q8D_WARPS * 8 * NT * 8;
-  // per stage: scales of the four 16-key groups, K then V, and a word of which groups are there
-  static constexpr int SC = 48;
+  // per stage, of the four 16-key groups: K scales (with the softmax scale), 1 / vs, log2(vs), and
+  // a word of which groups are there
+  static constexpr int SC = 64;
   static constexpr int BAR_OFF = SC_OFF + STAGES * SC;
   static constexpr int TOTAL = BAR_OFF + 2 * STAGES * 8 + 64 + 1024;
 };
@@ -184,7 +194,7 @@ struct Q8DecodeSmem {
 __device__ __forceinline__ void mma_16816(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2,
                                           uint32_t a3, uint32_t b0, uint32_t b1) {
   asm volatile(
-      "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, "
+      "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, "
       "{%0,%1,%2,%3};"
       : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
       : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
@@ -268,14 +278,18 @@ __global__ void __launch_bounds__(Q8D_THREADS, 1)
       for (int u = 0; u < n && ok; u += lot) {
         const int key = (at + u) * Q8D_BN + lane * box;  // this lane's first key
         int row = -1;
-        float ks = 0.0f, vs = 0.0f;
+        float ks = 0.0f, rv = 0.0f, lv = 0.0f;
         if (u + lane / per < n && key < keys) {
           const int page = table[key / a.block];
           if (page >= 0 && page < a.num_blocks) {
             const int unit = page * a.heads + w.head;
             row = unit * a.block + key % a.block;
-            ks = a.scales[0][unit] * a.scale_log2;
-            vs = a.scales[1][unit];
+            // the codes stand in f16 as their value over q8_f16_unit, those of K and of V
+            ks = a.scales[0][unit] * a.scale_log2 * q8_f16_unit<FMT>();
+            const float vs = a.scales[1][unit];
+            const float v = vs <= Q8_LEAST_V ? Q8_LEAST_V : vs;
+            rv = 1.0f / (v * q8_f16_unit<FMT>());
+            lv = log2f(v);
           } else {
             q8_flag(1);
           }
@@ -295,14 +309,16 @@ __global__ void __launch_bounds__(Q8D_THREADS, 1)
           // group g of 16 keys belongs to load g * per / 4
           const int src = l0 + (lane & 3) * per / PAGES;
           const float gk = __shfl_sync(0xffffffffu, ks, src);
-          const float gv = __shfl_sync(0xffffffffu, vs, src);
+          const float gr = __shfl_sync(0xffffffffu, rv, src);
+          const float gl = __shfl_sync(0xffffffffu, lv, src);
           const unsigned groups =
               __ballot_sync(0xffffffffu, lane < PAGES && ((there >> ((lane & 3) * per / PAGES)) & 1));
           if (lane < PAGES) {
             sc[lane] = gk;
-            sc[PAGES + lane] = gv;
+            sc[PAGES + lane] = gr;
+            sc[2 * PAGES + lane] = gl;
           }
-          if (lane == 0) reinterpret_cast<unsigned*>(sc)[2 * PAGES] = groups;
+          if (lane == 0) reinterpret_cast<unsigned*>(sc)[3 * PAGES] = groups;
           __syncwarp();
           if (lane == 0)
             mbar_expect_tx(&full[stage], static_cast<uint32_t>(__popc(there) * box * D * 2));
@@ -347,6 +363,7 @@ __global__ void __launch_bounds__(Q8D_THREADS, 1)
       // query row r of the item: token tok0 + r / group, head r % group
       uint32_t qf[NT][2 * KS];
       int limit[NT][2];  // keys that queries 2t and 2t + 1 see
+      float qm[NT][2];   // what their rows were divided by
 #pragma unroll
       for (int j = 0; j < NT; ++j) {
         const int r = j * 8 + g, tok = tok0 + r / a.group;
@@ -362,6 +379,25 @@ __global__ void __launch_bounds__(Q8D_THREADS, 1)
           qf[j][4 * c + 2] = raw.z;
           qf[j][4 * c + 3] = raw.w;
         }
+        // f16 queries: a power of two brings the row's largest value to [1, 2), and is taken back
+        // with the K scale (values below 2^-14 of the largest lose low bits, 2^-25 of it at most)
+        uint32_t top = 0;
+#pragma unroll
+        for (int i = 0; i < 2 * KS; ++i)
+          top = max(top, max((qf[j][i] & 0x7FFFu) << 16, qf[j][i] & 0x7FFF0000u));
+        top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
+        top = max(top, __shfl_xor_sync(0xffffffffu, top, 2));
+        const uint32_t ex = top >> 23;
+        const bool plain = ex == 0 || ex >= 254;  // zeros and subnormals, or not finite: as they are
+        const float down = plain ? 1.0f : __uint_as_float((254u - ex) << 23);
+        const float up = plain ? 1.0f : __uint_as_float(ex << 23);
+#pragma unroll
+        for (int i = 0; i < 2 * KS; ++i) {
+          const float2 f = unpack_bf16x2(qf[j][i]);
+          qf[j][i] = pack_f16x2(f.x * down, f.y * down);
+        }
+#pragma unroll
+        for (int e = 0; e < 2; ++e) qm[j][e] = __shfl_sync(0xffffffffu, up, (2 * t + e) * 4);
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
           const int r2 = j * 8 + 2 * t + e, tok2 = tok0 + r2 / a.group;
@@ -392,10 +428,10 @@ __global__ void __launch_bounds__(Q8D_THREADS, 1)
                               mbar_wait(&full[stage], (used / L::STAGES) & 1, abort_flag));
         if (!ok) continue;
         const float* sc = reinterpret_cast<const float*>(smem + L::SC_OFF + stage * L::SC);
-        const unsigned groups = reinterpret_cast<const unsigned*>(sc)[8];
+        const unsigned groups = reinterpret_cast<const unsigned*>(sc)[12];
         const int key0 = (at + u) * Q8D_BN + part * 16;
         if ((groups >> part) & 1) {
-          const float ks = sc[part], vs = sc[4 + part];
+          const float ks = sc[part], rv = sc[4 + part], lv = sc[8 + part];
           const uint8_t* sk = smem + stage * L::STAGE + part * 16 * D;
           const uint8_t* sv = sk + L::HALF;
           // scores of keys g and g + 8 for queries 2t, 2t + 1
@@ -412,8 +448,9 @@ __global__ void __launch_bounds__(Q8D_THREADS, 1)
             const uint32_t l4[4] = {lo.x, lo.y, lo.z, lo.w}, h4[4] = {hi.x, hi.y, hi.z, hi.w};
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
-              const uint32_t a0 = q8_pair<FMT>(l4[i], 0u, 0, 1), a2 = q8_pair<FMT>(l4[i], 0u, 2, 3);
-              const uint32_t a1 = q8_pair<FMT>(h4[i], 0u, 0, 1), a3 = q8_pair<FMT>(h4[i], 0u, 2, 3);
+              const uint32_t wl = q8_f16_bias<FMT>(l4[i]), wh = q8_f16_bias<FMT>(h4[i]);
+              const uint32_t a0 = q8_f16_pair<FMT>(wl, 0), a2 = q8_f16_pair<FMT>(wl, 1);
+              const uint32_t a1 = q8_f16_pair<FMT>(wh, 0), a3 = q8_f16_pair<FMT>(wh, 1);
 #pragma unroll
               for (int j = 0; j < NT; ++j)
                 mma_16816(s[j], a0, a1, a2, a3, qf[j][8 * c + 2 * i], qf[j][8 * c + 2 * i + 1]);
@@ -427,7 +464,7 @@ __global__ void __launch_bounds__(Q8D_THREADS, 1)
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
               in[e] = key0 + g + (e >> 1) * 8 < limit[j][e & 1];
-              x[e] = in[e] ? s[j][e] * ks : -INFINITY;
+              x[e] = in[e] ? fmaf(s[j][e], ks * qm[j][e & 1], lv) : -INFINITY;
             }
             // The maximum only moves when a score exceeds it by 2^8 (or there was none): the
             // stale one cancels in the division. Decided for the warp, so that every lane of a
@@ -459,12 +496,12 @@ __global__ void __launch_bounds__(Q8D_THREADS, 1)
             float p[4];
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
-              const float ex = ex2_approx(x[e] - m[j][e & 1]);
-              l[j][e & 1] += ex;
-              p[e] = in[e] ? ex * vs : 0.0f;  // a masked key's scale may be NaN
+              p[e] = ex2_approx(x[e] - m[j][e & 1]);
+              if (in[e]) l[j][e & 1] = fmaf(p[e], rv, l[j][e & 1]);  // a masked key's rv may be NaN
             }
-            pf[j][0] = movmatrix(pack_bf16x2(p[0], p[1]));
-            pf[j][1] = movmatrix(pack_bf16x2(p[2], p[3]));
+            if (lv == -90.0f) p[0] = p[1] = p[2] = p[3] = 0.0f;  // a V scale of 0
+            pf[j][0] = movmatrix(pack_f16x2(p[0], p[1]));
+            pf[j][1] = movmatrix(pack_f16x2(p[2], p[3]));
           }
           // o[dim, query] += v^T p: keys 2t, 2t + 1, 2t + 8, 2t + 9; dims (D / 8) g + 2i, + 1
           uint32_t vv[4][KS / 2];
@@ -484,14 +521,22 @@ __global__ void __launch_bounds__(Q8D_THREADS, 1)
             }
           }
 #pragma unroll
-          for (int i = 0; i < KS; ++i) {
-            const int by = (i & 1) * 2;
-            const uint32_t a0 = q8_pair<FMT>(vv[0][i >> 1], vv[1][i >> 1], by, 4 + by);
-            const uint32_t a1 = q8_pair<FMT>(vv[0][i >> 1], vv[1][i >> 1], by + 1, 5 + by);
-            const uint32_t a2 = q8_pair<FMT>(vv[2][i >> 1], vv[3][i >> 1], by, 4 + by);
-            const uint32_t a3 = q8_pair<FMT>(vv[2][i >> 1], vv[3][i >> 1], by + 1, 5 + by);
+          for (int r = 0; r < 4; ++r)
 #pragma unroll
-            for (int j = 0; j < NT; ++j) mma_16816(o[j][i], a0, a1, a2, a3, pf[j][0], pf[j][1]);
+            for (int i = 0; i < KS / 2; ++i) vv[r][i] = q8_f16_bias<FMT>(vv[r][i]);
+#pragma unroll
+          for (int i = 0; i < KS / 2; ++i) {
+            // bytes of the two keys side by side: dims 4i, 4i + 1 and 4i + 2, 4i + 3 of the run
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+              const uint32_t lo = __byte_perm(vv[0][i], vv[1][i], h ? 0x7362 : 0x5140);
+              const uint32_t hi = __byte_perm(vv[2][i], vv[3][i], h ? 0x7362 : 0x5140);
+              const uint32_t a0 = q8_f16_pair<FMT>(lo, 0), a1 = q8_f16_pair<FMT>(lo, 1);
+              const uint32_t a2 = q8_f16_pair<FMT>(hi, 0), a3 = q8_f16_pair<FMT>(hi, 1);
+#pragma unroll
+              for (int j = 0; j < NT; ++j)
+                mma_16816(o[j][2 * i + h], a0, a1, a2, a3, pf[j][0], pf[j][1]);
+            }
           }
         }
         __syncwarp();
@@ -560,56 +605,92 @@ __global__ void __launch_bounds__(Q8D_THREADS, 1)
 }
 
 // ---------------------------------------------------------------- many query rows
-// tcgen05: an item is up to two tiles of 128 query rows (128 / group tokens x group heads each, so
-// that grouped heads share the keys' tile), in ping-pong over blocks of 128 keys as in the dense
-// kernel; the ring's K and V blocks are written by a warpgroup that reads codes and stores exact
-// bf16 in the layout TMA would (128-byte swizzle). Bound by the exponentials and the conversion.
-//   warp 0        Q tiles by TMA, one item ahead of the first product that needs them
-//   warp 1        tensor memory, products
-//   warps 2..9    softmax (two warps a lane quarter, 64 of the block's keys each)
-//   warps 10..13  codes -> bf16: each thread keeps the next block's codes in registers
-// Tensor memory as in the dense kernel: S_A, S_B, O_A, O_B. All roles walk the same run of items;
-// the pipelines' phases go on over items.
+// tcgen05 on CTA pairs (cta_group::2): an item is up to two tiles of 256 query rows, 128 of each
+// in either CTA (chunks of 128 / group tokens x group heads, so that grouped heads share the keys'
+// tile), in ping-pong over blocks of 128 keys. A pair shares a block's operands: each CTA converts
+// 64 of its keys for the first product and half of the dims of its V for the second, which halves
+// the conversion and the shared-memory traffic that bound the same kernel on single CTAs (1400 us
+// against 1100 for 4608 queries x 9216 keys x 24 heads of 128).
+//   warp 0        Q chunks by TMA, when the last item's first products are done
+//   warp 1        tensor memory; in the even CTA the products
+//   warps 2..9    softmax of the CTA's rows (two warps a lane quarter, 64 of the keys each)
+//   warps 10..13  codes -> bf16 (K), f16 (V) in the layout TMA would write (128-byte swizzle);
+//                 each thread keeps the next block's codes in registers
+// Tensor memory as in the dense kernel: S_A, S_B, O_A, O_B. All roles of both CTAs walk the same
+// run of items; the pipelines' phases go on over items. Tile A sees a prefix of the item's keys
+// under a causal mask and leaves the blocks behind it out.
 constexpr int Q8P_BN = 128;
 constexpr int Q8P_THREADS = 448;
 
+template <int D>
 struct Q8PrefillSmem {
-  static constexpr int HALF = 128 * 64 * 2;  // 128 rows x 64 dims
+  static constexpr int HALF = 128 * 64 * 2;  // Q: 128 rows x 64 dims
+  static constexpr int KHALF = 64 * 64 * 2;  // K: this CTA's 64 keys x 64 dims
+  static constexpr int K_BYTES = D / 64 * KHALF;
+  static constexpr int V_BYTES = 128 * D;    // V: 128 keys x D / 2 dims
   static constexpr int Q_OFF = 0;            // tile t at t * 2 * HALF
-  static constexpr int KV_OFF = 4 * HALF;    // per stage: K 2 halves, V 2 halves
-  static constexpr int STAGE = 4 * HALF;
-  static constexpr int STAGES = 2;
+  static constexpr int KV_OFF = 4 * HALF;
+  static constexpr int STAGE = K_BYTES + V_BYTES;
+  static constexpr int STAGES = 4;
   static constexpr int X_OFF = KV_OFF + STAGES * STAGE;  // maxima [tile][parity][half][128]
   static constexpr int L_OFF = X_OFF + 2 * 2 * 2 * 128 * 4;  // sums [tile][half][128]
   static constexpr int SC_OFF = L_OFF + 2 * 2 * 128 * 4;
-  static constexpr int SC = 80;  // a stage's scales of 8 groups of 16 keys, K then V, and a mask
+  // a stage's 8 groups of 16 keys: K scales (with the softmax scale), 1 / vs, log2(vs), a mask of
+  // the groups that are there
+  static constexpr int SC = 112;
   static constexpr int BAR_OFF = SC_OFF + STAGES * SC;
-  // q_full, q_empty, kv_full[2], kv_empty[2], s_full[2], p_full[2], o_full, o_empty,
-  // xbar[4][2][2], lbar[4]
-  static constexpr int NBAR = 2 + 2 * STAGES + 2 + 2 + 2 + 16 + 4;
+  // q_full, q_empty, kv_full[S], kv_empty[S], sc_full[S], s_full[2], p_full[2], o_full, o_empty,
+  // drain, xbar[4][2][2], lbar[4]
+  static constexpr int NBAR = 2 + 3 * STAGES + 2 + 2 + 3 + 16 + 4;
   static constexpr int TOTAL = BAR_OFF + NBAR * 8 + 64 + 1024;
 };
+
+// sdesc_mn128 for 32 elements a row: 64-byte rows along K with the 64-byte swizzle, 8-row groups
+// 512 bytes apart.
+__device__ __forceinline__ uint64_t sdesc_mn64(uint32_t saddr) {
+  uint64_t d = 0;
+  d |= static_cast<uint64_t>((saddr & 0x3FFFFu) >> 4);
+  d |= static_cast<uint64_t>(1u) << 16;
+  d |= static_cast<uint64_t>(512u >> 4) << 32;
+  d |= static_cast<uint64_t>(1u) << 46;
+  d |= static_cast<uint64_t>(4u) << 61;
+  return d;
+}
+
+// D += A (each CTA's tensor memory) * B (halves of N in both CTAs' shared memory).
+__device__ __forceinline__ void umma_f16_ts_pair(uint32_t d_tmem, uint32_t a_tmem, uint64_t b_desc,
+                                                 uint32_t idesc, uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::2.kind::f16 [%0], [%1], %2, %3, {%5, %5, %5, %5, %5, %5, %5, %5}, "
+      "p;\n\t}" ::"r"(d_tmem),
+      "r"(a_tmem), "l"(b_desc), "r"(idesc), "r"(accumulate), "r"(0u)
+      : "memory");
+}
 
 template <int D, int FMT>
 __global__ void __launch_bounds__(Q8P_THREADS, 1)
     attention_q8_prefill_kernel(const __grid_constant__ CUtensorMap map_q, const Q8Attn a) {
-  using L = Q8PrefillSmem;
+  using L = Q8PrefillSmem<D>;
   using Work = Q8Work<Q8P_BN>;
   constexpr int NH = D / 64;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) &
                                              ~static_cast<uintptr_t>(1023));
   uint64_t* bars = reinterpret_cast<uint64_t*>(smem + L::BAR_OFF);
-  uint64_t* q_full = bars;
+  uint64_t* q_full = bars;                      // even CTA's
   uint64_t* q_empty = bars + 1;
-  uint64_t* kv_full = bars + 2;
+  uint64_t* kv_full = bars + 2;                 // even CTA's
   uint64_t* kv_empty = kv_full + L::STAGES;
-  uint64_t* s_full = kv_empty + L::STAGES;
-  uint64_t* p_full = s_full + 2;
+  uint64_t* sc_full = kv_empty + L::STAGES;
+  uint64_t* s_full = sc_full + L::STAGES;
+  uint64_t* p_full = s_full + 2;                // even CTA's
   uint64_t* o_full = p_full + 2;
-  uint64_t* o_empty = o_full + 1;
-  uint64_t* xbar = o_empty + 1;  // [quarter][tile][parity]
-  uint64_t* lbar = xbar + 16;    // [quarter]
+  uint64_t* o_empty = o_full + 1;               // even CTA's
+  uint64_t* drain = o_empty + 1;
+  uint64_t* xbar = drain + 1;                   // [quarter][tile][parity]
+  uint64_t* lbar = xbar + 16;                   // [quarter]
   int64_t* s_run = reinterpret_cast<int64_t*>(bars + L::NBAR);  // u0, u1, at
   int* s_item = reinterpret_cast<int*>(s_run + 3);              // b, tile, head
   volatile int* abort_flag = s_item + 3;
@@ -619,12 +700,14 @@ __global__ void __launch_bounds__(Q8P_THREADS, 1)
 
   const int warp = warp_id();
   const int lane = static_cast<int>(lane_id());
+  const int rank = static_cast<int>(cluster_rank());
+  const int pair = static_cast<int>(blockIdx.x >> 1);
   griddep_wait();
   Work w(a);
   if (warp == 0) {
     const int64_t total = w.total();
     const int64_t run = q8_run_units(a, total);
-    const int64_t u0 = blockIdx.x * run;
+    const int64_t u0 = pair * run;
     int64_t in = 0;
     if (u0 < total) in = w.seek(u0);
     if (lane == 0) {
@@ -641,25 +724,28 @@ __global__ void __launch_bounds__(Q8P_THREADS, 1)
       mbar_init(q_full, 1);
       mbar_init(q_empty, 1);
       for (int i = 0; i < L::STAGES; ++i) {
-        mbar_init(&kv_full[i], 4);
+        mbar_init(&kv_full[i], 8);  // the converting warps of both CTAs
         mbar_init(&kv_empty[i], 1);
+        mbar_init(&sc_full[i], 1);
       }
       for (int t = 0; t < 2; ++t) {
         mbar_init(&s_full[t], 1);
-        mbar_init(&p_full[t], 8);
+        mbar_init(&p_full[t], 16);  // the softmax warps of both CTAs
       }
       mbar_init(o_full, 1);
-      mbar_init(o_empty, 8);
+      mbar_init(o_empty, 16);
+      mbar_init(drain, 1);
       for (int i = 0; i < 16; ++i) mbar_init(&xbar[i], 64);
       for (int i = 0; i < 4; ++i) mbar_init(&lbar[i], 64);
       fence_barrier_init();
     }
     __syncwarp();
-    tmem_alloc(tmem_slot, 512);
-    tmem_relinquish();
+    tmem_alloc_pair(tmem_slot, 512);
+    tmem_relinquish_pair();
   }
   tc_fence_before();
   __syncthreads();
+  cluster_sync();  // both CTAs' barriers exist before any remote arrive
   tc_fence_after();
   const uint32_t tmem = *tmem_slot;
   griddep_launch();
@@ -671,7 +757,13 @@ __global__ void __launch_bounds__(Q8P_THREADS, 1)
     w.head = s_item[2];
     w.units = Work::units_of(a, w.count, w.len, w.tile);
   }
-  const int tile_q = a.tile_tokens >> 1;  // tokens of a 128-row tile
+  const int chunk = a.tile_tokens >> 2;  // tokens of 128 rows
+  // Blocks that tile A takes part in: those its last token sees, all if there is no tile B.
+  auto blocks_a = [&](int ntile) {
+    if (ntile == 1 || !a.causal) return w.units;
+    const int last = min(w.count, w.tile * a.tile_tokens + 2 * chunk);
+    return (max(0, w.len - w.count + last) + Q8P_BN - 1) / Q8P_BN;
+  };
 
   if (warp < 2) {
     if (warp == 0 && lane == 0) {
@@ -681,47 +773,49 @@ __global__ void __launch_bounds__(Q8P_THREADS, 1)
         const int n = static_cast<int>(left < w.units - at ? left : w.units - at);
         if (Work::keys(a, w.count, w.len, w.tile) > 0) {
           const int tok0 = w.tile * a.tile_tokens;
-          const int ntile = w.count - tok0 > tile_q ? 2 : 1;
+          const int ntile = w.count - tok0 > 2 * chunk ? 2 : 1;
           if (!mbar_wait(q_empty, (items & 1) ^ 1u, abort_flag)) break;
-          mbar_expect_tx(q_full, static_cast<uint32_t>(ntile * D * 2 * a.group * tile_q));
+          if (rank == 0)
+            mbar_expect_tx(q_full, static_cast<uint32_t>(ntile * 2 * D * 2 * a.group * chunk));
           for (int t = 0; t < ntile; ++t)
             for (int h = 0; h < NH; ++h)
-              tma_load_3d(smem + L::Q_OFF + (t * 2 + h) * L::HALF, &map_q, q_full, h * 64,
-                          w.head * a.group, static_cast<int>(w.first) + tok0 + t * tile_q);
+              tma_load_3d_pair(smem + L::Q_OFF + (t * 2 + h) * L::HALF, &map_q,
+                               smem_u32(q_full) & kPairLeaderMask, h * 64, w.head * a.group,
+                               static_cast<int>(w.first) + tok0 + (2 * t + rank) * chunk);
           ++items;
         }
         left -= n;
         at = 0;
         if (left > 0) w.next();
       }
-      if (*abort_flag && items > 0) {  // copies in flight land (bounded)
+      if (*abort_flag && items > 0) {  // a bounded moment for copies in flight
         const uint64_t t0 = global_ns();
-        while (!mbar_try_wait(q_full, (items - 1) & 1) && global_ns() - t0 < 200000000ull) {
+        while (global_ns() - t0 < 100000000ull) {
         }
       }
-    } else if (warp == 1 && lane == 0) {
+    } else if (warp == 1 && lane == 0 && rank == 0) {
       // ---- products
-      constexpr uint32_t idesc_s = idesc_bf16(128, 128);
-      constexpr uint32_t idesc_o = idesc_bf16(128, D) | (1u << 16);  // V: MN-major
+      constexpr uint32_t idesc_s = idesc_bf16(256, 128);
+      constexpr uint32_t idesc_o = idesc_f16(256, D) | (1u << 16);  // V: MN-major
       auto s_mma = [&](int t, int jb) {
         const uint32_t sq = smem_u32(smem + L::Q_OFF + t * 2 * L::HALF);
         const uint32_t sk = smem_u32(smem + L::KV_OFF + (jb % L::STAGES) * L::STAGE);
 #pragma unroll
-        for (int kk = 0; kk < D / 16; ++kk) {
-          const uint32_t off = (kk >> 2) * L::HALF + (kk & 3) * 32;
-          umma_bf16(tmem + t * 128, sdesc_k128(sq + off), sdesc_k128(sk + off), idesc_s,
-                    kk > 0 ? 1u : 0u);
-        }
-        umma_commit(&s_full[t]);
+        for (int kk = 0; kk < D / 16; ++kk)
+          umma_bf16_pair(tmem + t * 128, sdesc_k128(sq + (kk >> 2) * L::HALF + (kk & 3) * 32),
+                         sdesc_k128(sk + (kk >> 2) * L::KHALF + (kk & 3) * 32), idesc_s,
+                         kk > 0 ? 1u : 0u);
+        umma_commit_pair(&s_full[t], 0x3);
       };
       auto pv_mma = [&](int t, int jb, bool first) {
         const uint32_t sv =
-            smem_u32(smem + L::KV_OFF + (jb % L::STAGES) * L::STAGE + 2 * L::HALF);
+            smem_u32(smem + L::KV_OFF + (jb % L::STAGES) * L::STAGE + L::K_BYTES);
 #pragma unroll
         for (int kk = 0; kk < Q8P_BN / 16; ++kk)
-          umma_bf16_ts(tmem + 256 + t * 128, tmem + t * 128 + kk * 8 + (kk >= 4 ? 32 : 0),
-                       sdesc_mn128(sv + kk * 2048, L::HALF), idesc_o,
-                       (!first || kk > 0) ? 1u : 0u);
+          umma_f16_ts_pair(tmem + 256 + t * 128, tmem + t * 128 + kk * 8 + (kk >= 4 ? 32 : 0),
+                           D == 128 ? sdesc_mn128(sv + kk * 2048, L::V_BYTES)
+                                    : sdesc_mn64(sv + kk * 1024),
+                           idesc_o, (!first || kk > 0) ? 1u : 0u);
       };
       int items = 0, jb = 0;
       int cnt[2] = {0, 0};  // blocks that a tile has been given
@@ -729,37 +823,38 @@ __global__ void __launch_bounds__(Q8P_THREADS, 1)
       while (left > 0 && ok) {
         const int n = static_cast<int>(left < w.units - at ? left : w.units - at);
         if (Work::keys(a, w.count, w.len, w.tile) > 0) {
-          const int ntile = w.count - w.tile * a.tile_tokens > tile_q ? 2 : 1;
+          const int ntile = w.count - w.tile * a.tile_tokens > 2 * chunk ? 2 : 1;
+          const int na = blocks_a(ntile) - at;  // of this piece's blocks
           ok = mbar_wait(q_full, items & 1, abort_flag) &&
-               mbar_wait(&kv_full[jb % L::STAGES], (jb / L::STAGES) & 1, abort_flag);
+               mbar_wait(&kv_full[jb % L::STAGES], (jb / L::STAGES) & 1, abort_flag) &&
+               mbar_wait(o_empty, (items & 1) ^ 1u, abort_flag);  // the last output was read
           if (!ok) break;
           tc_fence_after();
-          for (int t = 0; t < ntile; ++t) s_mma(t, jb);
+          for (int t = na > 0 ? 0 : 1; t < ntile; ++t) s_mma(t, jb);
           for (int j = 0; j < n && ok; ++j, ++jb) {
-            const bool more = j + 1 < n;
-            for (int t = 0; t < ntile; ++t) {
+            bool next_there = false;
+            for (int t = j < na ? 0 : 1; t < ntile; ++t) {
               ok = mbar_wait(&p_full[t], cnt[t] & 1, abort_flag);
-              // the previous item's output has been read
-              if (ok && j == 0 && t == 0) ok = mbar_wait(o_empty, (items & 1) ^ 1u, abort_flag);
               if (!ok) break;
               ++cnt[t];
               tc_fence_after();
               pv_mma(t, jb, j == 0);
-              if (t == ntile - 1) umma_commit(&kv_empty[jb % L::STAGES]);
-              if (more) {
-                if (t == 0) {
+              if (t == ntile - 1) umma_commit_pair(&kv_empty[jb % L::STAGES], 0x3);
+              if (j + 1 < n && (t == 1 || j + 1 < na)) {
+                if (!next_there) {
                   ok = mbar_wait(&kv_full[(jb + 1) % L::STAGES], ((jb + 1) / L::STAGES) & 1,
                                  abort_flag);
                   if (!ok) break;
                   tc_fence_after();
+                  next_there = true;
                 }
                 s_mma(t, jb + 1);
               }
             }
           }
           if (!ok) break;
-          umma_commit(q_empty);
-          umma_commit(o_full);
+          umma_commit_pair(q_empty, 0x3);
+          umma_commit_pair(o_full, 0x3);
           ++items;
         }
         left -= n;
@@ -767,34 +862,36 @@ __global__ void __launch_bounds__(Q8P_THREADS, 1)
         if (left > 0) w.next();
       }
       // all issued products end before tensor memory is released (bounded)
-      if (!ok) {
-        umma_commit(o_full);
-        const uint64_t t0 = global_ns();
-        while (!mbar_try_wait(o_full, items & 1) && global_ns() - t0 < 200000000ull) {
-        }
+      umma_commit_pair(drain, 0x1);
+      const uint64_t t0 = global_ns();
+      while (!mbar_try_wait(drain, 0) && global_ns() - t0 < 200000000ull) {
       }
     }
     __syncwarp();
   } else if (warp >= 10) {
-    // ---- codes to bf16
-    constexpr int PER_ROW = D / 16;                 // 16-code runs of a token
-    constexpr int ROWS = 32 / PER_ROW;              // tokens a warp reads at once
-    constexpr int NV = Q8P_BN / (4 * ROWS);         // its reads of K (and of V) a block
+    // ---- codes to 16 bits
     const int cw = warp - 10;
-    // a quarter warp's 16-byte stores fall on even chunks of one token and odd ones of the next
-    const int run16 = D == 128 ? (lane & 3) + ((lane >> 3) & 1) * 4 : lane & 3;
-    const int row = cw * ROWS + (D == 128 ? ((lane >> 2) & 1) + (lane >> 4) * 2 : lane >> 2);
-    uint32_t dst0 = smem_u32(smem + L::KV_OFF) + (run16 >> 2) * L::HALF + row * 128;
-    const uint32_t c0 = dst0 + ((((run16 & 3) * 2) ^ (row & 7)) << 4);
-    const uint32_t c1 = dst0 + ((((run16 & 3) * 2 + 1) ^ (row & 7)) << 4);
-    int n = 0;        // units of the item that are left to look up
-    bool none = false;  // an item without keys has one unit and no block
-    auto settle = [&]() {
-      // the cursor stands on a block that has keys, or left == 0
+    // K: runs of 16 codes of this CTA's 64 keys; V: of D / 2 dims of 128 keys. The lanes of a
+    // quarter warp are laid so that its 16-byte stores fall on different banks.
+    constexpr int KPR = D / 16, VPR = D / 32;            // runs a row
+    constexpr int KROWS = 128 / KPR, VROWS = 128 / VPR;  // rows that the four warps read at once
+    constexpr int NK = 64 / KROWS, NVV = 128 / VROWS;    // reads a thread
+    const int k_run = D == 128 ? (lane & 3) + ((lane >> 3) & 1) * 4 : lane & 3;
+    const int k_row = cw * (32 / KPR) + (D == 128 ? ((lane >> 2) & 1) + (lane >> 4) * 2 : lane >> 2);
+    const int v_run = D == 128 ? lane & 3 : lane & 1;
+    const int v_row = cw * (32 / VPR) + (D == 128 ? lane >> 2 : lane >> 1);
+    const uint32_t k_dst = smem_u32(smem + L::KV_OFF) + (k_run >> 2) * L::KHALF + k_row * 128;
+    const uint32_t k0 = k_dst + ((((k_run & 3) * 2) ^ (k_row & 7)) << 4);
+    const uint32_t k1 = k_dst + ((((k_run & 3) * 2 + 1) ^ (k_row & 7)) << 4);
+    const uint32_t v_dst = smem_u32(smem + L::KV_OFF) + L::K_BYTES + v_row * D;
+    const int v_swz = D == 128 ? v_row & 7 : (v_row >> 1) & 3;
+    const uint32_t v0 = v_dst + (((v_run * 2) ^ v_swz) << 4);
+    const uint32_t v1 = v_dst + (((v_run * 2 + 1) ^ v_swz) << 4);
+    int n = 0;  // units of the item that are left to look up
+    auto settle = [&]() {  // on to a unit with keys (an item without any has one unit), or the end
       while (left > 0) {
         n = static_cast<int>(left < w.units - at ? left : w.units - at);
-        none = Work::keys(a, w.count, w.len, w.tile) == 0;
-        if (!none) return;
+        if (Work::keys(a, w.count, w.len, w.tile) > 0) return;
         left -= n;
         at = 0;
         if (left > 0) w.next();
@@ -811,11 +908,11 @@ __global__ void __launch_bounds__(Q8P_THREADS, 1)
         }
       }
     };
-    // lanes 0..7: where the cursor's 16-key groups are, and their scales
-    int there = -1;
+    // lanes 0..7: where the cursor's 16-key groups are (K and V), and their scales
+    int k_there = -1, v_there = -1;
     float ks = 0.0f, vs = 0.0f;
     auto look = [&]() {
-      there = -1;
+      k_there = v_there = -1;
       ks = vs = 0.0f;
       if (left > 0 && lane < 8) {
         const int key = at * Q8P_BN + lane * 16;
@@ -823,39 +920,51 @@ __global__ void __launch_bounds__(Q8P_THREADS, 1)
           const int page = a.table[static_cast<int64_t>(w.b) * a.ld_table + key / a.block];
           if (page >= 0 && page < a.num_blocks) {
             const int unit = page * a.heads + w.head;
-            there = unit * a.block + key % a.block;
+            k_there = unit * a.block + key % a.block;
             ks = a.scales[0][unit] * a.scale_log2;
             vs = a.scales[1][unit];
+            v_there = vs <= Q8_LEAST_V ? -1 : k_there;  // taken as zero codes
           } else {
             q8_flag(1);
           }
         }
       }
     };
-    uint4 raw[2][NV];
-    auto fetch = [&](int kv, int i) {
-      // rows of read i: group (i * 4 * ROWS + row) / 16, the same for the whole warp
-      const int r = i * 4 * ROWS + row;
-      const int base = __shfl_sync(0xffffffffu, there, r >> 4);
-      raw[kv][i] = make_uint4(0, 0, 0, 0);
+    uint4 kraw[NK], vraw[NVV];
+    auto fetch_k = [&](int i) {
+      const int r = rank * 64 + i * KROWS + k_row;
+      const int base = __shfl_sync(0xffffffffu, k_there, r >> 4);
+      kraw[i] = make_uint4(0, 0, 0, 0);
       if (base >= 0)
-        raw[kv][i] = __ldg(reinterpret_cast<const uint4*>(
-            a.codes[kv] + static_cast<int64_t>(base + (r & 15)) * D + run16 * 16));
+        kraw[i] = __ldg(reinterpret_cast<const uint4*>(
+            a.codes[0] + static_cast<int64_t>(base + (r & 15)) * D + k_run * 16));
+    };
+    auto fetch_v = [&](int i) {
+      const int r = i * VROWS + v_row;
+      const int base = __shfl_sync(0xffffffffu, v_there, r >> 4);
+      vraw[i] = make_uint4(0, 0, 0, 0);
+      if (base >= 0)
+        vraw[i] = __ldg(reinterpret_cast<const uint4*>(
+            a.codes[1] + static_cast<int64_t>(base + (r & 15)) * D + rank * (D / 2) + v_run * 16));
+    };
+    auto store = [&](uint32_t dst, uint32_t x, uint32_t y, uint32_t z, uint32_t t) {
+      asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(dst), "r"(x), "r"(y), "r"(z),
+                   "r"(t)
+                   : "memory");
     };
     settle();
     look();
-    int todo = left > 0;
+    bool todo = left > 0;
     if (todo) {
 #pragma unroll
-      for (int i = 0; i < NV; ++i) {
-        fetch(0, i);
-        fetch(1, i);
-      }
+      for (int i = 0; i < NK; ++i) fetch_k(i);
+#pragma unroll
+      for (int i = 0; i < NVV; ++i) fetch_v(i);
     }
     int jb = 0;
     while (todo) {
       const float ks_now = ks, vs_now = vs;
-      const unsigned groups = __ballot_sync(0xffffffffu, there >= 0) & 0xFFu;
+      const unsigned groups = __ballot_sync(0xffffffffu, k_there >= 0) & 0xFFu;
       step();
       look();
       todo = left > 0;
@@ -864,32 +973,48 @@ __global__ void __launch_bounds__(Q8P_THREADS, 1)
                                              abort_flag)))
         break;
 #pragma unroll
-      for (int kv = 0; kv < 2; ++kv)
+      for (int i = 0; i < NK; ++i) {
+        const uint32_t off = stage * L::STAGE + i * KROWS * 128;
+        const uint4 v = kraw[i];
+        store(k0 + off, q8_pair<FMT>(v.x, 0u, 0, 1), q8_pair<FMT>(v.x, 0u, 2, 3),
+              q8_pair<FMT>(v.y, 0u, 0, 1), q8_pair<FMT>(v.y, 0u, 2, 3));
+        store(k1 + off, q8_pair<FMT>(v.z, 0u, 0, 1), q8_pair<FMT>(v.z, 0u, 2, 3),
+              q8_pair<FMT>(v.w, 0u, 0, 1), q8_pair<FMT>(v.w, 0u, 2, 3));
+      }
+      if (todo) {
 #pragma unroll
-        for (int i = 0; i < NV; ++i) {
-          const uint32_t off = stage * L::STAGE + kv * 2 * L::HALF + i * 4 * ROWS * 128;
-          const uint4 v = raw[kv][i];
-          asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(c0 + off),
-                       "r"(q8_pair<FMT>(v.x, 0u, 0, 1)), "r"(q8_pair<FMT>(v.x, 0u, 2, 3)),
-                       "r"(q8_pair<FMT>(v.y, 0u, 0, 1)), "r"(q8_pair<FMT>(v.y, 0u, 2, 3))
-                       : "memory");
-          asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(c1 + off),
-                       "r"(q8_pair<FMT>(v.z, 0u, 0, 1)), "r"(q8_pair<FMT>(v.z, 0u, 2, 3)),
-                       "r"(q8_pair<FMT>(v.w, 0u, 0, 1)), "r"(q8_pair<FMT>(v.w, 0u, 2, 3))
-                       : "memory");
-          if (todo) fetch(kv, i);
-        }
+        for (int i = 0; i < NK; ++i) fetch_k(i);
+      }
+#pragma unroll
+      for (int i = 0; i < NVV; ++i) {
+        const uint32_t off = stage * L::STAGE + i * VROWS * D;
+        const uint32_t x = q8_f16_bias<FMT>(vraw[i].x), y = q8_f16_bias<FMT>(vraw[i].y);
+        const uint32_t z = q8_f16_bias<FMT>(vraw[i].z), t = q8_f16_bias<FMT>(vraw[i].w);
+        store(v0 + off, q8_f16_pair<FMT>(x, 0), q8_f16_pair<FMT>(x, 1), q8_f16_pair<FMT>(y, 0),
+              q8_f16_pair<FMT>(y, 1));
+        store(v1 + off, q8_f16_pair<FMT>(z, 0), q8_f16_pair<FMT>(z, 1), q8_f16_pair<FMT>(t, 0),
+              q8_f16_pair<FMT>(t, 1));
+      }
+      if (todo) {
+#pragma unroll
+        for (int i = 0; i < NVV; ++i) fetch_v(i);
+      }
       if (cw == 0) {
         float* sc = reinterpret_cast<float*>(smem + L::SC_OFF + stage * L::SC);
         if (lane < 8) {
           sc[lane] = ks_now;
-          sc[8 + lane] = vs_now;
+          const float v = vs_now <= Q8_LEAST_V ? Q8_LEAST_V : vs_now;
+          sc[8 + lane] = 1.0f / (v * q8_f16_unit<FMT>());
+          sc[16 + lane] = log2f(v);
         }
-        if (lane == 0) reinterpret_cast<unsigned*>(sc)[16] = groups;
+        if (lane == 0) reinterpret_cast<unsigned*>(sc)[24] = groups;
       }
       fence_proxy_async_smem();
       __syncwarp();
-      if (lane == 0) mbar_arrive(&kv_full[stage]);
+      if (lane == 0) {
+        if (cw == 0) mbar_arrive(&sc_full[stage]);
+        mbar_arrive_cluster(cluster_addr(smem_u32(&kv_full[stage]), 0));
+      }
       ++jb;
     }
   } else {
@@ -899,7 +1024,9 @@ __global__ void __launch_bounds__(Q8P_THREADS, 1)
     const int row = quarter * 32 + lane;
     const uint32_t lane_base = static_cast<uint32_t>(quarter * 32) << 16;
     const int row_tok = row / a.group, row_head = row % a.group;
-    const bool in_row = row < tile_q * a.group;
+    const bool in_row = row < chunk * a.group;
+    const uint32_t p_full0 = cluster_addr(smem_u32(&p_full[0]), 0);
+    const uint32_t o_empty0 = cluster_addr(smem_u32(o_empty), 0);
     int items = 0, jb = 0, piece = 0;
     int cnt[2] = {0, 0};
     bool ok = true;
@@ -907,12 +1034,12 @@ __global__ void __launch_bounds__(Q8P_THREADS, 1)
       const int n = static_cast<int>(left < w.units - at ? left : w.units - at);
       const bool whole = n == w.units;
       const int keys = Work::keys(a, w.count, w.len, w.tile);
-      const int tok0 = w.tile * a.tile_tokens;
-      const int ntile = w.count - tok0 > tile_q ? 2 : 1;
+      const int tok0 = w.tile * a.tile_tokens + rank * chunk;  // of tile A; tile B 2 chunks on
+      const int ntile = w.count - w.tile * a.tile_tokens > 2 * chunk ? 2 : 1;
       int limit[2], least[2];  // keys that this row sees; the least of the warp's rows
 #pragma unroll
       for (int t = 0; t < 2; ++t) {
-        const int tok = tok0 + t * tile_q + row_tok;
+        const int tok = tok0 + t * 2 * chunk + row_tok;
         const bool live = in_row && tok < w.count;
         // rows of no query are computed with whatever is there and not stored
         limit[t] = !live ? 0x7fffffff
@@ -922,17 +1049,17 @@ __global__ void __launch_bounds__(Q8P_THREADS, 1)
       float m_run[2] = {-INFINITY, -INFINITY};
       float l_run[2] = {0.0f, 0.0f};
       const int blocks = keys > 0 ? n : 0;
+      const int na = keys > 0 ? blocks_a(ntile) - at : 0;
       for (int j = 0; j < blocks && ok; ++j, ++jb) {
         const int stage = jb % L::STAGES;
-        const float* sc = reinterpret_cast<const float*>(smem + L::SC_OFF + stage * L::SC);
+        const uint8_t* sc = smem + L::SC_OFF + stage * L::SC;
         const int key0 = (at + j) * Q8P_BN + half * 64;
         ok = __all_sync(0xffffffffu,
-                        mbar_wait(&kv_full[stage], (jb / L::STAGES) & 1, abort_flag));
+                        mbar_wait(&sc_full[stage], (jb / L::STAGES) & 1, abort_flag));
         if (!ok) break;
-        const volatile float* ks = sc + half * 4;  // of the half's four groups of 16 keys
-        const volatile float* vs = ks + 8;
-        const unsigned groups = (reinterpret_cast<const unsigned*>(sc)[16] >> (half * 4)) & 15u;
-        for (int t = 0; t < ntile; ++t) {
+        const float4* sc4 = reinterpret_cast<const float4*>(sc);
+        const unsigned groups = (reinterpret_cast<const unsigned*>(sc)[24] >> (half * 4)) & 15u;
+        for (int t = j < na ? 0 : 1; t < ntile; ++t) {
           ok = __all_sync(0xffffffffu, mbar_wait(&s_full[t], cnt[t] & 1, abort_flag));
           if (!ok) break;
           tc_fence_after();
@@ -941,9 +1068,16 @@ __global__ void __launch_bounds__(Q8P_THREADS, 1)
           tmem_ld32(s_col, sr[0]);
           tmem_ld32(s_col + 32, sr[1]);
           tmem_wait_ld();
+          // Row i of the tile keeps one reference m, and the second product's operand is
+          //   P = vs exp2(s ks - m) = exp2(s ks + log2(vs) - m),
+          // so the reference follows the largest s ks + log2(vs) and P stays within f16's range
+          // whatever the blocks' V scales are; the row sum takes a group's sum of P over vs.
+          const float4 k4 = sc4[half], r4 = sc4[2 + half], g4 = sc4[4 + half];
+          const float ks[4] = {k4.x, k4.y, k4.z, k4.w}, rv[4] = {r4.x, r4.y, r4.z, r4.w};
+          const float lv[4] = {g4.x, g4.y, g4.z, g4.w};
           const bool masked = key0 + 64 > least[t] || groups != 15u;  // warp-uniform
+          const int valid = masked ? limit[t] - key0 : 64;
           if (masked) {
-            const int valid = limit[t] - key0;
 #pragma unroll
             for (int i = 0; i < 64; ++i)
               if (i >= valid || !((groups >> (i >> 4)) & 1))
@@ -962,7 +1096,8 @@ __global__ void __launch_bounds__(Q8P_THREADS, 1)
             x = max3f(x, __uint_as_float(v[13]), __uint_as_float(v[14]));
             x = fmaxf(x, __uint_as_float(v[15]));
             // scales are not negative; a masked group stays at -inf whatever its scale is
-            mine = fmaxf(mine, x == -INFINITY ? x : x * ks[q]);
+            const float y = fmaf(x, ks[q], lv[q]);
+            mine = fmaxf(mine, masked && x == -INFINITY ? x : y);
           }
           float* xm = xmax + (t * 2 + (cnt[t] & 1)) * 256;
           xm[half * 128 + row] = mine;
@@ -985,45 +1120,51 @@ __global__ void __launch_bounds__(Q8P_THREADS, 1)
             m_run[t] = m_blk;
           }
           const float ref = m_run[t] == -INFINITY ? 0.0f : m_run[t];
-          const uint64_t negm = f2_pack(-ref, -ref);
-          uint64_t lsum2[2] = {f2_pack(0.0f, 0.0f), f2_pack(0.0f, 0.0f)};
+          float l_blk = 0.0f;
+          auto exps = [&](auto tag) {
+            constexpr bool MASKED = decltype(tag)::value;
 #pragma unroll
-          for (int q8 = 0; q8 < 4; ++q8) {
-            uint32_t packed[8];
-            const uint64_t k2 = f2_pack(ks[q8], ks[q8]), v2 = f2_pack(vs[q8], vs[q8]);
+            for (int q8 = 0; q8 < 4; ++q8) {
+              uint32_t packed[8];
+              const uint64_t k2 = f2_pack(ks[q8], ks[q8]);
+              const float c = lv[q8] - ref;
+              const uint64_t c2 = f2_pack(c, c);
+              uint64_t sum2[2] = {f2_pack(0.0f, 0.0f), f2_pack(0.0f, 0.0f)};
 #pragma unroll
-            for (int u = 0; u < 8; ++u) {
-              const int i = q8 * 8 + u;
-              const uint32_t* v = sr[i >> 4];
-              const int e = (2 * i) & 31;
-              const uint64_t xs =
-                  f2_fma(f2_pack(__uint_as_float(v[e]), __uint_as_float(v[e + 1])), k2, negm);
-              uint64_t ev;
-              if ((ATT_EMU_MASK >> (i & 7)) & 1) {
-                ev = exp2_poly_x2(xs);
-              } else {
-                const float2 xv = f2_unpack(xs);
-                ev = f2_pack(ex2_approx(xv.x), ex2_approx(xv.y));
+              for (int u = 0; u < 8; ++u) {
+                const int i = q8 * 8 + u;
+                const uint32_t* v = sr[i >> 4];
+                const int e = (2 * i) & 31;
+                const uint64_t xs =
+                    f2_fma(f2_pack(__uint_as_float(v[e]), __uint_as_float(v[e + 1])), k2, c2);
+                uint64_t ev;
+                if ((ATT_EMU_MASK >> (i & 7)) & 1) {
+                  ev = exp2_poly_x2(xs);
+                } else {
+                  const float2 xv = f2_unpack(xs);
+                  ev = f2_pack(ex2_approx(xv.x), ex2_approx(xv.y));
+                }
+                float2 p2 = f2_unpack(ev);
+                if constexpr (MASKED) {  // a masked key counts for nothing, its scales may be NaN
+                  const bool g = (groups >> q8) & 1;
+                  p2.x = g && 2 * i < valid ? p2.x : 0.0f;
+                  p2.y = g && 2 * i + 1 < valid ? p2.y : 0.0f;
+                  ev = f2_pack(p2.x, p2.y);
+                }
+                sum2[u & 1] = f2_add(sum2[u & 1], ev);
+                packed[u] = pack_f16x2(p2.x, p2.y);
               }
-              float2 p2;
-              if (masked) {  // a masked key counts for nothing, also where its scales are NaN
-                const float2 e2 = f2_unpack(ev);
-                const bool in0 = v[e] != __float_as_uint(-INFINITY);
-                const bool in1 = v[e + 1] != __float_as_uint(-INFINITY);
-                ev = f2_pack(in0 ? e2.x : 0.0f, in1 ? e2.y : 0.0f);
-                p2 = f2_unpack(f2_mul(ev, v2));
-                p2.x = in0 ? p2.x : 0.0f;
-                p2.y = in1 ? p2.y : 0.0f;
-              } else {
-                p2 = f2_unpack(f2_mul(ev, v2));
-              }
-              lsum2[u & 1] = f2_add(lsum2[u & 1], ev);
-              packed[u] = pack_bf16x2(p2.x, p2.y);
+              tmem_st8(s_col + q8 * 8, packed);
+              const float2 s2 = f2_unpack(f2_add(sum2[0], sum2[1]));
+              if (!MASKED || (((groups >> q8) & 1) && q8 * 16 < valid))
+                l_blk = fmaf(s2.x + s2.y, rv[q8], l_blk);
             }
-            tmem_st8(s_col + q8 * 8, packed);
-          }
-          const float2 ls = f2_unpack(f2_add(lsum2[0], lsum2[1]));
-          l_run[t] += ls.x + ls.y;
+          };
+          if (masked)
+            exps(std::true_type{});
+          else
+            exps(std::false_type{});
+          l_run[t] += l_blk;
           if (rescale) {
             const uint32_t o_col = tmem + lane_base + 256 + t * 128 + half * (D / 2);
 #pragma unroll 1
@@ -1039,7 +1180,7 @@ __global__ void __launch_bounds__(Q8P_THREADS, 1)
           tmem_wait_st();
           tc_fence_before();
           __syncwarp();
-          if (lane == 0) mbar_arrive(&p_full[t]);
+          if (lane == 0) mbar_arrive_cluster(p_full0 + t * 8);
           ++cnt[t];
         }
       }
@@ -1052,13 +1193,15 @@ __global__ void __launch_bounds__(Q8P_THREADS, 1)
         if (!ok) break;
         tc_fence_after();
       }
-      const int slot = 2 * static_cast<int>(blockIdx.x) + (piece > 0 ? 1 : 0);
+      const int slot = 2 * pair + (piece > 0 ? 1 : 0);
       for (int t = 0; t < ntile; ++t) {
-        const int tok = tok0 + t * tile_q + row_tok;
+        const bool some = blocks > 0 && (t == 1 || na > 0);  // the tile's output was written
+        const int tok = tok0 + t * 2 * chunk + row_tok;
         const bool store = in_row && tok < w.count;
-        const float sum = blocks > 0 ? l_run[t] + xsum[(t * 2 + 1 - half) * 128 + row] : 0.0f;
+        const float sum = some ? l_run[t] + xsum[(t * 2 + 1 - half) * 128 + row] : 0.0f;
         const float inv = m_run[t] == -INFINITY ? 1.0f : 1.0f / sum;
-        const int64_t part = static_cast<int64_t>(slot) * a.tile_rows + t * tile_q * a.group + row;
+        const int64_t part =
+            static_cast<int64_t>(slot) * a.tile_rows + (2 * t + rank) * chunk * a.group + row;
         if (!whole && store && half == 0) {
           a.part_ml[part * 2] = m_run[t];
           a.part_ml[part * 2 + 1] = sum;
@@ -1067,7 +1210,7 @@ __global__ void __launch_bounds__(Q8P_THREADS, 1)
 #pragma unroll 1
         for (int c = 0; c < D / 64; ++c) {
           uint32_t o[32];
-          if (blocks > 0) {
+          if (some) {
             tmem_ld32(o_col + c * 32, o);
             tmem_wait_ld();
           } else {
@@ -1094,7 +1237,7 @@ __global__ void __launch_bounds__(Q8P_THREADS, 1)
       if (blocks > 0) {
         tc_fence_before();
         __syncwarp();
-        if (lane == 0) mbar_arrive(o_empty);
+        if (lane == 0) mbar_arrive_cluster(o_empty0);
         ++items;
       }
       left -= n;
@@ -1105,9 +1248,10 @@ __global__ void __launch_bounds__(Q8P_THREADS, 1)
   }
   tc_fence_before();
   __syncthreads();
+  cluster_sync();  // the products have drained; neither CTA's memory is in use any more
   if (warp == 1) {
     tc_fence_after();
-    tmem_dealloc(tmem, 512);
+    tmem_dealloc_pair(tmem, 512);
   }
 }
 

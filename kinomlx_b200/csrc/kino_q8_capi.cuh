@@ -145,10 +145,10 @@ kino_status plan_q8_attention(const kino_q8_cache* c, const kino_q8_attention_ar
   // kernels take any).
   const int64_t rows = (g->rows + c->batch - 1) / c->batch * group;
   p->decode_tiles = rows <= 8 ? 1 : rows <= 16 ? 2 : 0;
-  const int64_t tile = p->decode_tiles ? 8 * p->decode_tiles : 256;
-  p->tile_tokens = static_cast<int>(p->decode_tiles ? tile / group : 2 * (128 / group));
+  const int64_t tile = p->decode_tiles ? 8 * p->decode_tiles : 512;
+  p->tile_tokens = static_cast<int>(p->decode_tiles ? tile / group : 4 * (128 / group));
   p->tile_rows = static_cast<int>(tile);
-  p->runs = device_sms();
+  p->runs = p->decode_tiles ? device_sms() : device_sms() / 2;  // CTAs, or pairs of them
   p->bytes = 2LL * p->runs * tile * (c->dim + 2) * 4;
   return KINO_OK;
 }
@@ -184,14 +184,14 @@ kino_status launch_q8_attention(const kino_q8_cache* c, kino::Q8Attn& a, int dec
                             static_cast<uint64_t>(a.rows.rows)};
   const uint64_t strides[2] = {static_cast<uint64_t>(a.hs_q), static_cast<uint64_t>(a.ld_q)};
   const uint32_t box[3] = {64, static_cast<uint32_t>(a.group),
-                           static_cast<uint32_t>(a.tile_tokens / 2)};
+                           static_cast<uint32_t>(a.tile_tokens / 4)};
   kino_status st = make_map(&mq, a.q, 3, dims, strides, box);
   if (st != KINO_OK) return st;
-  using L = kino::Q8PrefillSmem;
+  using L = kino::Q8PrefillSmem<D>;
   constexpr auto kernel = kino::attention_q8_prefill_kernel<D, FMT>;
   st = q8_smem<kernel>(L::TOTAL);
   if (st != KINO_OK) return st;
-  launch_pdl(kernel, dim3(a.runs), dim3(kino::Q8P_THREADS), L::TOTAL, stream, mq, a);
+  launch_ex(kernel, dim3(2 * a.runs), dim3(kino::Q8P_THREADS), L::TOTAL, stream, 2, mq, a);
   if (a.runs > 1)
     launch_pdl(kino::attention_q8_combine_kernel<D, kino::Q8P_BN>, dim3(a.runs - 1, 16), dim3(256),
                0, stream, a);

@@ -97,6 +97,35 @@ __device__ __forceinline__ uint32_t q8_pair(uint32_t a, uint32_t b, int i, int j
   }
 }
 
+// The same as exact f16 pairs. int8: 0x64 in front of code + 128 is the f16 1024 + code + 128.
+// e4m3: the value times 2^(7 - 15), subnormals included; q8_f16_unit restores it.
+template <int FMT>
+__device__ __forceinline__ uint32_t q8_f16_bias(uint32_t w) {  // once for four codes
+  return FMT == Q8_INT8 ? w ^ 0x80808080u : w;
+}
+template <int FMT>
+__device__ __forceinline__ uint32_t q8_f16_of(uint32_t spread) {
+  uint32_t r;
+  if constexpr (FMT == Q8_INT8) {
+    asm("sub.rn.f16x2 %0, %1, %2;" : "=r"(r) : "r"(spread), "r"(0x64806480u));  // 1152
+  } else {
+    r = ((spread >> 1) & 0x3F803F80u) | (spread & 0x80008000u);
+  }
+  return r;
+}
+// Bytes 2 h, 2 h + 1 of a biased word.
+template <int FMT>
+__device__ __forceinline__ uint32_t q8_f16_pair(uint32_t w, int h) {
+  if constexpr (FMT == Q8_INT8)
+    return q8_f16_of<FMT>(__byte_perm(w, 0x64646464u, h ? 0x4342 : 0x4140));
+  else
+    return q8_f16_of<FMT>(__byte_perm(w, 0u, h ? 0x3424 : 0x1404));
+}
+template <int FMT>
+__device__ __forceinline__ constexpr float q8_f16_unit() {
+  return FMT == Q8_INT8 ? 1.0f : 256.0f;
+}
+
 // Four consecutive codes as fp32 values.
 template <int FMT>
 __device__ __forceinline__ void q8_decode4(uint32_t w, float (&f)[4]) {

@@ -105,14 +105,15 @@ def cached(codes, scales, table_row, length: int) -> torch.Tensor:
 
 def attention(q, k_codes, v_codes, k_scales, v_scales, table, lengths, starts=None, *, causal=True,
               scale=None):
-    """(out, weight, reach) float64 like q: softmax attention, zeros for rows without keys; weight
-    = softmax @ |v|, and reach = the largest sum of |q k| * scale a row meets: what the rounding
-    errors of an implementation in shorter types scale with."""
+    """(out, weight, reach, crowd) float64 like q: softmax attention, zeros for rows without keys.
+    What the rounding errors of an implementation in shorter types scale with: weight = softmax @
+    |v|, reach = the largest sum of |q k| * scale a row meets, crowd = the keys it sees times the
+    largest value that any of their V blocks can hold."""
     rows, heads, dim = q.shape
     group = heads // k_codes.shape[1]
     scale = dim**-0.5 if scale is None else scale
     out, weight = (torch.zeros(q.shape, dtype=F64) for _ in range(2))
-    reach = torch.zeros((rows, heads, 1), dtype=F64)
+    reach, crowd = (torch.zeros((rows, heads, 1), dtype=F64) for _ in range(2))
     for b, (first, n) in enumerate(rows_of(starts, len(lengths), rows)):
         length = int(lengths[b])
         k = cached(k_codes, k_scales, table[b], length)
@@ -127,4 +128,7 @@ def attention(q, k_codes, v_codes, k_scales, v_scales, table, lengths, starts=No
                 out[first + i, h] = p @ vv
                 weight[first + i, h] = p @ vv.abs()
                 reach[first + i, h] = (kk.abs() @ x.abs()).max() * scale
-    return out, weight, reach
+                blocks = [int(p) for p in table[b][: -(-seen // k_codes.shape[2])]]
+                crowd[first + i, h] = (seen * TOP[v_codes.dtype]
+                                       * v_scales[blocks, h // group].to(F64).max())
+    return out, weight, reach, crowd

@@ -275,20 +275,22 @@ def _attend(cuda_device, held, new, heads, group, dim, block, dtype, *, causal=T
         starts.to(cuda_device) if packed else None, causal=causal, scale=scale, out=out)
     ops.device_status()
     assert got is out and bool((out[rows:] == 5).all())
-    want, weight, reach = ref.attention(q[:rows], cpu.k_codes, cpu.v_codes, cpu.k_scales,
-                                        cpu.v_scales, table, lengths, starts, causal=causal,
-                                        scale=scale)
-    return out[:rows].cpu(), want, weight, reach
+    want = ref.attention(q[:rows], cpu.k_codes, cpu.v_codes, cpu.k_scales, cpu.v_scales, table,
+                         lengths, starts, causal=causal, scale=scale)
+    return out[:rows].cpu(), *want
 
 
-def _check_attention(got, want, weight, reach):
-    # probabilities and the result are rounded to bf16 (2^-8 of each term); a score's fp32 sum of
-    # up to 128 products and its scaling move it by at most 132 * 2^-24 of the sum of magnitudes,
-    # numerator and denominator alike; exponentials 2^-21
+def _check_attention(got, want, weight, reach, crowd):
+    # A score's fp32 sum of up to 128 products and its scaling move it by at most 132 * 2^-24 of the
+    # sum of magnitudes, numerator and denominator alike; exponentials 2^-20. The weights
+    # P = vs exp(s - m) are rounded to f16: 2^-11 of each, and 2^-25 where they are below 2^-14. The
+    # largest P of a row is at least 1, so the row sum of P / vs is at least 1 / (largest vs), and
+    # the latter is at most 2^-25 * sum |code| * (largest vs) <= 2^-25 * crowd. The result is
+    # rounded to bf16, 2^-8 of it.
     dim = want.shape[-1]
-    per = 2.0**-8 * 1.01 + 2 * ((dim + 4) * 2.0**-24 * reach + 2.0**-20)
+    inner = (2.0**-11 + 2 * ((dim + 4) * 2.0**-24 * reach + 2.0**-20)) * weight + 2.0**-25 * crowd
     off = (got.double() - want).abs()
-    limit = per * weight + 2.0**-8 * (want.abs() + per * weight) + 1e-30
+    limit = inner + 2.0**-8 * (want.abs() + inner) + 1e-30
     assert got.isfinite().all()
     assert bool((off <= limit).all()), float((off / limit).max())
 
