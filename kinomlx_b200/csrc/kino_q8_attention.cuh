@@ -613,7 +613,7 @@ __global__ void __launch_bounds__(Q8D_THREADS, 1)
 // against 1100 for 4608 queries x 9216 keys x 24 heads of 128).
 //   warp 0        Q chunks by TMA, when the last item's first products are done
 //   warp 1        tensor memory; in the even CTA the products
-//   warps 2..9    softmax of the CTA's rows (two warps a lane quarter, 64 of the keys each)
+//   warps 2..9    softmax of the CTA's rows, a warpgroup for each tile
 //   warps 10..13  codes -> bf16 (K), f16 (V) in the layout TMA would write (128-byte swizzle);
 //                 each thread keeps the next block's codes in registers
 // Tensor memory as in the dense kernel: S_A, S_B, O_A, O_B. All roles of both CTAs walk the same
@@ -632,16 +632,14 @@ struct Q8PrefillSmem {
   static constexpr int KV_OFF = 4 * HALF;
   static constexpr int STAGE = K_BYTES + V_BYTES;
   static constexpr int STAGES = 4;
-  static constexpr int X_OFF = KV_OFF + STAGES * STAGE;  // maxima [tile][parity][half][128]
-  static constexpr int L_OFF = X_OFF + 2 * 2 * 2 * 128 * 4;  // sums [tile][half][128]
-  static constexpr int SC_OFF = L_OFF + 2 * 2 * 128 * 4;
+  static constexpr int SC_OFF = KV_OFF + STAGES * STAGE;
   // a stage's 8 groups of 16 keys: K scales (with the softmax scale), 1 / vs, log2(vs), a mask of
   // the groups that are there
   static constexpr int SC = 112;
   static constexpr int BAR_OFF = SC_OFF + STAGES * SC;
   // q_full, q_empty, kv_full[S], kv_empty[S], sc_full[S], s_full[2], p_full[2], o_full, o_empty,
-  // drain, xbar[4][2][2], lbar[4]
-  static constexpr int NBAR = 2 + 3 * STAGES + 2 + 2 + 3 + 16 + 4;
+  // drain
+  static constexpr int NBAR = 2 + 3 * STAGES + 2 + 2 + 3;
   static constexpr int TOTAL = BAR_OFF + NBAR * 8 + 64 + 1024;
 };
 
@@ -689,14 +687,10 @@ __global__ void __launch_bounds__(Q8P_THREADS, 1)
   uint64_t* o_full = p_full + 2;
   uint64_t* o_empty = o_full + 1;               // even CTA's
   uint64_t* drain = o_empty + 1;
-  uint64_t* xbar = drain + 1;                   // [quarter][tile][parity]
-  uint64_t* lbar = xbar + 16;                   // [quarter]
   int64_t* s_run = reinterpret_cast<int64_t*>(bars + L::NBAR);  // u0, u1, at
   int* s_item = reinterpret_cast<int*>(s_run + 3);              // b, tile, head
   volatile int* abort_flag = s_item + 3;
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(s_item + 4);
-  float* xmax = reinterpret_cast<float*>(smem + L::X_OFF);
-  float* xsum = reinterpret_cast<float*>(smem + L::L_OFF);
 
   const int warp = warp_id();
   const int lane = static_cast<int>(lane_id());
@@ -730,13 +724,11 @@ __global__ void __launch_bounds__(Q8P_THREADS, 1)
       }
       for (int t = 0; t < 2; ++t) {
         mbar_init(&s_full[t], 1);
-        mbar_init(&p_full[t], 16);  // the softmax warps of both CTAs
+        mbar_init(&p_full[t], 8);  // the tile's softmax warps of both CTAs
       }
       mbar_init(o_full, 1);
       mbar_init(o_empty, 16);
       mbar_init(drain, 1);
-      for (int i = 0; i < 16; ++i) mbar_init(&xbar[i], 64);
-      for (int i = 0; i < 4; ++i) mbar_init(&lbar[i], 64);
       fence_barrier_init();
     }
     __syncwarp();
@@ -812,7 +804,7 @@ __global__ void __launch_bounds__(Q8P_THREADS, 1)
             smem_u32(smem + L::KV_OFF + (jb % L::STAGES) * L::STAGE + L::K_BYTES);
 #pragma unroll
         for (int kk = 0; kk < Q8P_BN / 16; ++kk)
-          umma_f16_ts_pair(tmem + 256 + t * 128, tmem + t * 128 + kk * 8 + (kk >= 4 ? 32 : 0),
+          umma_f16_ts_pair(tmem + 256 + t * 128, tmem + t * 128 + (kk >> 1) * 32 + (kk & 1) * 8,
                            D == 128 ? sdesc_mn128(sv + kk * 2048, L::V_BYTES)
                                     : sdesc_mn64(sv + kk * 1024),
                            idesc_o, (!first || kk > 0) ? 1u : 0u);
@@ -826,11 +818,11 @@ __global__ void __launch_bounds__(Q8P_THREADS, 1)
           const int ntile = w.count - w.tile * a.tile_tokens > 2 * chunk ? 2 : 1;
           const int na = blocks_a(ntile) - at;  // of this piece's blocks
           ok = mbar_wait(q_full, items & 1, abort_flag) &&
-               mbar_wait(&kv_full[jb % L::STAGES], (jb / L::STAGES) & 1, abort_flag) &&
-               mbar_wait(o_empty, (items & 1) ^ 1u, abort_flag);  // the last output was read
+               mbar_wait(&kv_full[jb % L::STAGES], (jb / L::STAGES) & 1, abort_flag);
           if (!ok) break;
           tc_fence_after();
           for (int t = na > 0 ? 0 : 1; t < ntile; ++t) s_mma(t, jb);
+          ok = mbar_wait(o_empty, (items & 1) ^ 1u, abort_flag);  // the last output was read
           for (int j = 0; j < n && ok; ++j, ++jb) {
             bool next_there = false;
             for (int t = j < na ? 0 : 1; t < ntile; ++t) {
@@ -1018,127 +1010,122 @@ __global__ void __launch_bounds__(Q8P_THREADS, 1)
       ++jb;
     }
   } else {
-    // ---- softmax
+    // ---- softmax: one row a thread, its 128 scores in chunks of 32 that are read twice (for the
+    // maximum, then for P), so that both tiles' warps fit and no row is shared between threads
+    const int t = (warp - 2) >> 2;
     const int quarter = warp & 3;
-    const int half = (warp - 2) >> 2;
     const int row = quarter * 32 + lane;
     const uint32_t lane_base = static_cast<uint32_t>(quarter * 32) << 16;
+    const uint32_t s_col = tmem + lane_base + t * 128;
+    const uint32_t o_col = s_col + 256;
     const int row_tok = row / a.group, row_head = row % a.group;
     const bool in_row = row < chunk * a.group;
-    const uint32_t p_full0 = cluster_addr(smem_u32(&p_full[0]), 0);
+    const uint32_t p_full0 = cluster_addr(smem_u32(&p_full[t]), 0);
     const uint32_t o_empty0 = cluster_addr(smem_u32(o_empty), 0);
     int items = 0, jb = 0, piece = 0;
-    int cnt[2] = {0, 0};
+    int cnt = 0;  // blocks of this tile
     bool ok = true;
-    while (left > 0 && ok) {
+    while (left > 0) {
       const int n = static_cast<int>(left < w.units - at ? left : w.units - at);
       const bool whole = n == w.units;
       const int keys = Work::keys(a, w.count, w.len, w.tile);
-      const int tok0 = w.tile * a.tile_tokens + rank * chunk;  // of tile A; tile B 2 chunks on
       const int ntile = w.count - w.tile * a.tile_tokens > 2 * chunk ? 2 : 1;
-      int limit[2], least[2];  // keys that this row sees; the least of the warp's rows
-#pragma unroll
-      for (int t = 0; t < 2; ++t) {
-        const int tok = tok0 + t * 2 * chunk + row_tok;
-        const bool live = in_row && tok < w.count;
-        // rows of no query are computed with whatever is there and not stored
-        limit[t] = !live ? 0x7fffffff
-                         : a.causal ? max(0, min(keys, w.len - w.count + tok + 1)) : keys;
-        least[t] = __reduce_min_sync(0xffffffffu, limit[t]);
-      }
-      float m_run[2] = {-INFINITY, -INFINITY};
-      float l_run[2] = {0.0f, 0.0f};
-      const int blocks = keys > 0 ? n : 0;
-      const int na = keys > 0 ? blocks_a(ntile) - at : 0;
-      for (int j = 0; j < blocks && ok; ++j, ++jb) {
-        const int stage = jb % L::STAGES;
-        const uint8_t* sc = smem + L::SC_OFF + stage * L::SC;
-        const int key0 = (at + j) * Q8P_BN + half * 64;
+      const int tok = w.tile * a.tile_tokens + (2 * t + rank) * chunk + row_tok;
+      const bool live = in_row && tok < w.count;
+      // keys that this row sees (rows of no query are computed with whatever is there and not
+      // stored), and the least of the warp's rows
+      const int limit = !live ? 0x7fffffff
+                              : a.causal ? max(0, min(keys, w.len - w.count + tok + 1)) : keys;
+      const int least = __reduce_min_sync(0xffffffffu, limit);
+      int blocks = 0;  // that the tile takes part in
+      if (keys > 0 && t < ntile) blocks = t == 1 ? n : min(n, blocks_a(ntile) - at);
+      float m_run = -INFINITY, l_run = 0.0f;
+      for (int j = 0; j < blocks; ++j) {
+        const int stage = (jb + j) % L::STAGES;
+        const int key0 = (at + j) * Q8P_BN;
         ok = __all_sync(0xffffffffu,
-                        mbar_wait(&sc_full[stage], (jb / L::STAGES) & 1, abort_flag));
+                        mbar_wait(&sc_full[stage], ((jb + j) / L::STAGES) & 1, abort_flag) &&
+                            mbar_wait(&s_full[t], cnt & 1, abort_flag));
         if (!ok) break;
-        const float4* sc4 = reinterpret_cast<const float4*>(sc);
-        const unsigned groups = (reinterpret_cast<const unsigned*>(sc)[24] >> (half * 4)) & 15u;
-        for (int t = j < na ? 0 : 1; t < ntile; ++t) {
-          ok = __all_sync(0xffffffffu, mbar_wait(&s_full[t], cnt[t] & 1, abort_flag));
-          if (!ok) break;
-          tc_fence_after();
-          const uint32_t s_col = tmem + lane_base + t * 128 + half * 64;
-          uint32_t sr[2][32];
-          tmem_ld32(s_col, sr[0]);
-          tmem_ld32(s_col + 32, sr[1]);
+        tc_fence_after();
+        // Row i of the tile keeps one reference m, and the second product's operand is
+        //   P = vs exp2(s ks - m) = exp2(s ks + log2(vs) - m),
+        // so the reference follows the largest s ks + log2(vs) and P stays within f16's range
+        // whatever the blocks' V scales are; the row sum takes a group's sum of P over vs.
+        const float* sc = reinterpret_cast<const float*>(smem + L::SC_OFF + stage * L::SC);
+        const unsigned groups = reinterpret_cast<const unsigned*>(sc)[24];
+        const bool masked = key0 + Q8P_BN > least || groups != 255u;  // warp-uniform
+        const int valid = masked ? limit - key0 : Q8P_BN;
+        uint32_t sr[2][32];
+        float mine = -INFINITY;
+        tmem_ld32(s_col, sr[0]);
+#pragma unroll
+        for (int c = 0; c < 4; ++c) {
           tmem_wait_ld();
-          // Row i of the tile keeps one reference m, and the second product's operand is
-          //   P = vs exp2(s ks - m) = exp2(s ks + log2(vs) - m),
-          // so the reference follows the largest s ks + log2(vs) and P stays within f16's range
-          // whatever the blocks' V scales are; the row sum takes a group's sum of P over vs.
-          const float4 k4 = sc4[half], r4 = sc4[2 + half], g4 = sc4[4 + half];
-          const float ks[4] = {k4.x, k4.y, k4.z, k4.w}, rv[4] = {r4.x, r4.y, r4.z, r4.w};
-          const float lv[4] = {g4.x, g4.y, g4.z, g4.w};
-          const bool masked = key0 + 64 > least[t] || groups != 15u;  // warp-uniform
-          const int valid = masked ? limit[t] - key0 : 64;
-          if (masked) {
+          if (c < 3) tmem_ld32(s_col + (c + 1) * 32, sr[(c + 1) & 1]);
 #pragma unroll
-            for (int i = 0; i < 64; ++i)
-              if (i >= valid || !((groups >> (i >> 4)) & 1))
-                sr[i >> 5][i & 31] = __float_as_uint(-INFINITY);
-          }
-          float mine = -INFINITY;
+          for (int q = 0; q < 2; ++q) {
+            const uint32_t* v = sr[c & 1] + q * 16;
+            const int g = 2 * c + q;
+            float x;
+            if (masked) {
+              x = -INFINITY;
 #pragma unroll
-          for (int q = 0; q < 4; ++q) {
-            const uint32_t* v = sr[q >> 1] + (q & 1) * 16;
-            float x = max3f(__uint_as_float(v[0]), __uint_as_float(v[1]), __uint_as_float(v[2]));
-            x = max3f(x, __uint_as_float(v[3]), __uint_as_float(v[4]));
-            x = max3f(x, __uint_as_float(v[5]), __uint_as_float(v[6]));
-            x = max3f(x, __uint_as_float(v[7]), __uint_as_float(v[8]));
-            x = max3f(x, __uint_as_float(v[9]), __uint_as_float(v[10]));
-            x = max3f(x, __uint_as_float(v[11]), __uint_as_float(v[12]));
-            x = max3f(x, __uint_as_float(v[13]), __uint_as_float(v[14]));
-            x = fmaxf(x, __uint_as_float(v[15]));
-            // scales are not negative; a masked group stays at -inf whatever its scale is
-            const float y = fmaf(x, ks[q], lv[q]);
-            mine = fmaxf(mine, masked && x == -INFINITY ? x : y);
-          }
-          float* xm = xmax + (t * 2 + (cnt[t] & 1)) * 256;
-          xm[half * 128 + row] = mine;
-          uint64_t* xb = &xbar[(quarter * 2 + t) * 2 + (cnt[t] & 1)];
-          mbar_arrive(xb);
-          ok = __all_sync(0xffffffffu, mbar_wait(xb, (cnt[t] >> 1) & 1, abort_flag));
-          if (!ok) break;
-          const float m_blk = fmaxf(mine, xm[(1 - half) * 128 + row]);
-          float alpha = 1.0f;
-          bool rescale = false;
-          if (j > 0) {
-            const bool need = m_blk > m_run[t] + 8.0f;
-            rescale = __any_sync(0xffffffffu, need);
-            if (need) {
-              alpha = ex2_approx(m_run[t] - m_blk);
-              m_run[t] = m_blk;
-              l_run[t] *= alpha;
+              for (int i = 0; i < 16; ++i)
+                x = fmaxf(x, g * 16 + i < valid ? __uint_as_float(v[i]) : -INFINITY);
+            } else {
+              x = max3f(__uint_as_float(v[0]), __uint_as_float(v[1]), __uint_as_float(v[2]));
+              x = max3f(x, __uint_as_float(v[3]), __uint_as_float(v[4]));
+              x = max3f(x, __uint_as_float(v[5]), __uint_as_float(v[6]));
+              float y = max3f(__uint_as_float(v[7]), __uint_as_float(v[8]), __uint_as_float(v[9]));
+              y = max3f(y, __uint_as_float(v[10]), __uint_as_float(v[11]));
+              y = max3f(y, __uint_as_float(v[12]), __uint_as_float(v[13]));
+              x = fmaxf(max3f(x, y, __uint_as_float(v[14])), __uint_as_float(v[15]));
             }
-          } else {
-            m_run[t] = m_blk;
+            // scales are not negative; a masked group stays at -inf whatever its scales are
+            const float y = fmaf(x, sc[g], sc[16 + g]);
+            mine = fmaxf(mine, masked && (g * 16 >= valid || !((groups >> g) & 1)) ? -INFINITY : y);
           }
-          const float ref = m_run[t] == -INFINITY ? 0.0f : m_run[t];
-          float l_blk = 0.0f;
-          auto exps = [&](auto tag) {
-            constexpr bool MASKED = decltype(tag)::value;
+        }
+        // The reference moves only when it is exceeded by 2^8 (the stale one cancels in the
+        // division). O holds the products of the blocks before this one.
+        float alpha = 1.0f;
+        bool rescale = false;
+        if (j > 0) {
+          const bool need = mine > m_run + 8.0f;
+          rescale = __any_sync(0xffffffffu, need);
+          if (need) {
+            alpha = ex2_approx(m_run - mine);
+            m_run = mine;
+            l_run *= alpha;
+          }
+        } else {
+          m_run = mine;
+        }
+        const float ref = m_run == -INFINITY ? 0.0f : m_run;
+        auto exps = [&](auto tag) {
+          constexpr bool MASKED = decltype(tag)::value;
+          // chunk 3 is still in registers
 #pragma unroll
-            for (int q8 = 0; q8 < 4; ++q8) {
-              uint32_t packed[8];
-              const uint64_t k2 = f2_pack(ks[q8], ks[q8]);
-              const float c = lv[q8] - ref;
-              const uint64_t c2 = f2_pack(c, c);
+          for (int k = 0; k < 4; ++k) {
+            const int c = (k + 3) & 3;
+            const uint32_t(&x32)[32] = sr[(k + 1) & 1];
+            if (k > 0) tmem_wait_ld();
+            if (k < 3) tmem_ld32(s_col + ((c + 1) & 3) * 32, sr[k & 1]);
+            uint32_t packed[16];
+#pragma unroll
+            for (int q = 0; q < 2; ++q) {
+              const int g = 2 * c + q;
+              const float kg = sc[g], cg = sc[16 + g] - ref;
+              const uint64_t k2 = f2_pack(kg, kg), c2 = f2_pack(cg, cg);
               uint64_t sum2[2] = {f2_pack(0.0f, 0.0f), f2_pack(0.0f, 0.0f)};
 #pragma unroll
               for (int u = 0; u < 8; ++u) {
-                const int i = q8 * 8 + u;
-                const uint32_t* v = sr[i >> 4];
-                const int e = (2 * i) & 31;
-                const uint64_t xs =
-                    f2_fma(f2_pack(__uint_as_float(v[e]), __uint_as_float(v[e + 1])), k2, c2);
+                const int e = q * 16 + 2 * u;
+                const uint64_t xs = f2_fma(
+                    f2_pack(__uint_as_float(x32[e]), __uint_as_float(x32[e + 1])), k2, c2);
                 uint64_t ev;
-                if ((ATT_EMU_MASK >> (i & 7)) & 1) {
+                if ((ATT_EMU_MASK >> u) & 1) {
                   ev = exp2_poly_x2(xs);
                 } else {
                   const float2 xv = f2_unpack(xs);
@@ -1146,95 +1133,85 @@ __global__ void __launch_bounds__(Q8P_THREADS, 1)
                 }
                 float2 p2 = f2_unpack(ev);
                 if constexpr (MASKED) {  // a masked key counts for nothing, its scales may be NaN
-                  const bool g = (groups >> q8) & 1;
-                  p2.x = g && 2 * i < valid ? p2.x : 0.0f;
-                  p2.y = g && 2 * i + 1 < valid ? p2.y : 0.0f;
+                  const bool in = (groups >> g) & 1;
+                  p2.x = in && c * 32 + e < valid ? p2.x : 0.0f;
+                  p2.y = in && c * 32 + e + 1 < valid ? p2.y : 0.0f;
                   ev = f2_pack(p2.x, p2.y);
                 }
                 sum2[u & 1] = f2_add(sum2[u & 1], ev);
-                packed[u] = pack_f16x2(p2.x, p2.y);
+                packed[q * 8 + u] = pack_f16x2(p2.x, p2.y);
               }
-              tmem_st8(s_col + q8 * 8, packed);
               const float2 s2 = f2_unpack(f2_add(sum2[0], sum2[1]));
-              if (!MASKED || (((groups >> q8) & 1) && q8 * 16 < valid))
-                l_blk = fmaf(s2.x + s2.y, rv[q8], l_blk);
+              if (!MASKED || (((groups >> g) & 1) && g * 16 < valid))
+                l_run = fmaf(s2.x + s2.y, sc[8 + g], l_run);
             }
-          };
-          if (masked)
-            exps(std::true_type{});
-          else
-            exps(std::false_type{});
-          l_run[t] += l_blk;
-          if (rescale) {
-            const uint32_t o_col = tmem + lane_base + 256 + t * 128 + half * (D / 2);
-#pragma unroll 1
-            for (int c = 0; c < D / 64; ++c) {
-              uint32_t o[32];
-              tmem_ld32(o_col + c * 32, o);
-              tmem_wait_ld();
-#pragma unroll
-              for (int i = 0; i < 32; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * alpha);
-              tmem_st32(o_col + c * 32, o);
-            }
+            // P of keys 32c .. over the first half of the chunk's own scores
+            tmem_st8(s_col + c * 32, *reinterpret_cast<const uint32_t(*)[8]>(packed));
+            tmem_st8(s_col + c * 32 + 8, *reinterpret_cast<const uint32_t(*)[8]>(packed + 8));
           }
-          tmem_wait_st();
-          tc_fence_before();
-          __syncwarp();
-          if (lane == 0) mbar_arrive_cluster(p_full0 + t * 8);
-          ++cnt[t];
+        };
+        if (masked)
+          exps(std::true_type{});
+        else
+          exps(std::false_type{});
+        if (rescale) {
+#pragma unroll 1
+          for (int c = 0; c < D / 32; ++c) {
+            uint32_t o[32];
+            tmem_ld32(o_col + c * 32, o);
+            tmem_wait_ld();
+#pragma unroll
+            for (int i = 0; i < 32; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * alpha);
+            tmem_st32(o_col + c * 32, o);
+          }
         }
+        tmem_wait_st();
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive_cluster(p_full0);
+        ++cnt;
       }
-      if (!ok) break;
-      if (blocks > 0) {
-        for (int t = 0; t < ntile; ++t) xsum[(t * 2 + half) * 128 + row] = l_run[t];
-        mbar_arrive(&lbar[quarter]);
-        ok = __all_sync(0xffffffffu, mbar_wait(&lbar[quarter], items & 1, abort_flag) &&
-                                         mbar_wait(o_full, items & 1, abort_flag));
+      if (keys > 0) {
+        ok = ok && __all_sync(0xffffffffu, mbar_wait(o_full, items & 1, abort_flag));
         if (!ok) break;
         tc_fence_after();
+        jb += n;
       }
-      const int slot = 2 * pair + (piece > 0 ? 1 : 0);
-      for (int t = 0; t < ntile; ++t) {
-        const bool some = blocks > 0 && (t == 1 || na > 0);  // the tile's output was written
-        const int tok = tok0 + t * 2 * chunk + row_tok;
-        const bool store = in_row && tok < w.count;
-        const float sum = some ? l_run[t] + xsum[(t * 2 + 1 - half) * 128 + row] : 0.0f;
-        const float inv = m_run[t] == -INFINITY ? 1.0f : 1.0f / sum;
-        const int64_t part =
-            static_cast<int64_t>(slot) * a.tile_rows + (2 * t + rank) * chunk * a.group + row;
-        if (!whole && store && half == 0) {
-          a.part_ml[part * 2] = m_run[t];
-          a.part_ml[part * 2 + 1] = sum;
+      if (t < ntile) {
+        const float inv = m_run == -INFINITY ? 1.0f : 1.0f / l_run;
+        const int64_t part = static_cast<int64_t>(2 * pair + (piece > 0 ? 1 : 0)) * a.tile_rows +
+                             (2 * t + rank) * chunk * a.group + row;
+        if (!whole && live) {
+          a.part_ml[part * 2] = m_run;
+          a.part_ml[part * 2 + 1] = l_run;
         }
-        const uint32_t o_col = tmem + lane_base + 256 + t * 128 + half * (D / 2);
+        __nv_bfloat16* out = a.out + (w.first + tok) * a.ld_out +
+                             static_cast<int64_t>(w.head * a.group + row_head) * a.hs_out;
 #pragma unroll 1
-        for (int c = 0; c < D / 64; ++c) {
+        for (int c = 0; c < D / 32; ++c) {
           uint32_t o[32];
-          if (some) {
+          if (blocks > 0) {
             tmem_ld32(o_col + c * 32, o);
             tmem_wait_ld();
           } else {
 #pragma unroll
             for (int i = 0; i < 32; ++i) o[i] = 0;
           }
-          const int col = half * (D / 2) + c * 32;
-          if (store && whole) {
+          if (live && whole) {
             uint32_t w16[16];
 #pragma unroll
             for (int i = 0; i < 16; ++i)
               w16[i] = pack_bf16x2(__uint_as_float(o[2 * i]) * inv, __uint_as_float(o[2 * i + 1]) * inv);
-            store_row32(a.out + (w.first + tok) * a.ld_out +
-                            static_cast<int64_t>(w.head * a.group + row_head) * a.hs_out + col,
-                        w16, 32);
-          } else if (store) {
-            uint4* dst = reinterpret_cast<uint4*>(a.part_o + part * D + col);
+            store_row32(out + c * 32, w16, 32);
+          } else if (live) {
+            uint4* dst = reinterpret_cast<uint4*>(a.part_o + part * D + c * 32);
 #pragma unroll
             for (int i = 0; i < 8; ++i)
               dst[i] = make_uint4(o[4 * i], o[4 * i + 1], o[4 * i + 2], o[4 * i + 3]);
           }
         }
       }
-      if (blocks > 0) {
+      if (keys > 0) {
         tc_fence_before();
         __syncwarp();
         if (lane == 0) mbar_arrive_cluster(o_empty0);
