@@ -37,6 +37,7 @@ struct Q8Attn {
   const int32_t* lengths;
   Q8Rows rows;
   int batch, heads, group, block, num_blocks;
+  int block_shift;  // log2(block)
   float scale_log2;
   int causal;
   int tile_tokens;  // query tokens of an item
@@ -280,10 +281,10 @@ __global__ void __launch_bounds__(Q8D_THREADS, 1)
         int row = -1;
         float ks = 0.0f, rv = 0.0f, lv = 0.0f;
         if (u + lane / per < n && key < keys) {
-          const int page = table[key / a.block];
+          const int page = table[key >> a.block_shift];
           if (page >= 0 && page < a.num_blocks) {
             const int unit = page * a.heads + w.head;
-            row = unit * a.block + key % a.block;
+            row = unit * a.block + (key & (a.block - 1));
             // the codes stand in f16 as their value over q8_f16_unit, those of K and of V
             ks = a.scales[0][unit] * a.scale_log2 * q8_f16_unit<FMT>();
             const float vs = a.scales[1][unit];
@@ -612,8 +613,10 @@ __global__ void __launch_bounds__(Q8D_THREADS, 1)
 // the conversion and the shared-memory traffic that bound the same kernel on single CTAs (1400 us
 // against 1100 for 4608 queries x 9216 keys x 24 heads of 128).
 //   warp 0        Q chunks by TMA, when the last item's first products are done
-//   warp 1        tensor memory; in the even CTA the products
-//   warps 2..9    softmax of the CTA's rows, a warpgroup for each tile
+//   warp 1        tensor memory; in the even CTA the products, in the odd one the word to the
+//                 even one that a block's converted operands are there (by a thread without loads
+//                 in flight, which a release at cluster scope would wait for)
+//   warps 2..9    softmax of the CTA's rows, four warps for each tile
 //   warps 10..13  codes -> bf16 (K), f16 (V) in the layout TMA would write (128-byte swizzle);
 //                 each thread keeps the next block's codes in registers
 // Tensor memory as in the dense kernel: S_A, S_B, O_A, O_B. All roles of both CTAs walk the same
@@ -621,7 +624,11 @@ __global__ void __launch_bounds__(Q8D_THREADS, 1)
 // under a causal mask and leaves the blocks behind it out.
 constexpr int Q8P_BN = 128;
 constexpr int Q8P_THREADS = 448;
-
+// Pairs of a group of 16 keys whose exponentials run on the FMA pipes (as ATT_EMU_MASK).
+#ifndef KINO_Q8P_EMU_MASK
+#define KINO_Q8P_EMU_MASK 0x00
+#endif
+constexpr unsigned Q8P_EMU_MASK = KINO_Q8P_EMU_MASK;
 template <int D>
 struct Q8PrefillSmem {
   static constexpr int HALF = 128 * 64 * 2;  // Q: 128 rows x 64 dims
@@ -637,7 +644,7 @@ struct Q8PrefillSmem {
   // the groups that are there
   static constexpr int SC = 112;
   static constexpr int BAR_OFF = SC_OFF + STAGES * SC;
-  // q_full, q_empty, kv_full[S], kv_empty[S], sc_full[S], s_full[2], p_full[2], o_full, o_empty,
+  // q_full, q_empty, kv_full[S], kv_empty[S], kv_peer[S], s_full[2], p_full[2], o_full, o_empty,
   // drain
   static constexpr int NBAR = 2 + 3 * STAGES + 2 + 2 + 3;
   static constexpr int TOTAL = BAR_OFF + NBAR * 8 + 64 + 1024;
@@ -679,10 +686,10 @@ __global__ void __launch_bounds__(Q8P_THREADS, 1)
   uint64_t* bars = reinterpret_cast<uint64_t*>(smem + L::BAR_OFF);
   uint64_t* q_full = bars;                      // even CTA's
   uint64_t* q_empty = bars + 1;
-  uint64_t* kv_full = bars + 2;                 // even CTA's
+  uint64_t* kv_full = bars + 2;                 // this CTA's converted operands and scales
   uint64_t* kv_empty = kv_full + L::STAGES;
-  uint64_t* sc_full = kv_empty + L::STAGES;
-  uint64_t* s_full = sc_full + L::STAGES;
+  uint64_t* kv_peer = kv_empty + L::STAGES;     // even CTA's: the odd one's operands
+  uint64_t* s_full = kv_peer + L::STAGES;
   uint64_t* p_full = s_full + 2;                // even CTA's
   uint64_t* o_full = p_full + 2;
   uint64_t* o_empty = o_full + 1;               // even CTA's
@@ -718,9 +725,9 @@ __global__ void __launch_bounds__(Q8P_THREADS, 1)
       mbar_init(q_full, 1);
       mbar_init(q_empty, 1);
       for (int i = 0; i < L::STAGES; ++i) {
-        mbar_init(&kv_full[i], 8);  // the converting warps of both CTAs
+        mbar_init(&kv_full[i], 4);  // the converting warps
         mbar_init(&kv_empty[i], 1);
-        mbar_init(&sc_full[i], 1);
+        mbar_init(&kv_peer[i], 1);
       }
       for (int t = 0; t < 2; ++t) {
         mbar_init(&s_full[t], 1);
@@ -790,24 +797,30 @@ __global__ void __launch_bounds__(Q8P_THREADS, 1)
       constexpr uint32_t idesc_s = idesc_bf16(256, 128);
       constexpr uint32_t idesc_o = idesc_f16(256, D) | (1u << 16);  // V: MN-major
       auto s_mma = [&](int t, int jb) {
-        const uint32_t sq = smem_u32(smem + L::Q_OFF + t * 2 * L::HALF);
-        const uint32_t sk = smem_u32(smem + L::KV_OFF + (jb % L::STAGES) * L::STAGE);
+        // (descriptors hold addresses in units of 16 bytes: steps are plain additions)
+        const uint64_t sq = sdesc_k128(smem_u32(smem + L::Q_OFF + t * 2 * L::HALF));
+        const uint64_t sk =
+            sdesc_k128(smem_u32(smem + L::KV_OFF + (jb % L::STAGES) * L::STAGE));
 #pragma unroll
         for (int kk = 0; kk < D / 16; ++kk)
-          umma_bf16_pair(tmem + t * 128, sdesc_k128(sq + (kk >> 2) * L::HALF + (kk & 3) * 32),
-                         sdesc_k128(sk + (kk >> 2) * L::KHALF + (kk & 3) * 32), idesc_s,
+          umma_bf16_pair(tmem + t * 128, sq + ((kk >> 2) * L::HALF + (kk & 3) * 32) / 16,
+                         sk + ((kk >> 2) * L::KHALF + (kk & 3) * 32) / 16, idesc_s,
                          kk > 0 ? 1u : 0u);
         umma_commit_pair(&s_full[t], 0x3);
       };
       auto pv_mma = [&](int t, int jb, bool first) {
-        const uint32_t sv =
+        const uint32_t at_v =
             smem_u32(smem + L::KV_OFF + (jb % L::STAGES) * L::STAGE + L::K_BYTES);
+        const uint64_t sv = D == 128 ? sdesc_mn128(at_v, L::V_BYTES) : sdesc_mn64(at_v);
 #pragma unroll
         for (int kk = 0; kk < Q8P_BN / 16; ++kk)
           umma_f16_ts_pair(tmem + 256 + t * 128, tmem + t * 128 + (kk >> 1) * 32 + (kk & 1) * 8,
-                           D == 128 ? sdesc_mn128(sv + kk * 2048, L::V_BYTES)
-                                    : sdesc_mn64(sv + kk * 1024),
-                           idesc_o, (!first || kk > 0) ? 1u : 0u);
+                           sv + kk * 16 * D / 16, idesc_o, (!first || kk > 0) ? 1u : 0u);
+      };
+      auto block_there = [&](int jb) {
+        const uint32_t parity = (jb / L::STAGES) & 1;
+        return mbar_wait(&kv_full[jb % L::STAGES], parity, abort_flag) &&
+               mbar_wait(&kv_peer[jb % L::STAGES], parity, abort_flag);
       };
       int items = 0, jb = 0;
       int cnt[2] = {0, 0};  // blocks that a tile has been given
@@ -817,8 +830,7 @@ __global__ void __launch_bounds__(Q8P_THREADS, 1)
         if (Work::keys(a, w.count, w.len, w.tile) > 0) {
           const int ntile = w.count - w.tile * a.tile_tokens > 2 * chunk ? 2 : 1;
           const int na = blocks_a(ntile) - at;  // of this piece's blocks
-          ok = mbar_wait(q_full, items & 1, abort_flag) &&
-               mbar_wait(&kv_full[jb % L::STAGES], (jb / L::STAGES) & 1, abort_flag);
+          ok = mbar_wait(q_full, items & 1, abort_flag) && block_there(jb);
           if (!ok) break;
           tc_fence_after();
           for (int t = na > 0 ? 0 : 1; t < ntile; ++t) s_mma(t, jb);
@@ -834,8 +846,7 @@ __global__ void __launch_bounds__(Q8P_THREADS, 1)
               if (t == ntile - 1) umma_commit_pair(&kv_empty[jb % L::STAGES], 0x3);
               if (j + 1 < n && (t == 1 || j + 1 < na)) {
                 if (!next_there) {
-                  ok = mbar_wait(&kv_full[(jb + 1) % L::STAGES], ((jb + 1) / L::STAGES) & 1,
-                                 abort_flag);
+                  ok = block_there(jb + 1);
                   if (!ok) break;
                   tc_fence_after();
                   next_there = true;
@@ -857,6 +868,23 @@ __global__ void __launch_bounds__(Q8P_THREADS, 1)
       umma_commit_pair(drain, 0x1);
       const uint64_t t0 = global_ns();
       while (!mbar_try_wait(drain, 0) && global_ns() - t0 < 200000000ull) {
+      }
+    }
+    if (warp == 1 && lane == 0 && rank == 1) {
+      // ---- word to the even CTA
+      const uint32_t there = cluster_addr(smem_u32(kv_peer), 0);
+      int jb = 0;
+      bool ok = true;
+      while (left > 0 && ok) {
+        const int n = static_cast<int>(left < w.units - at ? left : w.units - at);
+        if (Work::keys(a, w.count, w.len, w.tile) > 0)
+          for (int j = 0; j < n && ok; ++j, ++jb) {
+            ok = mbar_wait(&kv_full[jb % L::STAGES], (jb / L::STAGES) & 1, abort_flag);
+            if (ok) mbar_arrive_cluster(there + (jb % L::STAGES) * 8);
+          }
+        left -= n;
+        at = 0;
+        if (left > 0) w.next();
       }
     }
     __syncwarp();
@@ -909,10 +937,10 @@ __global__ void __launch_bounds__(Q8P_THREADS, 1)
       if (left > 0 && lane < 8) {
         const int key = at * Q8P_BN + lane * 16;
         if (key < Work::keys(a, w.count, w.len, w.tile)) {
-          const int page = a.table[static_cast<int64_t>(w.b) * a.ld_table + key / a.block];
+          const int page = a.table[static_cast<int64_t>(w.b) * a.ld_table + (key >> a.block_shift)];
           if (page >= 0 && page < a.num_blocks) {
             const int unit = page * a.heads + w.head;
-            k_there = unit * a.block + key % a.block;
+            k_there = unit * a.block + (key & (a.block - 1));
             ks = a.scales[0][unit] * a.scale_log2;
             vs = a.scales[1][unit];
             v_there = vs <= Q8_LEAST_V ? -1 : k_there;  // taken as zero codes
@@ -1003,15 +1031,12 @@ __global__ void __launch_bounds__(Q8P_THREADS, 1)
       }
       fence_proxy_async_smem();
       __syncwarp();
-      if (lane == 0) {
-        if (cw == 0) mbar_arrive(&sc_full[stage]);
-        mbar_arrive_cluster(cluster_addr(smem_u32(&kv_full[stage]), 0));
-      }
+      if (lane == 0) mbar_arrive(&kv_full[stage]);
       ++jb;
     }
   } else {
-    // ---- softmax: one row a thread, its 128 scores in chunks of 32 that are read twice (for the
-    // maximum, then for P), so that both tiles' warps fit and no row is shared between threads
+    // ---- softmax: one row a thread, its 128 scores in chunks of 32 of which two are held at a
+    // time (read for the maximum, and the first two again for P)
     const int t = (warp - 2) >> 2;
     const int quarter = warp & 3;
     const int row = quarter * 32 + lane;
@@ -1044,7 +1069,7 @@ __global__ void __launch_bounds__(Q8P_THREADS, 1)
         const int stage = (jb + j) % L::STAGES;
         const int key0 = (at + j) * Q8P_BN;
         ok = __all_sync(0xffffffffu,
-                        mbar_wait(&sc_full[stage], ((jb + j) / L::STAGES) & 1, abort_flag) &&
+                        mbar_wait(&kv_full[stage], ((jb + j) / L::STAGES) & 1, abort_flag) &&
                             mbar_wait(&s_full[t], cnt & 1, abort_flag));
         if (!ok) break;
         tc_fence_after();
@@ -1058,11 +1083,13 @@ __global__ void __launch_bounds__(Q8P_THREADS, 1)
         const int valid = masked ? limit - key0 : Q8P_BN;
         uint32_t sr[2][32];
         float mine = -INFINITY;
-        tmem_ld32(s_col, sr[0]);
 #pragma unroll
         for (int c = 0; c < 4; ++c) {
-          tmem_wait_ld();
-          if (c < 3) tmem_ld32(s_col + (c + 1) * 32, sr[(c + 1) & 1]);
+          if ((c & 1) == 0) {
+            tmem_ld32(s_col + c * 32, sr[0]);
+            tmem_ld32(s_col + c * 32 + 32, sr[1]);
+            tmem_wait_ld();
+          }
 #pragma unroll
           for (int q = 0; q < 2; ++q) {
             const uint32_t* v = sr[c & 1] + q * 16;
@@ -1105,13 +1132,12 @@ __global__ void __launch_bounds__(Q8P_THREADS, 1)
         const float ref = m_run == -INFINITY ? 0.0f : m_run;
         auto exps = [&](auto tag) {
           constexpr bool MASKED = decltype(tag)::value;
-          // chunk 3 is still in registers
+          // chunks 2 and 3 are still in registers; 0 and 1 come back as those are done
 #pragma unroll
           for (int k = 0; k < 4; ++k) {
-            const int c = (k + 3) & 3;
-            const uint32_t(&x32)[32] = sr[(k + 1) & 1];
-            if (k > 0) tmem_wait_ld();
-            if (k < 3) tmem_ld32(s_col + ((c + 1) & 3) * 32, sr[k & 1]);
+            const int c = k ^ 2;
+            const uint32_t(&x32)[32] = sr[k & 1];
+            if (k == 3) tmem_wait_ld();
             uint32_t packed[16];
 #pragma unroll
             for (int q = 0; q < 2; ++q) {
@@ -1125,7 +1151,7 @@ __global__ void __launch_bounds__(Q8P_THREADS, 1)
                 const uint64_t xs = f2_fma(
                     f2_pack(__uint_as_float(x32[e]), __uint_as_float(x32[e + 1])), k2, c2);
                 uint64_t ev;
-                if ((ATT_EMU_MASK >> u) & 1) {
+                if ((Q8P_EMU_MASK >> u) & 1) {
                   ev = exp2_poly_x2(xs);
                 } else {
                   const float2 xv = f2_unpack(xs);
@@ -1145,9 +1171,14 @@ __global__ void __launch_bounds__(Q8P_THREADS, 1)
               if (!MASKED || (((groups >> g) & 1) && g * 16 < valid))
                 l_run = fmaf(s2.x + s2.y, sc[8 + g], l_run);
             }
-            // P of keys 32c .. over the first half of the chunk's own scores
+            // P of keys 32c .. over the first half of the chunk's scores
             tmem_st8(s_col + c * 32, *reinterpret_cast<const uint32_t(*)[8]>(packed));
             tmem_st8(s_col + c * 32 + 8, *reinterpret_cast<const uint32_t(*)[8]>(packed + 8));
+            if (k == 0) tmem_ld32(s_col, sr[0]);
+            if (k == 1) {
+              tmem_wait_ld();
+              tmem_ld32(s_col + 32, sr[1]);
+            }
           }
         };
         if (masked)
@@ -1168,7 +1199,7 @@ __global__ void __launch_bounds__(Q8P_THREADS, 1)
         tmem_wait_st();
         tc_fence_before();
         __syncwarp();
-        if (lane == 0) mbar_arrive_cluster(p_full0);
+        if (lane == 0) mbar_arrive_cluster_relaxed(p_full0);  // tensor memory only, written above
         ++cnt;
       }
       if (keys > 0) {
@@ -1214,7 +1245,7 @@ __global__ void __launch_bounds__(Q8P_THREADS, 1)
       if (keys > 0) {
         tc_fence_before();
         __syncwarp();
-        if (lane == 0) mbar_arrive_cluster(o_empty0);
+        if (lane == 0) mbar_arrive_cluster_relaxed(o_empty0);
         ++items;
       }
       left -= n;

@@ -443,6 +443,7 @@ kino_status kino_q8_attention(const kino_q8_cache* cache, const kino_q8_attentio
   a.group = static_cast<int>(args->q_heads / cache->heads);
   a.block = static_cast<int>(cache->block);
   a.num_blocks = static_cast<int>(cache->num_blocks);
+  a.block_shift = a.block == 16 ? 4 : a.block == 32 ? 5 : a.block == 64 ? 6 : 7;
   a.scale_log2 = args->scale * 1.4426950408889634f;
   a.causal = args->causal != 0;
   a.tile_tokens = p.tile_tokens;
