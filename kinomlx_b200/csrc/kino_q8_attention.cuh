@@ -640,13 +640,13 @@ struct Q8PrefillSmem {
   static constexpr int STAGE = K_BYTES + V_BYTES;
   static constexpr int STAGES = 4;
   static constexpr int SC_OFF = KV_OFF + STAGES * STAGE;
-  // a stage's 8 groups of 16 keys: K scales (with the softmax scale), 1 / vs, log2(vs), a mask of
+  // a stage's 8 groups of 16 keys: (K scale times the softmax scale, log2(vs)) each, and a mask of
   // the groups that are there
-  static constexpr int SC = 112;
+  static constexpr int SC = 80;
   static constexpr int BAR_OFF = SC_OFF + STAGES * SC;
-  // q_full, q_empty, kv_full[S], kv_empty[S], kv_peer[S], s_full[2], p_full[2], o_full, o_empty,
+  // q_full, q_empty, kv_full[S], kv_empty[S], kv_peer[S], s_full[2], p_full[4], o_full, o_empty,
   // drain
-  static constexpr int NBAR = 2 + 3 * STAGES + 2 + 2 + 3;
+  static constexpr int NBAR = 2 + 3 * STAGES + 2 + 4 + 3;
   static constexpr int TOTAL = BAR_OFF + NBAR * 8 + 64 + 1024;
 };
 
@@ -690,8 +690,8 @@ __global__ void __launch_bounds__(Q8P_THREADS, 1)
   uint64_t* kv_empty = kv_full + L::STAGES;
   uint64_t* kv_peer = kv_empty + L::STAGES;     // even CTA's: the odd one's operands
   uint64_t* s_full = kv_peer + L::STAGES;
-  uint64_t* p_full = s_full + 2;                // even CTA's
-  uint64_t* o_full = p_full + 2;
+  uint64_t* p_full = s_full + 2;                // even CTA's: [half][tile]
+  uint64_t* o_full = p_full + 4;
   uint64_t* o_empty = o_full + 1;               // even CTA's
   uint64_t* drain = o_empty + 1;
   int64_t* s_run = reinterpret_cast<int64_t*>(bars + L::NBAR);  // u0, u1, at
@@ -732,6 +732,7 @@ __global__ void __launch_bounds__(Q8P_THREADS, 1)
       for (int t = 0; t < 2; ++t) {
         mbar_init(&s_full[t], 1);
         mbar_init(&p_full[t], 8);  // the tile's softmax warps of both CTAs
+        mbar_init(&p_full[2 + t], 8);
       }
       mbar_init(o_full, 1);
       mbar_init(o_empty, 16);
@@ -808,14 +809,16 @@ __global__ void __launch_bounds__(Q8P_THREADS, 1)
                          kk > 0 ? 1u : 0u);
         umma_commit_pair(&s_full[t], 0x3);
       };
-      auto pv_mma = [&](int t, int jb, bool first) {
+      auto pv_mma = [&](int t, int jb, int k0, bool first) {
         const uint32_t at_v =
             smem_u32(smem + L::KV_OFF + (jb % L::STAGES) * L::STAGE + L::K_BYTES);
         const uint64_t sv = D == 128 ? sdesc_mn128(at_v, L::V_BYTES) : sdesc_mn64(at_v);
 #pragma unroll
-        for (int kk = 0; kk < Q8P_BN / 16; ++kk)
+        for (int i = 0; i < Q8P_BN / 32; ++i) {
+          const int kk = k0 + i;
           umma_f16_ts_pair(tmem + 256 + t * 128, tmem + t * 128 + (kk >> 1) * 32 + (kk & 1) * 8,
-                           sv + kk * 16 * D / 16, idesc_o, (!first || kk > 0) ? 1u : 0u);
+                           sv + kk * 16 * D / 16, idesc_o, (!first || i > 0) ? 1u : 0u);
+        }
       };
       auto block_there = [&](int jb) {
         const uint32_t parity = (jb / L::STAGES) & 1;
@@ -836,23 +839,23 @@ __global__ void __launch_bounds__(Q8P_THREADS, 1)
           for (int t = na > 0 ? 0 : 1; t < ntile; ++t) s_mma(t, jb);
           ok = mbar_wait(o_empty, (items & 1) ^ 1u, abort_flag);  // the last output was read
           for (int j = 0; j < n && ok; ++j, ++jb) {
-            bool next_there = false;
+            // (before the wait for P, which takes longer)
+            if (j + 1 < n) {
+              ok = block_there(jb + 1);
+              if (!ok) break;
+            }
             for (int t = j < na ? 0 : 1; t < ntile; ++t) {
               ok = mbar_wait(&p_full[t], cnt[t] & 1, abort_flag);
               if (!ok) break;
+              tc_fence_after();
+              pv_mma(t, jb, 4, j == 0);
+              ok = mbar_wait(&p_full[2 + t], cnt[t] & 1, abort_flag);
+              if (!ok) break;
               ++cnt[t];
               tc_fence_after();
-              pv_mma(t, jb, j == 0);
+              pv_mma(t, jb, 0, false);
               if (t == ntile - 1) umma_commit_pair(&kv_empty[jb % L::STAGES], 0x3);
-              if (j + 1 < n && (t == 1 || j + 1 < na)) {
-                if (!next_there) {
-                  ok = block_there(jb + 1);
-                  if (!ok) break;
-                  tc_fence_after();
-                  next_there = true;
-                }
-                s_mma(t, jb + 1);
-              }
+              if (j + 1 < n && (t == 1 || j + 1 < na)) s_mma(t, jb + 1);
             }
           }
           if (!ok) break;
@@ -1022,12 +1025,10 @@ __global__ void __launch_bounds__(Q8P_THREADS, 1)
       if (cw == 0) {
         float* sc = reinterpret_cast<float*>(smem + L::SC_OFF + stage * L::SC);
         if (lane < 8) {
-          sc[lane] = ks_now;
-          const float v = vs_now <= Q8_LEAST_V ? Q8_LEAST_V : vs_now;
-          sc[8 + lane] = 1.0f / (v * q8_f16_unit<FMT>());
-          sc[16 + lane] = log2f(v);
+          sc[2 * lane] = ks_now;
+          sc[2 * lane + 1] = log2f(vs_now <= Q8_LEAST_V ? Q8_LEAST_V : vs_now);
         }
-        if (lane == 0) reinterpret_cast<unsigned*>(sc)[24] = groups;
+        if (lane == 0) reinterpret_cast<unsigned*>(sc)[16] = groups;
       }
       fence_proxy_async_smem();
       __syncwarp();
@@ -1077,8 +1078,8 @@ __global__ void __launch_bounds__(Q8P_THREADS, 1)
         //   P = vs exp2(s ks - m) = exp2(s ks + log2(vs) - m),
         // so the reference follows the largest s ks + log2(vs) and P stays within f16's range
         // whatever the blocks' V scales are; the row sum takes a group's sum of P over vs.
-        const float* sc = reinterpret_cast<const float*>(smem + L::SC_OFF + stage * L::SC);
-        const unsigned groups = reinterpret_cast<const unsigned*>(sc)[24];
+        const float4* sc = reinterpret_cast<const float4*>(smem + L::SC_OFF + stage * L::SC);
+        const unsigned groups = reinterpret_cast<const unsigned*>(sc)[16];
         const bool masked = key0 + Q8P_BN > least || groups != 255u;  // warp-uniform
         const int valid = masked ? limit - key0 : Q8P_BN;
         uint32_t sr[2][32];
@@ -1090,6 +1091,7 @@ __global__ void __launch_bounds__(Q8P_THREADS, 1)
             tmem_ld32(s_col + c * 32 + 32, sr[1]);
             tmem_wait_ld();
           }
+          const float4 sc2 = sc[c];  // of groups 2c, 2c + 1
 #pragma unroll
           for (int q = 0; q < 2; ++q) {
             const uint32_t* v = sr[c & 1] + q * 16;
@@ -1110,7 +1112,7 @@ __global__ void __launch_bounds__(Q8P_THREADS, 1)
               x = fmaxf(max3f(x, y, __uint_as_float(v[14])), __uint_as_float(v[15]));
             }
             // scales are not negative; a masked group stays at -inf whatever its scales are
-            const float y = fmaf(x, sc[g], sc[16 + g]);
+            const float y = fmaf(x, q ? sc2.z : sc2.x, q ? sc2.w : sc2.y);
             mine = fmaxf(mine, masked && (g * 16 >= valid || !((groups >> g) & 1)) ? -INFINITY : y);
           }
         }
@@ -1130,6 +1132,14 @@ __global__ void __launch_bounds__(Q8P_THREADS, 1)
           m_run = mine;
         }
         const float ref = m_run == -INFINITY ? 0.0f : m_run;
+        // The products of the last 64 keys may start when their P is there (unless the output is to
+        // be rescaled first).
+        auto half_done = [&]() {
+          tmem_wait_st();
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) mbar_arrive_cluster_relaxed(p_full0);  // tensor memory only, written above
+        };
         auto exps = [&](auto tag) {
           constexpr bool MASKED = decltype(tag)::value;
           // chunks 2 and 3 are still in registers; 0 and 1 come back as those are done
@@ -1139,10 +1149,11 @@ __global__ void __launch_bounds__(Q8P_THREADS, 1)
             const uint32_t(&x32)[32] = sr[k & 1];
             if (k == 3) tmem_wait_ld();
             uint32_t packed[16];
+            const float4 sc2 = sc[c];
 #pragma unroll
             for (int q = 0; q < 2; ++q) {
               const int g = 2 * c + q;
-              const float kg = sc[g], cg = sc[16 + g] - ref;
+              const float kg = q ? sc2.z : sc2.x, lg = q ? sc2.w : sc2.y, cg = lg - ref;
               const uint64_t k2 = f2_pack(kg, kg), c2 = f2_pack(cg, cg);
               uint64_t sum2[2] = {f2_pack(0.0f, 0.0f), f2_pack(0.0f, 0.0f)};
 #pragma unroll
@@ -1169,7 +1180,7 @@ __global__ void __launch_bounds__(Q8P_THREADS, 1)
               }
               const float2 s2 = f2_unpack(f2_add(sum2[0], sum2[1]));
               if (!MASKED || (((groups >> g) & 1) && g * 16 < valid))
-                l_run = fmaf(s2.x + s2.y, sc[8 + g], l_run);
+                l_run = fmaf(s2.x + s2.y, ex2_approx(-lg), l_run);
             }
             // P of keys 32c .. over the first half of the chunk's scores
             tmem_st8(s_col + c * 32, *reinterpret_cast<const uint32_t(*)[8]>(packed));
@@ -1178,6 +1189,7 @@ __global__ void __launch_bounds__(Q8P_THREADS, 1)
             if (k == 1) {
               tmem_wait_ld();
               tmem_ld32(s_col + 32, sr[1]);
+              if (!rescale) half_done();
             }
           }
         };
@@ -1196,10 +1208,11 @@ __global__ void __launch_bounds__(Q8P_THREADS, 1)
             tmem_st32(o_col + c * 32, o);
           }
         }
+        if (rescale) half_done();
         tmem_wait_st();
         tc_fence_before();
         __syncwarp();
-        if (lane == 0) mbar_arrive_cluster_relaxed(p_full0);  // tensor memory only, written above
+        if (lane == 0) mbar_arrive_cluster_relaxed(p_full0 + 16);
         ++cnt;
       }
       if (keys > 0) {
@@ -1208,6 +1221,7 @@ __global__ void __launch_bounds__(Q8P_THREADS, 1)
         tc_fence_after();
         jb += n;
       }
+      l_run *= 1.0f / q8_f16_unit<FMT>();  // the V codes stand as their value over it
       if (t < ntile) {
         const float inv = m_run == -INFINITY ? 1.0f : 1.0f / l_run;
         const int64_t part = static_cast<int64_t>(2 * pair + (piece > 0 ? 1 : 0)) * a.tile_rows +
