@@ -644,9 +644,9 @@ struct Q8PrefillSmem {
   // the groups that are there
   static constexpr int SC = 80;
   static constexpr int BAR_OFF = SC_OFF + STAGES * SC;
-  // q_full, q_empty, kv_full[S], kv_empty[S], kv_peer[S], s_full[2], p_full[4], o_full, o_empty,
-  // drain
-  static constexpr int NBAR = 2 + 3 * STAGES + 2 + 4 + 3;
+  // q_full, q_empty, kv_full[S], kv_empty[S], kv_peer[S], s_full[4], p_full[4], pv_done[2], o_full,
+  // o_empty, drain
+  static constexpr int NBAR = 2 + 3 * STAGES + 4 + 4 + 2 + 3;
   static constexpr int TOTAL = BAR_OFF + NBAR * 8 + 64 + 1024;
 };
 
@@ -674,6 +674,23 @@ __device__ __forceinline__ void umma_f16_ts_pair(uint32_t d_tmem, uint32_t a_tme
       : "memory");
 }
 
+// One lane of the warp.
+__device__ __forceinline__ bool elect_one() {
+  uint32_t p;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "elect.sync _|p, 0xffffffff;\n\t"
+      "selp.u32 %0, 1, 0, p;\n\t}"
+      : "=r"(p));
+  return p != 0;
+}
+// The same value in every lane (which the compiler then knows).
+__device__ __forceinline__ int uniform(int v) { return __shfl_sync(0xffffffffu, v, 0); }
+// mbar_wait by a whole warp, which goes on or gives up together.
+__device__ __forceinline__ bool warp_wait(uint64_t* bar, uint32_t parity, volatile int* abort) {
+  return __all_sync(0xffffffffu, mbar_wait(bar, parity, abort));
+}
+
 template <int D, int FMT>
 __global__ void __launch_bounds__(Q8P_THREADS, 1)
     attention_q8_prefill_kernel(const __grid_constant__ CUtensorMap map_q, const Q8Attn a) {
@@ -690,8 +707,9 @@ __global__ void __launch_bounds__(Q8P_THREADS, 1)
   uint64_t* kv_empty = kv_full + L::STAGES;
   uint64_t* kv_peer = kv_empty + L::STAGES;     // even CTA's: the odd one's operands
   uint64_t* s_full = kv_peer + L::STAGES;
-  uint64_t* p_full = s_full + 2;                // even CTA's: [half][tile]
-  uint64_t* o_full = p_full + 4;
+  uint64_t* p_full = s_full + 4;                // even CTA's; both [half][tile]
+  uint64_t* pv_done = p_full + 4;               // [tile]
+  uint64_t* o_full = pv_done + 2;
   uint64_t* o_empty = o_full + 1;               // even CTA's
   uint64_t* drain = o_empty + 1;
   int64_t* s_run = reinterpret_cast<int64_t*>(bars + L::NBAR);  // u0, u1, at
@@ -699,7 +717,7 @@ __global__ void __launch_bounds__(Q8P_THREADS, 1)
   volatile int* abort_flag = s_item + 3;
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(s_item + 4);
 
-  const int warp = warp_id();
+  const int warp = uniform(warp_id());
   const int lane = static_cast<int>(lane_id());
   const int rank = static_cast<int>(cluster_rank());
   const int pair = static_cast<int>(blockIdx.x >> 1);
@@ -730,9 +748,11 @@ __global__ void __launch_bounds__(Q8P_THREADS, 1)
         mbar_init(&kv_peer[i], 1);
       }
       for (int t = 0; t < 2; ++t) {
-        mbar_init(&s_full[t], 1);
-        mbar_init(&p_full[t], 8);  // the tile's softmax warps of both CTAs
-        mbar_init(&p_full[2 + t], 8);
+        for (int h = 0; h < 2; ++h) {
+          mbar_init(&s_full[h * 2 + t], 1);
+          mbar_init(&p_full[h * 2 + t], 8);  // the tile's softmax warps of both CTAs
+        }
+        mbar_init(&pv_done[t], 1);
       }
       mbar_init(o_full, 1);
       mbar_init(o_empty, 16);
@@ -747,7 +767,7 @@ __global__ void __launch_bounds__(Q8P_THREADS, 1)
   __syncthreads();
   cluster_sync();  // both CTAs' barriers exist before any remote arrive
   tc_fence_after();
-  const uint32_t tmem = *tmem_slot;
+  const uint32_t tmem = uniform(*tmem_slot);
   griddep_launch();
   int64_t left = s_run[1] - s_run[0];
   int at = static_cast<int>(s_run[2]);
@@ -793,74 +813,82 @@ __global__ void __launch_bounds__(Q8P_THREADS, 1)
         while (global_ns() - t0 < 100000000ull) {
         }
       }
-    } else if (warp == 1 && lane == 0 && rank == 0) {
-      // ---- products
-      constexpr uint32_t idesc_s = idesc_bf16(256, 128);
+    } else if (warp == 1 && rank == 0) {
+      // ---- products: the whole warp walks the run, with values that the compiler knows to be the
+      // same in all lanes, and one lane issues
+      const bool issue = elect_one();
+      constexpr uint32_t idesc_s = idesc_bf16(256, 64);
       constexpr uint32_t idesc_o = idesc_f16(256, D) | (1u << 16);  // V: MN-major
-      auto s_mma = [&](int t, int jb) {
-        // (descriptors hold addresses in units of 16 bytes: steps are plain additions)
+      // (descriptors hold addresses in units of 16 bytes: steps are plain additions)
+      auto s_mma = [&](int t, int jb, int half) {
         const uint64_t sq = sdesc_k128(smem_u32(smem + L::Q_OFF + t * 2 * L::HALF));
         const uint64_t sk =
-            sdesc_k128(smem_u32(smem + L::KV_OFF + (jb % L::STAGES) * L::STAGE));
+            sdesc_k128(smem_u32(smem + L::KV_OFF + (jb % L::STAGES) * L::STAGE + half * 32 * 128));
+        if (issue) {
 #pragma unroll
-        for (int kk = 0; kk < D / 16; ++kk)
-          umma_bf16_pair(tmem + t * 128, sq + ((kk >> 2) * L::HALF + (kk & 3) * 32) / 16,
-                         sk + ((kk >> 2) * L::KHALF + (kk & 3) * 32) / 16, idesc_s,
-                         kk > 0 ? 1u : 0u);
-        umma_commit_pair(&s_full[t], 0x3);
+          for (int kk = 0; kk < D / 16; ++kk)
+            umma_bf16_pair(tmem + t * 128 + half * 64,
+                           sq + ((kk >> 2) * L::HALF + (kk & 3) * 32) / 16,
+                           sk + ((kk >> 2) * L::KHALF + (kk & 3) * 32) / 16, idesc_s,
+                           kk > 0 ? 1u : 0u);
+          umma_commit_pair(&s_full[half * 2 + t], 0x3);
+        }
       };
-      auto pv_mma = [&](int t, int jb, int k0, bool first) {
+      auto pv_mma = [&](int t, int jb, int half, bool first, bool free_stage) {
         const uint32_t at_v =
             smem_u32(smem + L::KV_OFF + (jb % L::STAGES) * L::STAGE + L::K_BYTES);
-        const uint64_t sv = D == 128 ? sdesc_mn128(at_v, L::V_BYTES) : sdesc_mn64(at_v);
+        const uint64_t sv = (D == 128 ? sdesc_mn128(at_v, L::V_BYTES) : sdesc_mn64(at_v)) +
+                            half * 32 * D / 16;
+        if (issue) {
 #pragma unroll
-        for (int i = 0; i < Q8P_BN / 32; ++i) {
-          const int kk = k0 + i;
-          umma_f16_ts_pair(tmem + 256 + t * 128, tmem + t * 128 + (kk >> 1) * 32 + (kk & 1) * 8,
-                           sv + kk * 16 * D / 16, idesc_o, (!first || i > 0) ? 1u : 0u);
+          for (int kk = 0; kk < 4; ++kk)  // keys 32 half + 16 kk, then 64 + 32 half + 16 (kk - 2)
+            umma_f16_ts_pair(tmem + 256 + t * 128, tmem + t * 128 + half * 64 + kk * 8,
+                             sv + (kk * 16 + (kk >= 2 ? 32 : 0)) * D / 16, idesc_o,
+                             (!first || kk > 0) ? 1u : 0u);
+          umma_commit_pair(&pv_done[t], 0x3);
+          if (free_stage) umma_commit_pair(&kv_empty[jb % L::STAGES], 0x3);
         }
       };
       auto block_there = [&](int jb) {
         const uint32_t parity = (jb / L::STAGES) & 1;
-        return mbar_wait(&kv_full[jb % L::STAGES], parity, abort_flag) &&
-               mbar_wait(&kv_peer[jb % L::STAGES], parity, abort_flag);
+        return warp_wait(&kv_full[jb % L::STAGES], parity, abort_flag) &&
+               warp_wait(&kv_peer[jb % L::STAGES], parity, abort_flag);
       };
       int items = 0, jb = 0;
-      int cnt[2] = {0, 0};  // blocks that a tile has been given
+      uint32_t parity = 0;  // bit t: of the blocks that tile t has been given
       bool ok = true;
-      while (left > 0 && ok) {
-        const int n = static_cast<int>(left < w.units - at ? left : w.units - at);
-        if (Work::keys(a, w.count, w.len, w.tile) > 0) {
-          const int ntile = w.count - w.tile * a.tile_tokens > 2 * chunk ? 2 : 1;
-          const int na = blocks_a(ntile) - at;  // of this piece's blocks
-          ok = mbar_wait(q_full, items & 1, abort_flag) && block_there(jb);
+      while (__any_sync(0xffffffffu, left > 0) && ok) {
+        const int n = uniform(static_cast<int>(left < w.units - at ? left : w.units - at));
+        if (__any_sync(0xffffffffu, Work::keys(a, w.count, w.len, w.tile) > 0)) {
+          const int ntile = uniform(w.count - w.tile * a.tile_tokens > 2 * chunk ? 2 : 1);
+          const int na = uniform(blocks_a(ntile) - at);  // of this piece's blocks
+          ok = warp_wait(q_full, items & 1, abort_flag) && block_there(jb);
           if (!ok) break;
           tc_fence_after();
-          for (int t = na > 0 ? 0 : 1; t < ntile; ++t) s_mma(t, jb);
-          ok = mbar_wait(o_empty, (items & 1) ^ 1u, abort_flag);  // the last output was read
+          for (int half = 0; half < 2; ++half)
+            for (int t = na > 0 ? 0 : 1; t < ntile; ++t) s_mma(t, jb, half);
+          ok = warp_wait(o_empty, (items & 1) ^ 1u, abort_flag);  // the last output was read
           for (int j = 0; j < n && ok; ++j, ++jb) {
             // (before the wait for P, which takes longer)
             if (j + 1 < n) {
               ok = block_there(jb + 1);
               if (!ok) break;
             }
-            for (int t = j < na ? 0 : 1; t < ntile; ++t) {
-              ok = mbar_wait(&p_full[t], cnt[t] & 1, abort_flag);
-              if (!ok) break;
-              tc_fence_after();
-              pv_mma(t, jb, 4, j == 0);
-              ok = mbar_wait(&p_full[2 + t], cnt[t] & 1, abort_flag);
-              if (!ok) break;
-              ++cnt[t];
-              tc_fence_after();
-              pv_mma(t, jb, 0, false);
-              if (t == ntile - 1) umma_commit_pair(&kv_empty[jb % L::STAGES], 0x3);
-              if (j + 1 < n && (t == 1 || j + 1 < na)) s_mma(t, jb + 1);
-            }
+#pragma unroll 1
+            for (int half = 0; half < 2 && ok; ++half)
+#pragma unroll 1
+              for (int t = j < na ? 0 : 1; t < ntile; ++t) {
+                ok = warp_wait(&p_full[half * 2 + t], (parity >> t) & 1, abort_flag);
+                if (!ok) break;
+                parity ^= static_cast<uint32_t>(half) << t;
+                tc_fence_after();
+                pv_mma(t, jb, half, j == 0 && half == 0, half == 1 && t == ntile - 1);
+                if (j + 1 < n && (t == 1 || j + 1 < na)) s_mma(t, jb + 1, half);
+              }
           }
           if (!ok) break;
-          umma_commit_pair(q_empty, 0x3);
-          umma_commit_pair(o_full, 0x3);
+          if (issue) umma_commit_pair(q_empty, 0x3);
+          if (issue) umma_commit_pair(o_full, 0x3);
           ++items;
         }
         left -= n;
@@ -868,7 +896,7 @@ __global__ void __launch_bounds__(Q8P_THREADS, 1)
         if (left > 0) w.next();
       }
       // all issued products end before tensor memory is released (bounded)
-      umma_commit_pair(drain, 0x1);
+      if (issue) umma_commit_pair(drain, 0x1);
       const uint64_t t0 = global_ns();
       while (!mbar_try_wait(drain, 0) && global_ns() - t0 < 200000000ull) {
       }
@@ -1036,20 +1064,18 @@ __global__ void __launch_bounds__(Q8P_THREADS, 1)
       ++jb;
     }
   } else {
-    // ---- softmax: one row a thread, its 128 scores in chunks of 32 of which two are held at a
-    // time (read for the maximum, and the first two again for P)
+    // ---- softmax: one row a thread, 64 of the block's keys at a time
     const int t = (warp - 2) >> 2;
     const int quarter = warp & 3;
     const int row = quarter * 32 + lane;
     const uint32_t lane_base = static_cast<uint32_t>(quarter * 32) << 16;
-    const uint32_t s_col = tmem + lane_base + t * 128;
-    const uint32_t o_col = s_col + 256;
+    const uint32_t o_col = tmem + lane_base + 256 + t * 128;
     const int row_tok = row / a.group, row_head = row % a.group;
     const bool in_row = row < chunk * a.group;
     const uint32_t p_full0 = cluster_addr(smem_u32(&p_full[t]), 0);
     const uint32_t o_empty0 = cluster_addr(smem_u32(o_empty), 0);
     int items = 0, jb = 0, piece = 0;
-    int cnt = 0;  // blocks of this tile
+    int cnt = 0;  // half blocks of this tile
     bool ok = true;
     while (left > 0) {
       const int n = static_cast<int>(left < w.units - at ? left : w.units - at);
@@ -1066,61 +1092,63 @@ __global__ void __launch_bounds__(Q8P_THREADS, 1)
       int blocks = 0;  // that the tile takes part in
       if (keys > 0 && t < ntile) blocks = t == 1 ? n : min(n, blocks_a(ntile) - at);
       float m_run = -INFINITY, l_run = 0.0f;
-      for (int j = 0; j < blocks; ++j) {
+#pragma unroll 1
+      for (int hj = 0; hj < 2 * blocks; ++hj, ++cnt) {
+        const int half = hj & 1, j = hj >> 1;
         const int stage = (jb + j) % L::STAGES;
-        const int key0 = (at + j) * Q8P_BN;
         ok = __all_sync(0xffffffffu,
                         mbar_wait(&kv_full[stage], ((jb + j) / L::STAGES) & 1, abort_flag) &&
-                            mbar_wait(&s_full[t], cnt & 1, abort_flag));
+                            mbar_wait(&s_full[half * 2 + t], (cnt >> 1) & 1, abort_flag));
         if (!ok) break;
         tc_fence_after();
         // Row i of the tile keeps one reference m, and the second product's operand is
         //   P = vs exp2(s ks - m) = exp2(s ks + log2(vs) - m),
         // so the reference follows the largest s ks + log2(vs) and P stays within f16's range
         // whatever the blocks' V scales are; the row sum takes a group's sum of P over vs.
-        const float4* sc = reinterpret_cast<const float4*>(smem + L::SC_OFF + stage * L::SC);
-        const unsigned groups = reinterpret_cast<const unsigned*>(sc)[16];
-        const bool masked = key0 + Q8P_BN > least || groups != 255u;  // warp-uniform
-        const int valid = masked ? limit - key0 : Q8P_BN;
+        const uint32_t s_col = tmem + lane_base + t * 128 + half * 64;
         uint32_t sr[2][32];
+        tmem_ld32(s_col, sr[0]);
+        tmem_ld32(s_col + 32, sr[1]);
+        // columns 0..31 are keys key0 .., columns 32..63 keys key0 + 64 ..
+        const int key0 = (at + j) * Q8P_BN + half * 32;
+        const float4* sc = reinterpret_cast<const float4*>(smem + L::SC_OFF + stage * L::SC) + half;
+        const float4 sc2[2] = {sc[0], sc[2]};
+        const unsigned word =
+            reinterpret_cast<const unsigned*>(smem + L::SC_OFF + stage * L::SC)[16] >> (2 * half);
+        const unsigned groups = (word & 3u) | ((word >> 2) & 12u);
+        const bool masked = key0 + 96 > least || groups != 15u;  // warp-uniform
+        const int valid[2] = {masked ? limit - key0 : 32, masked ? limit - key0 - 64 : 32};
+        tmem_wait_ld();
         float mine = -INFINITY;
 #pragma unroll
-        for (int c = 0; c < 4; ++c) {
-          if ((c & 1) == 0) {
-            tmem_ld32(s_col + c * 32, sr[0]);
-            tmem_ld32(s_col + c * 32 + 32, sr[1]);
-            tmem_wait_ld();
-          }
-          const float4 sc2 = sc[c];  // of groups 2c, 2c + 1
+        for (int g = 0; g < 4; ++g) {
+          const uint32_t* v = sr[g >> 1] + (g & 1) * 16;
+          const int of = (g & 1) * 16;
+          float x;
+          if (masked) {
+            x = -INFINITY;
 #pragma unroll
-          for (int q = 0; q < 2; ++q) {
-            const uint32_t* v = sr[c & 1] + q * 16;
-            const int g = 2 * c + q;
-            float x;
-            if (masked) {
-              x = -INFINITY;
-#pragma unroll
-              for (int i = 0; i < 16; ++i)
-                x = fmaxf(x, g * 16 + i < valid ? __uint_as_float(v[i]) : -INFINITY);
-            } else {
-              x = max3f(__uint_as_float(v[0]), __uint_as_float(v[1]), __uint_as_float(v[2]));
-              x = max3f(x, __uint_as_float(v[3]), __uint_as_float(v[4]));
-              x = max3f(x, __uint_as_float(v[5]), __uint_as_float(v[6]));
-              float y = max3f(__uint_as_float(v[7]), __uint_as_float(v[8]), __uint_as_float(v[9]));
-              y = max3f(y, __uint_as_float(v[10]), __uint_as_float(v[11]));
-              y = max3f(y, __uint_as_float(v[12]), __uint_as_float(v[13]));
-              x = fmaxf(max3f(x, y, __uint_as_float(v[14])), __uint_as_float(v[15]));
-            }
-            // scales are not negative; a masked group stays at -inf whatever its scales are
-            const float y = fmaf(x, q ? sc2.z : sc2.x, q ? sc2.w : sc2.y);
-            mine = fmaxf(mine, masked && (g * 16 >= valid || !((groups >> g) & 1)) ? -INFINITY : y);
+            for (int i = 0; i < 16; ++i)
+              x = fmaxf(x, of + i < valid[g >> 1] ? __uint_as_float(v[i]) : -INFINITY);
+          } else {
+            x = max3f(__uint_as_float(v[0]), __uint_as_float(v[1]), __uint_as_float(v[2]));
+            x = max3f(x, __uint_as_float(v[3]), __uint_as_float(v[4]));
+            x = max3f(x, __uint_as_float(v[5]), __uint_as_float(v[6]));
+            float y = max3f(__uint_as_float(v[7]), __uint_as_float(v[8]), __uint_as_float(v[9]));
+            y = max3f(y, __uint_as_float(v[10]), __uint_as_float(v[11]));
+            y = max3f(y, __uint_as_float(v[12]), __uint_as_float(v[13]));
+            x = fmaxf(max3f(x, y, __uint_as_float(v[14])), __uint_as_float(v[15]));
           }
+          // scales are not negative; a masked group stays at -inf whatever its scales are
+          const float4 s4 = sc2[g >> 1];
+          const float y = fmaf(x, g & 1 ? s4.z : s4.x, g & 1 ? s4.w : s4.y);
+          mine = fmaxf(mine, masked && (of >= valid[g >> 1] || !((groups >> g) & 1)) ? -INFINITY : y);
         }
         // The reference moves only when it is exceeded by 2^8 (the stale one cancels in the
-        // division). O holds the products of the blocks before this one.
+        // division).
         float alpha = 1.0f;
         bool rescale = false;
-        if (j > 0) {
+        if (hj > 0) {
           const bool need = mine > m_run + 8.0f;
           rescale = __any_sync(0xffffffffu, need);
           if (need) {
@@ -1132,65 +1160,42 @@ __global__ void __launch_bounds__(Q8P_THREADS, 1)
           m_run = mine;
         }
         const float ref = m_run == -INFINITY ? 0.0f : m_run;
-        // The products of the last 64 keys may start when their P is there (unless the output is to
-        // be rescaled first).
-        auto half_done = [&]() {
-          tmem_wait_st();
-          tc_fence_before();
-          __syncwarp();
-          if (lane == 0) mbar_arrive_cluster_relaxed(p_full0);  // tensor memory only, written above
-        };
         auto exps = [&](auto tag) {
           constexpr bool MASKED = decltype(tag)::value;
-          // chunks 2 and 3 are still in registers; 0 and 1 come back as those are done
 #pragma unroll
-          for (int k = 0; k < 4; ++k) {
-            const int c = k ^ 2;
-            const uint32_t(&x32)[32] = sr[k & 1];
-            if (k == 3) tmem_wait_ld();
-            uint32_t packed[16];
-            const float4 sc2 = sc[c];
+          for (int g = 0; g < 4; ++g) {
+            const uint32_t* v = sr[g >> 1] + (g & 1) * 16;
+            const float4 s4 = sc2[g >> 1];
+            const float kg = g & 1 ? s4.z : s4.x, lg = g & 1 ? s4.w : s4.y, cg = lg - ref;
+            const uint64_t k2 = f2_pack(kg, kg), c2 = f2_pack(cg, cg);
+            uint64_t sum2[2] = {f2_pack(0.0f, 0.0f), f2_pack(0.0f, 0.0f)};
+            uint32_t packed[8];
 #pragma unroll
-            for (int q = 0; q < 2; ++q) {
-              const int g = 2 * c + q;
-              const float kg = q ? sc2.z : sc2.x, lg = q ? sc2.w : sc2.y, cg = lg - ref;
-              const uint64_t k2 = f2_pack(kg, kg), c2 = f2_pack(cg, cg);
-              uint64_t sum2[2] = {f2_pack(0.0f, 0.0f), f2_pack(0.0f, 0.0f)};
-#pragma unroll
-              for (int u = 0; u < 8; ++u) {
-                const int e = q * 16 + 2 * u;
-                const uint64_t xs = f2_fma(
-                    f2_pack(__uint_as_float(x32[e]), __uint_as_float(x32[e + 1])), k2, c2);
-                uint64_t ev;
-                if ((Q8P_EMU_MASK >> u) & 1) {
-                  ev = exp2_poly_x2(xs);
-                } else {
-                  const float2 xv = f2_unpack(xs);
-                  ev = f2_pack(ex2_approx(xv.x), ex2_approx(xv.y));
-                }
-                float2 p2 = f2_unpack(ev);
-                if constexpr (MASKED) {  // a masked key counts for nothing, its scales may be NaN
-                  const bool in = (groups >> g) & 1;
-                  p2.x = in && c * 32 + e < valid ? p2.x : 0.0f;
-                  p2.y = in && c * 32 + e + 1 < valid ? p2.y : 0.0f;
-                  ev = f2_pack(p2.x, p2.y);
-                }
-                sum2[u & 1] = f2_add(sum2[u & 1], ev);
-                packed[q * 8 + u] = pack_f16x2(p2.x, p2.y);
+            for (int u = 0; u < 8; ++u) {
+              const int e = 2 * u;
+              const uint64_t xs =
+                  f2_fma(f2_pack(__uint_as_float(v[e]), __uint_as_float(v[e + 1])), k2, c2);
+              uint64_t ev;
+              if ((Q8P_EMU_MASK >> u) & 1) {
+                ev = exp2_poly_x2(xs);
+              } else {
+                const float2 xv = f2_unpack(xs);
+                ev = f2_pack(ex2_approx(xv.x), ex2_approx(xv.y));
               }
-              const float2 s2 = f2_unpack(f2_add(sum2[0], sum2[1]));
-              if (!MASKED || (((groups >> g) & 1) && g * 16 < valid))
-                l_run = fmaf(s2.x + s2.y, ex2_approx(-lg), l_run);
+              float2 p2 = f2_unpack(ev);
+              if constexpr (MASKED) {  // a masked key counts for nothing, its scales may be NaN
+                const bool in = (groups >> g) & 1;
+                p2.x = in && (g & 1) * 16 + e < valid[g >> 1] ? p2.x : 0.0f;
+                p2.y = in && (g & 1) * 16 + e + 1 < valid[g >> 1] ? p2.y : 0.0f;
+                ev = f2_pack(p2.x, p2.y);
+              }
+              sum2[u & 1] = f2_add(sum2[u & 1], ev);
+              packed[u] = pack_f16x2(p2.x, p2.y);
             }
-            // P of keys 32c .. over the first half of the chunk's scores
-            tmem_st8(s_col + c * 32, *reinterpret_cast<const uint32_t(*)[8]>(packed));
-            tmem_st8(s_col + c * 32 + 8, *reinterpret_cast<const uint32_t(*)[8]>(packed + 8));
-            if (k == 0) tmem_ld32(s_col, sr[0]);
-            if (k == 1) {
-              tmem_wait_ld();
-              tmem_ld32(s_col + 32, sr[1]);
-              if (!rescale) half_done();
-            }
+            const float2 s2 = f2_unpack(f2_add(sum2[0], sum2[1]));
+            if (!MASKED || (((groups >> g) & 1) && (g & 1) * 16 < valid[g >> 1]))
+              l_run = fmaf(s2.x + s2.y, ex2_approx(-lg), l_run);
+            tmem_st8(s_col + g * 8, packed);  // over the scores, which are in registers
           }
         };
         if (masked)
@@ -1198,6 +1203,10 @@ __global__ void __launch_bounds__(Q8P_THREADS, 1)
         else
           exps(std::false_type{});
         if (rescale) {
+          // the product of the half block before this one has to be in the output
+          ok = __all_sync(0xffffffffu, mbar_wait(&pv_done[t], (cnt - 1) & 1, abort_flag));
+          if (!ok) break;
+          tc_fence_after();
 #pragma unroll 1
           for (int c = 0; c < D / 32; ++c) {
             uint32_t o[32];
@@ -1208,12 +1217,11 @@ __global__ void __launch_bounds__(Q8P_THREADS, 1)
             tmem_st32(o_col + c * 32, o);
           }
         }
-        if (rescale) half_done();
         tmem_wait_st();
         tc_fence_before();
         __syncwarp();
-        if (lane == 0) mbar_arrive_cluster_relaxed(p_full0 + 16);
-        ++cnt;
+        // (tensor memory only, written above: no memory to release)
+        if (lane == 0) mbar_arrive_cluster_relaxed(p_full0 + half * 16);
       }
       if (keys > 0) {
         ok = ok && __all_sync(0xffffffffu, mbar_wait(o_full, items & 1, abort_flag));
