@@ -624,11 +624,7 @@ __global__ void __launch_bounds__(Q8D_THREADS, 1)
 // under a causal mask and leaves the blocks behind it out.
 constexpr int Q8P_BN = 128;
 constexpr int Q8P_THREADS = 448;
-// Pairs of a group of 16 keys whose exponentials run on the FMA pipes (as ATT_EMU_MASK).
-#ifndef KINO_Q8P_EMU_MASK
-#define KINO_Q8P_EMU_MASK 0x00
-#endif
-constexpr unsigned Q8P_EMU_MASK = KINO_Q8P_EMU_MASK;
+
 template <int D>
 struct Q8PrefillSmem {
   static constexpr int HALF = 128 * 64 * 2;  // Q: 128 rows x 64 dims
@@ -1119,30 +1115,37 @@ __global__ void __launch_bounds__(Q8P_THREADS, 1)
         const bool masked = key0 + 96 > least || groups != 15u;  // warp-uniform
         const int valid[2] = {masked ? limit - key0 : 32, masked ? limit - key0 - 64 : 32};
         tmem_wait_ld();
-        float mine = -INFINITY;
+        // (scales are not negative: a group's largest score gives its largest scaled one)
+        float best[4];
+        if (masked) {
 #pragma unroll
-        for (int g = 0; g < 4; ++g) {
-          const uint32_t* v = sr[g >> 1] + (g & 1) * 16;
-          const int of = (g & 1) * 16;
-          float x;
-          if (masked) {
-            x = -INFINITY;
+          for (int g = 0; g < 4; ++g) {
+            const uint32_t* v = sr[g >> 1] + (g & 1) * 16;
+            const int of = (g & 1) * 16;
+            float x = -INFINITY;
 #pragma unroll
             for (int i = 0; i < 16; ++i)
               x = fmaxf(x, of + i < valid[g >> 1] ? __uint_as_float(v[i]) : -INFINITY);
-          } else {
-            x = max3f(__uint_as_float(v[0]), __uint_as_float(v[1]), __uint_as_float(v[2]));
-            x = max3f(x, __uint_as_float(v[3]), __uint_as_float(v[4]));
-            x = max3f(x, __uint_as_float(v[5]), __uint_as_float(v[6]));
-            float y = max3f(__uint_as_float(v[7]), __uint_as_float(v[8]), __uint_as_float(v[9]));
-            y = max3f(y, __uint_as_float(v[10]), __uint_as_float(v[11]));
-            y = max3f(y, __uint_as_float(v[12]), __uint_as_float(v[13]));
-            x = fmaxf(max3f(x, y, __uint_as_float(v[14])), __uint_as_float(v[15]));
+            best[g] = x;
           }
-          // scales are not negative; a masked group stays at -inf whatever its scales are
+        } else {
+#pragma unroll
+          for (int g = 0; g < 4; ++g) {
+            const uint32_t* v = sr[g >> 1] + (g & 1) * 16;
+            auto f = [&](int i) { return __uint_as_float(v[i]); };
+            const float x = max3f(f(0), f(1), f(2)), y = max3f(f(3), f(4), f(5));
+            const float z = max3f(f(6), f(7), f(8)), u = max3f(f(9), f(10), f(11));
+            best[g] = max3f(max3f(x, y, z), max3f(u, f(12), f(13)), fmaxf(f(14), f(15)));
+          }
+        }
+        float mine = -INFINITY;
+#pragma unroll
+        for (int g = 0; g < 4; ++g) {
           const float4 s4 = sc2[g >> 1];
-          const float y = fmaf(x, g & 1 ? s4.z : s4.x, g & 1 ? s4.w : s4.y);
-          mine = fmaxf(mine, masked && (of >= valid[g >> 1] || !((groups >> g) & 1)) ? -INFINITY : y);
+          const float y = fmaf(best[g], g & 1 ? s4.z : s4.x, g & 1 ? s4.w : s4.y);
+          // a masked group stays at -inf whatever its scales are
+          mine = fmaxf(mine, masked && ((g & 1) * 16 >= valid[g >> 1] || !((groups >> g) & 1))
+                                 ? -INFINITY : y);
         }
         // The reference moves only when it is exceeded by 2^8 (the stale one cancels in the
         // division).
@@ -1175,21 +1178,14 @@ __global__ void __launch_bounds__(Q8P_THREADS, 1)
               const int e = 2 * u;
               const uint64_t xs =
                   f2_fma(f2_pack(__uint_as_float(v[e]), __uint_as_float(v[e + 1])), k2, c2);
-              uint64_t ev;
-              if ((Q8P_EMU_MASK >> u) & 1) {
-                ev = exp2_poly_x2(xs);
-              } else {
-                const float2 xv = f2_unpack(xs);
-                ev = f2_pack(ex2_approx(xv.x), ex2_approx(xv.y));
-              }
-              float2 p2 = f2_unpack(ev);
+              const float2 xv = f2_unpack(xs);
+              float2 p2 = make_float2(ex2_approx(xv.x), ex2_approx(xv.y));
               if constexpr (MASKED) {  // a masked key counts for nothing, its scales may be NaN
                 const bool in = (groups >> g) & 1;
                 p2.x = in && (g & 1) * 16 + e < valid[g >> 1] ? p2.x : 0.0f;
                 p2.y = in && (g & 1) * 16 + e + 1 < valid[g >> 1] ? p2.y : 0.0f;
-                ev = f2_pack(p2.x, p2.y);
               }
-              sum2[u & 1] = f2_add(sum2[u & 1], ev);
+              sum2[u & 1] = f2_add(sum2[u & 1], f2_pack(p2.x, p2.y));
               packed[u] = pack_f16x2(p2.x, p2.y);
             }
             const float2 s2 = f2_unpack(f2_add(sum2[0], sum2[1]));
