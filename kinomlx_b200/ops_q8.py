@@ -22,8 +22,7 @@ from typing import NamedTuple
 
 import torch
 
-from . import _lib
-from .ops import _need, _ptr, _stream, _timed
+from . import _lib, ops
 
 BF16 = torch.bfloat16
 I32 = torch.int32
@@ -42,34 +41,49 @@ __all__ = [
 ]
 
 
+# Decoded tokens take a few microseconds on the GPU, so the host side of a call counts: one look at
+# each tensor, entry points bound once, no wrapper objects.
+_entries: dict[str, object] = {}
+
+
+def _launch(label: str, flops: float, nbytes: float, device: torch.device, name: str, *args) -> None:
+    """One kino_q8_* call on the device's current stream."""
+    entry = _entries.get(name)
+    if entry is None:
+        entry = _entries[name] = getattr(_lib.load(), name)
+    index = device.index
+    if index != torch.cuda.current_device():
+        with torch.cuda.device(index):
+            return _launch(label, flops, nbytes, device, name, *args)
+    stream = torch._C._cuda_getCurrentRawStream(index)
+    if ops._log is None:
+        ops.launches += 1
+        status = entry(*args, stream)
+    else:
+        with ops._timed(label, flops, nbytes):
+            status = entry(*args, stream)
+    if status:
+        label = _lib.STATUS_NAMES.get(status, str(status))
+        raise RuntimeError(f"{name} failed with {label}: {_lib.last_error()}")
+
+
 def _format(dtype: torch.dtype) -> int:
-    if dtype not in FORMATS:
-        raise ValueError(f"codes are int8 or float8_e4m3fn, not {dtype}")
-    return FORMATS[dtype]
+    try:
+        return FORMATS[dtype]
+    except KeyError:
+        raise ValueError(f"codes are int8 or float8_e4m3fn, not {dtype}") from None
 
 
-def _same_device(t: torch.Tensor, name: str, device: torch.device) -> None:
-    if t.device != device:
+def _need(t: torch.Tensor, name: str, dtype: torch.dtype, device: torch.device | None = None) -> None:
+    """A CUDA tensor of this type (on this device) with a unit stride in its last dimension."""
+    if not t.is_cuda:
+        raise ValueError(f"{name} must be a CUDA tensor (the kinomlx_b200 kernels have no CPU path)")
+    if t.dtype != dtype:
+        raise ValueError(f"{name} must be {dtype}, got {t.dtype}")
+    if device is not None and t.device != device:
         raise ValueError(f"{name} is on {t.device}, not on {device}")
-
-
-class _on:
-    """Makes a tensor's GPU the current one for a call (and its stream the one launched on)."""
-
-    __slots__ = ("guard",)
-
-    def __init__(self, device: torch.device):
-        other = device.index is not None and device.index != torch.cuda.current_device()
-        self.guard = torch.cuda.device(device) if other else None
-
-    def __enter__(self):
-        if self.guard is not None:
-            self.guard.__enter__()
-
-    def __exit__(self, *exc):
-        if self.guard is not None:
-            self.guard.__exit__(*exc)
-        return False
+    if not t.is_contiguous() and t.stride(-1) != 1 and t.shape[-1] != 1:
+        raise ValueError(f"{name} needs a unit stride in its last dimension")
 
 
 def _rows(t: torch.Tensor, name: str) -> torch.Tensor:
@@ -79,46 +93,44 @@ def _rows(t: torch.Tensor, name: str) -> torch.Tensor:
     if t.dim() == 0:
         raise ValueError(f"{name} needs rows")
     try:
-        return t.view(-1, t.shape[-1])
+        return t.view(-1, t.shape[-1]) if t.numel() else t.reshape(0, t.shape[-1])
     except RuntimeError:
         raise ValueError(f"{name}: rows of {tuple(t.shape)} are not at one stride") from None
 
 
 def _quantize_rows(x, weight, eps, residual, dtype, weight_offset, norm, hidden, label):
     fmt = _format(dtype)
-    _need(x, "x")
+    _need(x, "x", BF16)
     x2 = _rows(x, "x")
     rows, dim = x2.shape
     device = x.device
-    codes = torch.empty(x.shape, device=device, dtype=dtype)
-    scales = torch.empty(x.shape[:-1], device=device, dtype=F32)
-    r2 = h2 = None
+    r_ptr = h_ptr = w_ptr = None
+    ld_r = ld_h = 0
     if residual is not None:
-        _need(residual, "residual")
-        _same_device(residual, "residual", device)
+        _need(residual, "residual", BF16, device)
         if residual.shape != x.shape:
             raise ValueError(f"residual {tuple(residual.shape)} does not match {tuple(x.shape)}")
         if hidden is None:
-            hidden = torch.empty(x.shape, device=device, dtype=BF16)
-        _need(hidden, "hidden")
-        _same_device(hidden, "hidden", device)
-        if hidden.shape != x.shape:
-            raise ValueError(f"hidden {tuple(hidden.shape)} does not match {tuple(x.shape)}")
+            hidden = x.new_empty(x.shape)
+        else:
+            _need(hidden, "hidden", BF16, device)
+            if hidden.shape != x.shape:
+                raise ValueError(f"hidden {tuple(hidden.shape)} does not match {tuple(x.shape)}")
         r2, h2 = _rows(residual, "residual"), _rows(hidden, "hidden")
+        r_ptr, ld_r, h_ptr, ld_h = r2.data_ptr(), r2.stride(0), h2.data_ptr(), h2.stride(0)
     elif hidden is not None:
         raise ValueError("hidden is the sum with a residual: give one")
     if weight is not None:
-        _need(weight, "weight")
-        _same_device(weight, "weight", device)
-        if tuple(weight.shape) != (dim,):
+        _need(weight, "weight", BF16, device)
+        if weight.shape != (dim,):
             raise ValueError(f"weight {tuple(weight.shape)} does not match width {dim}")
+        w_ptr = weight.data_ptr()
+    codes = x.new_empty(x.shape, dtype=dtype)
+    scales = x.new_empty(x.shape[:-1], dtype=F32)
     if rows and dim:
-        with _on(device), _timed(label, 0.0, (3.0 if r2 is None else 7.0) * rows * dim):
-            _lib.call(
-                "kino_q8_rows", x2.data_ptr(), x2.stride(0), _ptr(r2),
-                0 if r2 is None else r2.stride(0), _ptr(weight), weight_offset, eps, norm,
-                _ptr(h2), 0 if h2 is None else h2.stride(0), codes.data_ptr(), scales.data_ptr(),
-                fmt, rows, dim, _stream())
+        _launch(label, 0.0, (3.0 if residual is None else 7.0) * rows * dim, device,
+                "kino_q8_rows", x2.data_ptr(), x2.stride(0), r_ptr, ld_r, w_ptr, weight_offset, eps,
+                norm, h_ptr, ld_h, codes.data_ptr(), scales.data_ptr(), fmt, rows, dim)
     return codes, scales, x if hidden is None else hidden
 
 
@@ -158,40 +170,38 @@ def linear_int8(
     scale for each row and an int8 weight (n, k) with one for each channel; the sum over k is
     exact. k a multiple of 16, n of 8."""
     _need(codes, "codes", torch.int8)
-    _need(w_codes, "w_codes", torch.int8)
-    _need(scales, "scales", F32)
-    _need(w_scales, "w_scales", F32)
+    device = codes.device
+    _need(w_codes, "w_codes", torch.int8, device)
+    _need(scales, "scales", F32, device)
+    _need(w_scales, "w_scales", F32, device)
     x2 = _rows(codes, "codes")
     m, k = x2.shape
     if w_codes.dim() != 2 or w_codes.shape[1] != k:
         raise ValueError(f"weight {tuple(w_codes.shape)} does not match input width {k}")
     n = w_codes.shape[0]
-    device = codes.device
     if scales.shape != codes.shape[:-1] or not scales.is_contiguous():
         raise ValueError(f"scales {tuple(scales.shape)} are not one for each row, contiguous")
     if w_scales.shape != (n,):
         raise ValueError(f"w_scales {tuple(w_scales.shape)} are not one for each of {n} channels")
-    for t, name in ((scales, "scales"), (w_codes, "w_codes"), (w_scales, "w_scales")):
-        _same_device(t, name, device)
+    b_ptr = None
     if bias is not None:
-        _need(bias, "bias")
-        _same_device(bias, "bias", device)
+        _need(bias, "bias", BF16, device)
         if bias.shape != (n,):
             raise ValueError(f"bias {tuple(bias.shape)} is not one for each of {n} channels")
+        b_ptr = bias.data_ptr()
+    shape = (*codes.shape[:-1], n)
     if out is None:
-        out = torch.empty((*codes.shape[:-1], n), device=device, dtype=BF16)
+        out = codes.new_empty(shape, dtype=BF16)
     else:
-        _need(out, "out")
-        _same_device(out, "out", device)
-        if out.shape != (*codes.shape[:-1], n):
-            raise ValueError(f"out {tuple(out.shape)} does not match ({m}, {n})")
+        _need(out, "out", BF16, device)
+        if out.shape != shape:
+            raise ValueError(f"out {tuple(out.shape)} does not match {shape}")
     o2 = _rows(out, "out")
     if m and n:
-        with _on(device), _timed("linear_int8", 2.0 * m * n * k, 1.0 * m * k + n * k + 2 * m * n):
-            _lib.call(
+        _launch("linear_int8", 2.0 * m * n * k, 1.0 * m * k + n * k + 2 * m * n, device,
                 "kino_q8_linear", x2.data_ptr(), x2.stride(0) if m > 1 else k, scales.data_ptr(),
-                w_codes.data_ptr(), w_codes.stride(0) if n > 1 else k, w_scales.data_ptr(),
-                _ptr(bias), out.data_ptr(), o2.stride(0) if m > 1 else n, m, n, k, _stream())
+                w_codes.data_ptr(), w_codes.stride(0) if n > 1 else k, w_scales.data_ptr(), b_ptr,
+                out.data_ptr(), o2.stride(0) if m > 1 else n, m, n, k)
     return out
 
 
@@ -224,7 +234,6 @@ def new_kv_cache(blocks: int, heads: int, dim: int, *, block_tokens: int = 64,
 
 def _cache_args(cache: KVCache, table: torch.Tensor, lengths: torch.Tensor) -> _lib.Q8Cache:
     k, v, ks, vs = cache
-    device = k.device
     fmt = _format(k.dtype)
     if k.dim() != 4 or v.shape != k.shape or v.dtype != k.dtype:
         raise ValueError(f"codes of keys {tuple(k.shape)} and values {tuple(v.shape)} are not one "
@@ -240,12 +249,12 @@ def _cache_args(cache: KVCache, table: torch.Tensor, lengths: torch.Tensor) -> _
     if table.dim() != 2 or lengths.shape != table.shape[:1]:
         raise ValueError(f"table {tuple(table.shape)} and lengths {tuple(lengths.shape)} are not "
                          "(batch, blocks) and (batch,)")
-    if table.stride(1) != 1 and table.shape[1] > 1 or not lengths.is_contiguous():
-        raise ValueError("block table rows and lengths need unit strides")
-    for t in (v, ks, vs, table, lengths):
-        if t.device != device:
-            raise ValueError(f"cache, table and lengths on {t.device} and {device}")
     batch, wide = table.shape
+    if (wide > 1 and table.stride(1) != 1) or not lengths.is_contiguous():
+        raise ValueError("block table rows and lengths need unit strides")
+    device = k.device
+    if not (v.device == ks.device == vs.device == table.device == lengths.device == device):
+        raise ValueError(f"cache, table and lengths are not all on {device}")
     return _lib.Q8Cache(k.data_ptr(), v.data_ptr(), ks.data_ptr(), vs.data_ptr(), blocks, heads,
                         dim, block, fmt, table.data_ptr(),
                         table.stride(0) if batch > 1 else max(wide, 1), wide, lengths.data_ptr(),
@@ -261,13 +270,13 @@ def _starts(token_starts: torch.Tensor | None, batch: int, rows: int,
     if token_starts.dtype != I32 or token_starts.shape != (batch + 1,) \
             or not token_starts.is_contiguous():
         raise ValueError(f"token_starts are batch + 1 = {batch + 1} int32, contiguous")
-    _same_device(token_starts, "token_starts", device)
+    if token_starts.device != device:
+        raise ValueError(f"token_starts is on {token_starts.device}, not on {device}")
     return token_starts.data_ptr()
 
 
 def _heads(t: torch.Tensor, name: str, dim: int, device: torch.device) -> None:
-    _need(t, name)
-    _same_device(t, name, device)
+    _need(t, name, BF16, device)
     if t.dim() != 3 or t.shape[2] != dim:
         raise ValueError(f"{name} {tuple(t.shape)} is not (rows, heads, {dim})")
 
@@ -299,9 +308,9 @@ def kv_cache_write(
     if not rows or not args.batch:
         return
     starts = _starts(token_starts, args.batch, rows, device)
-    with _on(device), _timed("kv_cache_write", 0.0, 6.0 * k.numel()):
-        _lib.call("kino_q8_cache_write", args, k.data_ptr(), k.stride(0), k.stride(1),
-                  v.data_ptr(), v.stride(0), v.stride(1), starts, rows, _stream())
+    _launch("kv_cache_write", 0.0, 6.0 * k.numel(), device, "kino_q8_cache_write", args,
+            k.data_ptr(), k.stride(0), k.stride(1), v.data_ptr(), v.stride(0), v.stride(1), starts,
+            rows)
 
 
 def kv_cache_read(
@@ -319,8 +328,8 @@ def kv_cache_read(
     shape = (args.batch, tokens, args.heads, args.dim)
     k, v = (torch.empty(shape, device=device, dtype=BF16) for _ in range(2))
     if k.numel():
-        with _on(device), _timed("kv_cache_read", 0.0, 6.0 * k.numel()):
-            _lib.call("kino_q8_cache_read", args, k.data_ptr(), v.data_ptr(), tokens, _stream())
+        _launch("kv_cache_read", 0.0, 6.0 * k.numel(), device, "kino_q8_cache_read", args,
+                k.data_ptr(), v.data_ptr(), tokens)
     return k, v
 
 
@@ -348,22 +357,27 @@ def kv_cache_attention(
     if heads % args.heads:
         raise ValueError(f"{heads} query heads on {args.heads} cache heads")
     if out is None:
-        out = torch.empty(q.shape, device=device, dtype=BF16)
+        out = torch.empty_like(q, memory_format=torch.contiguous_format)
     else:
         _heads(out, "out", args.dim, device)
         if out.shape != q.shape:
             raise ValueError(f"out {tuple(out.shape)} does not match q {tuple(q.shape)}")
     if not rows or not heads or not args.batch:
         return out
-    starts = _starts(token_starts, args.batch, rows, device)
-    with _on(device), _timed("kv_cache_attention"):
-        call = _lib.Q8AttentionArgs(
-            q.data_ptr(), q.stride(0), q.stride(1), out.data_ptr(), out.stride(0), out.stride(1),
-            starts, rows, heads, args.dim**-0.5 if scale is None else scale, int(causal))
-        size = _lib.load().kino_q8_attention_workspace_size(args, call)
-        if size < 0:
-            raise RuntimeError(f"kino_q8_attention: {_lib.last_error()}")
-        space = torch.empty(size, device=device, dtype=torch.uint8)
-        call.workspace, call.workspace_bytes = space.data_ptr(), size
-        _lib.call("kino_q8_attention", args, call, _stream())
+    call = _lib.Q8AttentionArgs(
+        q.data_ptr(), q.stride(0), q.stride(1), out.data_ptr(), out.stride(0), out.stride(1),
+        _starts(token_starts, args.batch, rows, device), rows, heads,
+        args.dim**-0.5 if scale is None else scale, causal)
+    size = _entries.get("size") or _entries.setdefault(
+        "size", _lib.load().kino_q8_attention_workspace_size)
+    if device.index == torch.cuda.current_device():
+        nbytes = size(args, call)
+    else:  # it goes by the device's SMs
+        with torch.cuda.device(device):
+            nbytes = size(args, call)
+    if nbytes < 0:
+        raise RuntimeError(f"kino_q8_attention: {_lib.last_error()}")
+    space = torch.empty(nbytes, device=device, dtype=torch.uint8)
+    call.workspace, call.workspace_bytes = space.data_ptr(), nbytes
+    _launch("kv_cache_attention", 0.0, 0.0, device, "kino_q8_attention", args, call)
     return out
