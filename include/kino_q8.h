@@ -4,9 +4,9 @@
  *
  * Values are held as 8-bit codes times an fp32 scale for a group: a token's row, a weight's output
  * channel, or the tokens of one cache block and head. With top = 127 (KINO_Q8_INT8) or 448
- * (KINO_Q8_E4M3): scale = amax / top, codes = round-to-even(x * (1 / scale)). A group whose scale
- * would be below 2^-126 is zeros with scale 0; one with an infinity or a NaN gets the scale NaN
- * and codes 0 and reads back as NaN. The NaN pattern of e4m3 is never written and not expected.
+ * (KINO_Q8_E4M3): scale = amax / top, code = x * top / amax to the nearest code, ties to even. A
+ * group whose scale would be below 2^-126 is zeros with scale 0; one with an infinity or a NaN
+ * gets the scale NaN and codes 0 and reads back as NaN. The NaN pattern of e4m3 is never written and not expected.
  *
  * Sizes that the host cannot see (lengths, token starts, block tables) are checked by the kernels:
  * what does not fit is skipped, nothing out of range is touched, and kino_device_status() then

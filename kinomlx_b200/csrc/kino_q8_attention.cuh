@@ -162,8 +162,8 @@ __device__ __forceinline__ int64_t q8_run_units(const Q8Attn& a, int64_t total) 
 
 // ---------------------------------------------------------------- few query rows
 // Up to 8 NT query rows (tokens x group) an item, keys in units of 64. Bound by reading the cache:
-// warp 8 brings each unit (K and V of 64 tokens, 128 D bytes) to shared memory by TMA, up to
-// Q8D_STAGES units ahead; warps 0..3 and 4..7 take turns on the units, 16 keys a warp.
+// the last warp brings each unit (K and V of 64 tokens, 128 D bytes) to shared memory by TMA, up to
+// STAGES units ahead; the others take turns on the units in groups of four, 16 keys a warp.
 //
 // The products use mma.sync with the keys (then the dims of V) as the 16 rows and the query rows
 // as the 8 columns, so that a single decoded token with a group of up to 8 heads fills a tile;
@@ -172,8 +172,9 @@ __device__ __forceinline__ int64_t q8_run_units(const Q8Attn& a, int64_t total) 
 // a fragment's rows and columns stand for, so nothing is transposed but the 16 x 8
 // probabilities (movmatrix).
 constexpr int Q8D_BN = 64;
-constexpr int Q8D_WARPS = 8;
-constexpr int Q8D_THREADS = 32 * (Q8D_WARPS + 1);
+// Warps that compute: one takes about 1300 cycles for its 16 keys, mostly latency, so three a
+// scheduler for one tile of rows; two tiles' accumulators leave registers for two.
+constexpr int q8d_warps(int nt) { return nt == 1 ? 12 : 8; }
 
 template <int D, int NT>
 struct Q8DecodeSmem {
@@ -182,9 +183,10 @@ struct Q8DecodeSmem {
   static constexpr int STAGES = D == 128 ? 8 : 16;
   static constexpr int LDO = D + 4;        // padded row of the merge buffer, in floats
   static constexpr int MERGE_OFF = STAGES * STAGE;
-  static constexpr int MERGE = Q8D_WARPS * 8 * NT * LDO * 4;
+  static constexpr int WARPS = q8d_warps(NT);
+  static constexpr int MERGE = WARPS * 8 * NT * LDO * 4;
   static constexpr int ML_OFF = MERGE_OFF + MERGE;      // [warp][8 NT][2]
-  static constexpr int SC_OFF = ML_OFF + Q8D_WARPS * 8 * NT * 8;
+  static constexpr int SC_OFF = ML_OFF + WARPS * 8 * NT * 8;
   // per stage, of the four 16-key groups: K scales (with the softmax scale), 1 / vs, log2(vs), and
   // a word of which groups are there
   static constexpr int SC = 64;
@@ -215,7 +217,7 @@ __device__ __forceinline__ uint32_t q8_chunk(int r, int c) {
 }
 
 template <int D, int NT, int FMT>
-__global__ void __launch_bounds__(Q8D_THREADS, 1)
+__global__ void __launch_bounds__(32 * (q8d_warps(NT) + 1), 1)
     attention_q8_decode_kernel(const __grid_constant__ CUtensorMap map_k,
                                const __grid_constant__ CUtensorMap map_v, const Q8Attn a) {
   using L = Q8DecodeSmem<D, NT>;
@@ -249,7 +251,7 @@ __global__ void __launch_bounds__(Q8D_THREADS, 1)
     }
   } else if (warp == 1 && lane == 0) {
     for (int i = 0; i < L::STAGES; ++i) {
-      mbar_init(&full[i], 1);
+      mbar_init(&full[i], 2);  // the copies, the scales
       mbar_init(&empty[i], 4);
     }
     fence_barrier_init();
@@ -263,7 +265,8 @@ __global__ void __launch_bounds__(Q8D_THREADS, 1)
   w.head = s_item[2];
   w.units = Q8Work<Q8D_BN>::units_of(a, w.count, w.len, w.tile);
 
-  if (warp == Q8D_WARPS) {
+  constexpr int WARPS = L::WARPS;
+  if (warp == WARPS) {
     // ---- loads
     constexpr int PAGES = Q8D_BN / 16;  // cache blocks of a unit, at most
     const int per = a.block >= Q8D_BN ? 1 : Q8D_BN / a.block;
@@ -306,6 +309,15 @@ __global__ void __launch_bounds__(Q8D_THREADS, 1)
           }
           const int l0 = i * per;  // the unit's first lane
           const unsigned there = (__ballot_sync(0xffffffffu, row >= 0) >> l0) & ((1u << per) - 1);
+          // the copies first: the scales of the lot may still be on their way
+          if (lane == 0)
+            mbar_expect_tx(&full[stage], static_cast<uint32_t>(__popc(there) * box * D * 2));
+          __syncwarp();
+          if (lane >= l0 && lane < l0 + per && row >= 0) {
+            uint8_t* dst = smem + stage * L::STAGE + (lane - l0) * box * D;
+            tma_load_2d(dst, &map_k, &full[stage], 0, row);
+            tma_load_2d(dst + L::HALF, &map_v, &full[stage], 0, row);
+          }
           float* sc = reinterpret_cast<float*>(smem + L::SC_OFF + stage * L::SC);
           // group g of 16 keys belongs to load g * per / 4
           const int src = l0 + (lane & 3) * per / PAGES;
@@ -321,14 +333,7 @@ __global__ void __launch_bounds__(Q8D_THREADS, 1)
           }
           if (lane == 0) reinterpret_cast<unsigned*>(sc)[3 * PAGES] = groups;
           __syncwarp();
-          if (lane == 0)
-            mbar_expect_tx(&full[stage], static_cast<uint32_t>(__popc(there) * box * D * 2));
-          __syncwarp();
-          if (lane >= l0 && lane < l0 + per && row >= 0) {
-            uint8_t* dst = smem + stage * L::STAGE + (lane - l0) * box * D;
-            tma_load_2d(dst, &map_k, &full[stage], 0, row);
-            tma_load_2d(dst + L::HALF, &map_v, &full[stage], 0, row);
-          }
+          if (lane == 0) mbar_arrive(&full[stage]);
           ++issued;
         }
       }
@@ -349,11 +354,11 @@ __global__ void __launch_bounds__(Q8D_THREADS, 1)
     // ---- products and softmax
     const int g = lane >> 2, t = lane & 3;
     const int part = warp & 3;   // 16 keys of the unit
-    const int turn = warp >> 2;  // which of two units
+    const int turn = warp >> 2;  // which of WARPS / 4 units
     constexpr int KS = D / 16;   // steps of the first product, row tiles of the second
     float* merge = reinterpret_cast<float*>(smem + L::MERGE_OFF);
     float* ml = reinterpret_cast<float*>(smem + L::ML_OFF);
-    int used = 0;
+    int used = 0, mine = 0;  // units so far, and of WARPS / 4 the one that is next
     int piece = 0;
     bool ok = true;
     while (left > 0) {
@@ -423,7 +428,9 @@ __global__ void __launch_bounds__(Q8D_THREADS, 1)
         }
       }
       for (int u = 0; u < n; ++u, ++used) {
-        if ((used & 1) != turn) continue;
+        const bool take = mine == turn;
+        mine = mine + 1 == WARPS / 4 ? 0 : mine + 1;
+        if (!take) continue;
         const int stage = used % L::STAGES;
         ok = ok && __all_sync(0xffffffffu,
                               mbar_wait(&full[stage], (used / L::STAGES) & 1, abort_flag));
@@ -543,7 +550,7 @@ __global__ void __launch_bounds__(Q8D_THREADS, 1)
         __syncwarp();
         if (lane == 0) mbar_arrive(&empty[stage]);
       }
-      // ---- the eight warps' results of this item
+      // ---- the warps' results of this item
 #pragma unroll
       for (int j = 0; j < NT; ++j)
 #pragma unroll
@@ -560,20 +567,20 @@ __global__ void __launch_bounds__(Q8D_THREADS, 1)
           for (int i = 0; i < KS; ++i)
             *reinterpret_cast<float2*>(dst + 2 * i) = make_float2(o[j][i][e], o[j][i][2 + e]);
         }
-      asm volatile("bar.sync 1, 256;" ::: "memory");
+      asm volatile("bar.sync 1, %0;" ::"n"(32 * WARPS) : "memory");
       const int slot = 2 * static_cast<int>(blockIdx.x) + (piece > 0 ? 1 : 0);
-      for (int e = threadIdx.x; e < 8 * NT * (D / 4); e += 32 * Q8D_WARPS) {
+      for (int e = threadIdx.x; e < 8 * NT * (D / 4); e += 32 * WARPS) {
         const int r = e / (D / 4), c = (e % (D / 4)) * 4;
         const int tok = tok0 + r / a.group;
         if (r >= a.tile_tokens * a.group || tok >= w.count) continue;
         float top = -INFINITY;
 #pragma unroll
-        for (int k = 0; k < Q8D_WARPS; ++k) top = fmaxf(top, ml[(k * 8 * NT + r) * 2]);
+        for (int k = 0; k < WARPS; ++k) top = fmaxf(top, ml[(k * 8 * NT + r) * 2]);
         const float ref = top > -INFINITY ? top : 0.0f;
         float sum = 0.0f;
         float4 y = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
 #pragma unroll
-        for (int k = 0; k < Q8D_WARPS; ++k) {
+        for (int k = 0; k < WARPS; ++k) {
           const float wt = ex2_approx(ml[(k * 8 * NT + r) * 2] - ref);
           sum += wt * ml[(k * 8 * NT + r) * 2 + 1];
           const float4 x = *reinterpret_cast<const float4*>(merge + (k * 8 * NT + r) * L::LDO + c);
@@ -596,7 +603,7 @@ __global__ void __launch_bounds__(Q8D_THREADS, 1)
           }
         }
       }
-      asm volatile("bar.sync 1, 256;" ::: "memory");
+      asm volatile("bar.sync 1, %0;" ::"n"(32 * WARPS) : "memory");
       left -= n;
       at = 0;
       ++piece;
@@ -1288,8 +1295,8 @@ __global__ void __launch_bounds__(Q8P_THREADS, 1)
 // first and last is in slot 0.) gridDim.y CTAs share the rows.
 template <int D, int BN>
 __global__ void __launch_bounds__(256) attention_q8_combine_kernel(const Q8Attn a) {
-  griddep_wait();
-  griddep_launch();
+  // This kernel may start when every CTA of the attention has passed its own wait for what ran
+  // before it, so lengths and starts are there and the items can be found while it still runs.
   __shared__ int s_item[4];      // b, tile, head, pieces (0: nothing to do)
   __shared__ int s_slot0;
   Q8Work<BN> w(a);
@@ -1315,6 +1322,8 @@ __global__ void __launch_bounds__(256) attention_q8_combine_kernel(const Q8Attn 
     }
   }
   __syncthreads();
+  griddep_wait();  // the pieces
+  griddep_launch();
   const int pieces = s_item[3];
   if (pieces == 0) return;
   w.enter(s_item[0]);

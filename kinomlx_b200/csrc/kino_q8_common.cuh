@@ -2,13 +2,14 @@
 // conversions between codes and floating values.
 //
 // A group of values (a token's row, a weight's output channel, the tokens of one cache block and
-// head) is held as codes times one fp32 scale:
-//   scale = amax / top (top 127 for int8, 448 for e4m3), codes = round-to-even(x * (1 / scale)).
-// The reciprocal is taken once a group (IEEE) and multiplied, so that a code is one fp32 product
-// and one rounding: the same two operations in any implementation give the same code. A group
-// whose scale would fall below 2^-126 (1 / scale would overflow) is a group of zeros with scale 0;
-// one that holds an infinity or a NaN gets the scale NaN and codes 0, so that it reads back as
-// NaN wherever it is used and no code is ever a NaN pattern.
+// head) is held as codes times one fp32 scale, amax / top (top 127 for int8, 448 for e4m3):
+//   code = x * top / amax, rounded to fp32 and then to the code grid, to nearest even both times.
+// The quotient's first rounding is exact to 2^-48 (see Q8Factor), so a value that lies on the
+// border of two codes, which bf16 values often do (amax / 2 in int8), goes to the even one and
+// not where the rounding of a reciprocal happens to push it. A group whose scale would fall below
+// 2^-126 (1 / scale would overflow) is a group of zeros with scale 0; one that holds an infinity
+// or a NaN gets the scale NaN and codes 0, so that it reads back as NaN wherever it is used and no
+// code is ever a NaN pattern.
 #pragma once
 #include <cuda_fp8.h>
 
@@ -37,9 +38,18 @@ __device__ __forceinline__ float q8_scale(uint32_t amax_bits) {
   return s < Q8_LEAST_SCALE ? 0.0f : s;
 }
 
-// What a group's values are multiplied by; 0 for scales 0 and NaN.
-__device__ __forceinline__ float q8_inverse(float scale) {
-  return scale > 0.0f ? __frcp_rn(scale) : 0.0f;
+// A factor of about 48 bits: x * (hi + lo) as fma(x, hi, x * lo) has one rounding that counts.
+struct Q8Factor {
+  float hi, lo;
+  __device__ __forceinline__ float times(float x) const { return fmaf(x, hi, x * lo); }
+};
+
+// a / b (b > 0 and the quotient in range).
+__device__ __forceinline__ Q8Factor q8_quotient(float a, float b) {
+  Q8Factor f;
+  f.hi = __fdiv_rn(a, b);
+  f.lo = __fdiv_rn(fmaf(-f.hi, b, a), b);
+  return f;
 }
 
 __device__ __forceinline__ uint32_t abs_bits(float x) { return __float_as_uint(x) & 0x7FFFFFFFu; }

@@ -16,12 +16,14 @@ __device__ __forceinline__ void q8_unpack8(const uint4& raw, float (&f)[8]) {
 }
 
 // ---------------------------------------------------------------- token rows
-// One CTA a row: h = bf16(x + residual), y = h * rsqrt(mean h^2 + eps) * (weight + offset) in
-// fp32, then codes and a scale for the row. The row is read once and stays in registers over the
-// two reductions (sum of squares, largest magnitude), so the kernel moves 2 bytes of x, 2 of the
-// residual in, 2 of the sum out and 1 of code per element: it is bound by HBM. The statistics are
-// taken from the rounded sum, which is what the next layer reads, so that the fused form equals
-// an addition followed by the norm.
+// One CTA a row: h = bf16(x + residual), y = h * rsqrt(mean h^2 + eps) * (weight + offset), then
+// codes and a scale for the row. The row's common factor r = rsqrt(..) cancels in the codes,
+// y top / amax(y) = p top / amax(p) with p = h * (weight + offset), so the sum of squares and the
+// largest |p| come from one reduction and r only enters the scale. The row is read once and stays
+// in registers: 2 bytes of x, 2 of the residual in, 2 of the sum out and 1 of code per element;
+// bound by HBM. The statistics are taken from the rounded sum, which is what the next layer reads,
+// so that the fused form equals an addition followed by the norm. (p is exact for bf16 weights
+// without an offset.)
 constexpr int Q8_ROW_MAX_THREADS = 512;
 
 struct Q8RowArgs {
@@ -66,8 +68,10 @@ __global__ void __launch_bounds__(Q8_ROW_MAX_THREADS) q8_rows_kernel(const Q8Row
   }
   float v[NV][8];
   float sum = 0.0f;
+  uint32_t top = 0;
 #pragma unroll
   for (int i = 0; i < NV; ++i) {
+    const int c = threadIdx.x + i * blockDim.x;
     q8_unpack8(raw[i], v[i]);
     if (a.residual != nullptr) {
       float r[8];
@@ -75,65 +79,52 @@ __global__ void __launch_bounds__(Q8_ROW_MAX_THREADS) q8_rows_kernel(const Q8Row
 #pragma unroll
       for (int j = 0; j < 8; ++j) v[i][j] = bf16_round(v[i][j] + r[j]);
     }
+    if (a.hidden != nullptr && c < nvec)
+      reinterpret_cast<uint4*>(a.hidden + row * a.ld_hidden)[c] =
+          make_uint4(pack_bf16x2(v[i][0], v[i][1]), pack_bf16x2(v[i][2], v[i][3]),
+                     pack_bf16x2(v[i][4], v[i][5]), pack_bf16x2(v[i][6], v[i][7]));
 #pragma unroll
     for (int j = 0; j < 8; ++j) sum = fmaf(v[i][j], v[i][j], sum);
-  }
-  if (a.hidden != nullptr) {
-    uint4* hr = reinterpret_cast<uint4*>(a.hidden + row * a.ld_hidden);
+    if (a.weight != nullptr && c < nvec) {
+      float w[8];
+      q8_unpack8(__ldg(reinterpret_cast<const uint4*>(a.weight) + c), w);
 #pragma unroll
-    for (int i = 0; i < NV; ++i) {
-      const int c = threadIdx.x + i * blockDim.x;
-      if (c < nvec)
-        hr[c] = make_uint4(pack_bf16x2(v[i][0], v[i][1]), pack_bf16x2(v[i][2], v[i][3]),
-                           pack_bf16x2(v[i][4], v[i][5]), pack_bf16x2(v[i][6], v[i][7]));
+      for (int j = 0; j < 8; ++j) v[i][j] *= w[j] + a.weight_offset;
     }
-  }
-  if (a.norm) {
-    sum = warp_sum_f(sum);
-    if (warps > 1) {
-      if ((threadIdx.x & 31) == 0) s_sum[threadIdx.x >> 5] = sum;
-      __syncthreads();
-      sum = (threadIdx.x & 31) < warps ? s_sum[threadIdx.x & 31] : 0.0f;
-      sum = warp_sum_f(sum);
-    }
-    const float inv = rsqrtf(sum / static_cast<float>(a.dim) + a.eps);
-#pragma unroll
-    for (int i = 0; i < NV; ++i) {
-      const int c = threadIdx.x + i * blockDim.x;
-      if (a.weight != nullptr && c < nvec) {
-        float w[8];
-        q8_unpack8(__ldg(reinterpret_cast<const uint4*>(a.weight) + c), w);
-#pragma unroll
-        for (int j = 0; j < 8; ++j) v[i][j] = v[i][j] * inv * (w[j] + a.weight_offset);
-      } else {
-#pragma unroll
-        for (int j = 0; j < 8; ++j) v[i][j] *= inv;
-      }
-    }
-  }
-  uint32_t top = 0;
-#pragma unroll
-  for (int i = 0; i < NV; ++i)
 #pragma unroll
     for (int j = 0; j < 8; ++j) top = max(top, abs_bits(v[i][j]));
-  top = __reduce_max_sync(0xffffffffu, top);
-  if (warps > 1) {
-    if ((threadIdx.x & 31) == 0) s_max[threadIdx.x >> 5] = top;
-    __syncthreads();
-    top = (threadIdx.x & 31) < warps ? s_max[threadIdx.x & 31] : 0u;
-    top = __reduce_max_sync(0xffffffffu, top);
   }
-  const float scale = q8_scale<FMT>(top);
-  const float inv = q8_inverse(scale);
+  top = __reduce_max_sync(0xffffffffu, top);
+  if (a.norm) sum = warp_sum_f(sum);
+  if (warps > 1) {
+    if ((threadIdx.x & 31) == 0) {
+      s_sum[threadIdx.x >> 5] = sum;
+      s_max[threadIdx.x >> 5] = top;
+    }
+    __syncthreads();
+    const int w = threadIdx.x & 31;
+    top = __reduce_max_sync(0xffffffffu, w < warps ? s_max[w] : 0u);
+    if (a.norm) sum = warp_sum_f(w < warps ? s_sum[w] : 0.0f);
+  }
+  float scale = q8_scale<FMT>(top);
+  Q8Factor f = {0.0f, 0.0f};
+  if (scale > 0.0f) {
+    f = q8_quotient(q8_top<FMT>(), __uint_as_float(top));
+    if (a.norm) {
+      scale *= rsqrtf(sum / static_cast<float>(a.dim) + a.eps);
+      if (scale < Q8_LEAST_SCALE) scale = f.hi = f.lo = 0.0f;
+    }
+  }
   if (threadIdx.x == 0) a.scales[row] = scale;
   uint2* cr = reinterpret_cast<uint2*>(a.codes + row * a.dim);
 #pragma unroll
   for (int i = 0; i < NV; ++i) {
     const int c = threadIdx.x + i * blockDim.x;
     if (c < nvec)
-      cr[c] = make_uint2(
-          q8_encode4<FMT>(v[i][0] * inv, v[i][1] * inv, v[i][2] * inv, v[i][3] * inv),
-          q8_encode4<FMT>(v[i][4] * inv, v[i][5] * inv, v[i][6] * inv, v[i][7] * inv));
+      cr[c] = make_uint2(q8_encode4<FMT>(f.times(v[i][0]), f.times(v[i][1]), f.times(v[i][2]),
+                                         f.times(v[i][3])),
+                         q8_encode4<FMT>(f.times(v[i][4]), f.times(v[i][5]), f.times(v[i][6]),
+                                         f.times(v[i][7])));
   }
 }
 
@@ -242,21 +233,30 @@ __global__ void __launch_bounds__(Q8_WRITE_THREADS) q8_cache_write_kernel(const 
   __syncthreads();  // every thread has read the old scale
 #pragma unroll
   for (int i = 0; i < Q8_WRITE_THREADS / 32; ++i) top = max(top, s_max[i]);
-  float scale = q8_scale<FMT>(top);
-  if (!(before <= scale)) scale = before == before && scale == scale ? before : __uint_as_float(0x7FC00000u);
-  const float inv = q8_inverse(scale);
+  const float own = q8_scale<FMT>(top);
+  // the larger of the two; NaN wins
+  const float scale = before > own ? before : before == before ? own : before;
+  Q8Factor f = {0.0f, 0.0f}, again = {0.0f, 0.0f};
+  if (scale > 0.0f) {
+    if (scale > before) {  // the new tokens' own
+      f = q8_quotient(q8_top<FMT>(), __uint_as_float(top));
+      again.hi = before * f.hi;  // what the earlier codes are multiplied by
+      again.lo = fmaf(before, f.hi, -again.hi) + before * f.lo;
+    } else {
+      f = q8_quotient(1.0f, before);
+    }
+  }
   if (threadIdx.x == 0) a.scales[kv][unit] = scale;
   const bool grown = earlier && scale > before;
-  const float ratio = before * inv;
 #pragma unroll
   for (int i = 0; i < NV; ++i) {
     const int e = threadIdx.x + i * Q8_WRITE_THREADS;
     uint2* dst = reinterpret_cast<uint2*>(codes) + e;
-    float f[8];
+    float v[8];
     if (fresh[i]) {
-      q8_unpack8(raw[i], f);
+      q8_unpack8(raw[i], v);
 #pragma unroll
-      for (int j = 0; j < 8; ++j) f[j] *= inv;
+      for (int j = 0; j < 8; ++j) v[j] = f.times(v[j]);
     } else if (grown && at0 + e / chunks < held) {
       const uint2 old = *dst;
       float lo[4], hi[4];
@@ -264,14 +264,14 @@ __global__ void __launch_bounds__(Q8_WRITE_THREADS) q8_cache_write_kernel(const 
       q8_decode4<FMT>(old.y, hi);
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
-        f[j] = lo[j] * ratio;
-        f[4 + j] = hi[j] * ratio;
+        v[j] = again.times(lo[j]);
+        v[4 + j] = again.times(hi[j]);
       }
     } else {
       continue;
     }
-    *dst = make_uint2(q8_encode4<FMT>(f[0], f[1], f[2], f[3]),
-                      q8_encode4<FMT>(f[4], f[5], f[6], f[7]));
+    *dst = make_uint2(q8_encode4<FMT>(v[0], v[1], v[2], v[3]),
+                      q8_encode4<FMT>(v[4], v[5], v[6], v[7]));
   }
 }
 

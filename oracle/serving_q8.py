@@ -1,9 +1,9 @@
 """The 8-bit serving operators from their definitions in 64 bits, on the CPU.
 
-Codes are whole numbers (int8) or the values of e4m3 codes, as float64. The quantisation of bf16
-values is also given in fp32 steps (`scale_f32`, `codes_f32`): one correctly rounded quotient, one
-reciprocal, one product and one rounding, so that another implementation of the same steps has to
-give the same codes bit for bit.
+Codes are whole numbers (int8) or the values of e4m3 codes, as float64. Quantisation of bf16 values
+is given with the roundings of an implementation in fp32 (`scale_f32`, `codes`): the scale is one
+correctly rounded quotient, a code the exact quotient x * top / amax rounded to fp32 and then to the
+code grid, so that another implementation of the same steps has to give the same codes bit for bit.
 """
 
 from __future__ import annotations
@@ -23,26 +23,34 @@ def scale_f32(amax: torch.Tensor, dtype: torch.dtype) -> torch.Tensor:
     return torch.where(torch.isfinite(amax), s, torch.full_like(s, math.nan))
 
 
-def inverse_f32(scale: torch.Tensor) -> torch.Tensor:
-    return torch.where(scale > 0, 1.0 / scale, torch.zeros_like(scale))
-
-
-def codes_f32(scaled: torch.Tensor, dtype: torch.dtype) -> torch.Tensor:
-    """Codes of already scaled fp32 values; NaN gives 0."""
-    x = torch.nan_to_num(scaled, nan=0.0, posinf=TOP[dtype], neginf=-TOP[dtype])
+def codes(quotient: torch.Tensor, dtype: torch.dtype) -> torch.Tensor:
+    """Codes of float64 quotients; what is not finite gives 0."""
+    x = torch.where(torch.isfinite(quotient), quotient, torch.zeros_like(quotient)).float()
     if dtype == torch.int8:
         return x.round().clamp(-127, 127).to(torch.int8)
     return x.clamp(-448, 448).to(torch.float8_e4m3fn)
 
 
+def amax(x: torch.Tensor, dims) -> torch.Tensor:
+    """Largest magnitudes over dims as float64, NaN where something is not finite."""
+    top = torch.nan_to_num(x, nan=0.0, posinf=0.0, neginf=0.0).to(F64).abs().amax(dims)
+    bad = ~torch.isfinite(x)
+    for d in sorted(dims, reverse=True):
+        bad = bad.any(d)
+    return torch.where(bad, torch.full_like(top, math.nan), top)
+
+
+def quotients(x: torch.Tensor, top: torch.Tensor, scale: torch.Tensor, dtype: torch.dtype):
+    """x * (127 or 448) / top where the scale counts, 0 where it is 0 or NaN."""
+    y = x.to(F64) * TOP[dtype] / top
+    return torch.where(scale > 0, y, torch.zeros_like(y))
+
+
 def quantize_rows(x: torch.Tensor, dtype: torch.dtype):
-    """(codes, scales) of the last dimension, in fp32 steps."""
-    x = x.float()
-    bad = ~torch.isfinite(x).all(-1)
-    amax = torch.nan_to_num(x, nan=0.0, posinf=0.0, neginf=0.0).abs().amax(-1)
-    scale = scale_f32(torch.where(bad, torch.full_like(amax, math.nan), amax), dtype)
-    codes = codes_f32(x * inverse_f32(scale)[..., None], dtype)
-    return torch.where(bad[..., None], torch.zeros_like(codes.float()), codes.float()).to(dtype), scale
+    """(codes, scales) of the last dimension."""
+    top = amax(x, (x.dim() - 1,))
+    scale = scale_f32(top, dtype)
+    return codes(quotients(x, top[..., None], scale[..., None], dtype), dtype), scale
 
 
 def rms_norm(x, weight=None, eps=1e-6, residual=None, offset=0.0):
@@ -66,10 +74,10 @@ def rows_of(starts, batch: int, rows: int) -> list[tuple[int, int]]:
     return [(s[b], s[b + 1] - s[b]) for b in range(batch)]
 
 
-def cache_write(codes, scales, x, table, lengths, starts=None):
-    """New (codes, scales) of one of keys or values, in fp32 steps; x (rows, heads, dim)."""
-    dtype, block = codes.dtype, codes.shape[2]
-    codes, scales = codes.float().clone(), scales.clone()
+def cache_write(held_codes, held_scales, x, table, lengths, starts=None):
+    """New (codes, scales) of one of keys or values; x (rows, heads, dim)."""
+    dtype, block = held_codes.dtype, held_codes.shape[2]
+    out, scales = held_codes.float().clone(), held_scales.clone()
     for b, (first, n) in enumerate(rows_of(starts, len(lengths), x.shape[0])):
         held = int(lengths[b])
         for j in range(held // block, (held + n - 1) // block + 1 if n else 0):
@@ -77,20 +85,19 @@ def cache_write(codes, scales, x, table, lengths, starts=None):
             t0, t1 = max(held, j * block), min(held + n, (j + 1) * block)
             new = x[first + t0 - held : first + t1 - held].float().transpose(0, 1)
             earlier = max(0, held - j * block)
-            bad = ~torch.isfinite(new).all(-1).all(-1)
-            amax = torch.nan_to_num(new, nan=0.0, posinf=0.0, neginf=0.0).abs().amax((1, 2))
-            scale = scale_f32(torch.where(bad, torch.full_like(amax, math.nan), amax), dtype)
+            top = amax(new, (1, 2))[:, None, None]
+            own = scale_f32(top, dtype)
+            before = scales[page][:, None, None] if earlier else torch.zeros_like(own)
+            scale = torch.maximum(own, before)  # NaN wins
             if earlier:
-                before = scales[page]
-                scale = torch.maximum(scale, before)  # NaN wins
-                ratio = torch.where(scale > before, before * inverse_f32(scale), torch.ones_like(scale))
-                old = codes[page, :, :earlier]
-                again = codes_f32(old * ratio[:, None, None], dtype).float()
-                codes[page, :, :earlier] = torch.where((scale > before)[:, None, None], again, old)
-            codes[page, :, t0 - j * block : t1 - j * block] = codes_f32(
-                new * inverse_f32(scale)[:, None, None], dtype).float()
-            scales[page] = scale
-    return codes.to(dtype), scales
+                old = out[page, :, :earlier]
+                again = codes(quotients(old.to(F64) * before.to(F64), top, scale, dtype), dtype).float()
+                out[page, :, :earlier] = torch.where(scale > before, again, old)
+            value = torch.where(scale > before, quotients(new, top, scale, dtype),
+                                torch.where(scale > 0, new.to(F64) / before.to(F64), 0.0))
+            out[page, :, t0 - j * block : t1 - j * block] = codes(value, dtype).float()
+            scales[page] = scale[:, 0, 0]
+    return out.to(dtype), scales
 
 
 def cached(codes, scales, table_row, length: int) -> torch.Tensor:
