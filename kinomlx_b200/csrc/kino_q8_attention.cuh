@@ -180,10 +180,15 @@ template <int D, int NT>
 struct Q8DecodeSmem {
   static constexpr int HALF = Q8D_BN * D;  // K or V of a unit
   static constexpr int STAGE = 2 * HALF;
-  static constexpr int STAGES = D == 128 ? 8 : 16;
+  static constexpr int WARPS = q8d_warps(NT);
+  // A multiple of the groups that take turns: a stage then always belongs to the same group, which
+  // has seen each earlier phase of its barrier. (Another group could come to a stage whose last
+  // load is still on its way, since loads need not arrive in order, and take the phase before that
+  // for its own.)
+  static constexpr int STAGES = WARPS == 12 ? (D == 128 ? 9 : 18) : (D == 128 ? 8 : 16);
+  static_assert(STAGES % (WARPS / 4) == 0, "a stage belongs to one group of warps");
   static constexpr int LDO = D + 4;        // padded row of the merge buffer, in floats
   static constexpr int MERGE_OFF = STAGES * STAGE;
-  static constexpr int WARPS = q8d_warps(NT);
   static constexpr int MERGE = WARPS * 8 * NT * LDO * 4;
   static constexpr int ML_OFF = MERGE_OFF + MERGE;      // [warp][8 NT][2]
   static constexpr int SC_OFF = ML_OFF + WARPS * 8 * NT * 8;
