@@ -172,26 +172,24 @@ __device__ __forceinline__ int64_t q8_run_units(const Q8Attn& a, int64_t total) 
 // a fragment's rows and columns stand for, so nothing is transposed but the 16 x 8
 // probabilities (movmatrix).
 constexpr int Q8D_BN = 64;
-// Warps that compute: one takes about 1300 cycles for its 16 keys, mostly latency, so three a
-// scheduler for one tile of rows; two tiles' accumulators leave registers for two.
-constexpr int q8d_warps(int nt) { return nt == 1 ? 12 : 8; }
+constexpr int Q8D_WARPS = 8;  // that compute; one more loads
+constexpr int Q8D_THREADS = 32 * (Q8D_WARPS + 1);
 
 template <int D, int NT>
 struct Q8DecodeSmem {
   static constexpr int HALF = Q8D_BN * D;  // K or V of a unit
   static constexpr int STAGE = 2 * HALF;
-  static constexpr int WARPS = q8d_warps(NT);
   // A multiple of the groups that take turns: a stage then always belongs to the same group, which
   // has seen each earlier phase of its barrier. (Another group could come to a stage whose last
   // load is still on its way, since loads need not arrive in order, and take the phase before that
   // for its own.)
-  static constexpr int STAGES = WARPS == 12 ? (D == 128 ? 9 : 18) : (D == 128 ? 8 : 16);
-  static_assert(STAGES % (WARPS / 4) == 0, "a stage belongs to one group of warps");
+  static constexpr int STAGES = (NT == 1 ? 10 : 8) * (D == 128 ? 1 : 2);
+  static_assert(STAGES % (Q8D_WARPS / 4) == 0, "a stage belongs to one group of warps");
   static constexpr int LDO = D + 4;        // padded row of the merge buffer, in floats
   static constexpr int MERGE_OFF = STAGES * STAGE;
-  static constexpr int MERGE = WARPS * 8 * NT * LDO * 4;
+  static constexpr int MERGE = Q8D_WARPS * 8 * NT * LDO * 4;
   static constexpr int ML_OFF = MERGE_OFF + MERGE;      // [warp][8 NT][2]
-  static constexpr int SC_OFF = ML_OFF + WARPS * 8 * NT * 8;
+  static constexpr int SC_OFF = ML_OFF + Q8D_WARPS * 8 * NT * 8;
   // per stage, of the four 16-key groups: K scales (with the softmax scale), 1 / vs, log2(vs), and
   // a word of which groups are there
   static constexpr int SC = 64;
@@ -222,7 +220,7 @@ __device__ __forceinline__ uint32_t q8_chunk(int r, int c) {
 }
 
 template <int D, int NT, int FMT>
-__global__ void __launch_bounds__(32 * (q8d_warps(NT) + 1), 1)
+__global__ void __launch_bounds__(Q8D_THREADS, 1)
     attention_q8_decode_kernel(const __grid_constant__ CUtensorMap map_k,
                                const __grid_constant__ CUtensorMap map_v, const Q8Attn a) {
   using L = Q8DecodeSmem<D, NT>;
@@ -270,81 +268,84 @@ __global__ void __launch_bounds__(32 * (q8d_warps(NT) + 1), 1)
   w.head = s_item[2];
   w.units = Q8Work<Q8D_BN>::units_of(a, w.count, w.len, w.tile);
 
-  constexpr int WARPS = L::WARPS;
-  if (warp == WARPS) {
-    // ---- loads
-    constexpr int PAGES = Q8D_BN / 16;  // cache blocks of a unit, at most
-    const int per = a.block >= Q8D_BN ? 1 : Q8D_BN / a.block;
+  if (warp == Q8D_WARPS) {
+    // ---- loads: the places and scales of up to eight units are looked up at once, a lane for each
+    // group of 16 keys, while the eight before them are issued (a look-up is two dependent reads,
+    // about a microsecond, in which two or three units arrive)
+    constexpr int GROUPS = Q8D_BN / 16, LOT = 32 / GROUPS, STEP = 2;
     const int box = a.block >= Q8D_BN ? Q8D_BN : a.block;
-    int issued = 0;
-    bool ok = true;
-    while (left > 0 && ok) {
+    const bool leads = (lane & 3) * 16 % box == 0;  // the copy of its group's box
+    const unsigned lead_groups = box == 64 ? 1u : box == 32 ? 5u : 15u;
+    int row = -1, count = 0;  // of the next units
+    float ks = 0.0f, rv = 0.0f, lv = 0.0f;
+    auto look = [&]() {
+      count = 0;
+      row = -1;
+      if (left <= 0) return;
       const int n = static_cast<int>(left < w.units - at ? left : w.units - at);
-      const int keys = Q8Work<Q8D_BN>::keys(a, w.count, w.len, w.tile);
-      const int32_t* table = a.table + static_cast<int64_t>(w.b) * a.ld_table;
-      // 32 / per units at a time: each lane looks up the place and scales of one load
-      const int lot = 32 / per;
-      for (int u = 0; u < n && ok; u += lot) {
-        const int key = (at + u) * Q8D_BN + lane * box;  // this lane's first key
-        int row = -1;
-        float ks = 0.0f, rv = 0.0f, lv = 0.0f;
-        if (u + lane / per < n && key < keys) {
-          const int page = table[key >> a.block_shift];
-          if (page >= 0 && page < a.num_blocks) {
-            const int unit = page * a.heads + w.head;
-            row = unit * a.block + (key & (a.block - 1));
-            // the codes stand in f16 as their value over q8_f16_unit, those of K and of V
-            ks = a.scales[0][unit] * a.scale_log2 * q8_f16_unit<FMT>();
-            const float vs = a.scales[1][unit];
-            const float v = vs <= Q8_LEAST_V ? Q8_LEAST_V : vs;
-            rv = 1.0f / (v * q8_f16_unit<FMT>());
-            lv = log2f(v);
-          } else {
-            q8_flag(1);
-          }
-        }
-        const int some = min(lot, n - u);
-        for (int i = 0; i < some; ++i) {
-          const int stage = issued % L::STAGES;
-          // (the whole warp goes on or gives up together)
-          if (!__all_sync(0xffffffffu, mbar_wait(&empty[stage], ((issued / L::STAGES) & 1) ^ 1u,
-                                                 abort_flag))) {
-            ok = false;
-            break;
-          }
-          const int l0 = i * per;  // the unit's first lane
-          const unsigned there = (__ballot_sync(0xffffffffu, row >= 0) >> l0) & ((1u << per) - 1);
-          // the copies first: the scales of the lot may still be on their way
-          if (lane == 0)
-            mbar_expect_tx(&full[stage], static_cast<uint32_t>(__popc(there) * box * D * 2));
-          __syncwarp();
-          if (lane >= l0 && lane < l0 + per && row >= 0) {
-            uint8_t* dst = smem + stage * L::STAGE + (lane - l0) * box * D;
-            tma_load_2d(dst, &map_k, &full[stage], 0, row);
-            tma_load_2d(dst + L::HALF, &map_v, &full[stage], 0, row);
-          }
-          float* sc = reinterpret_cast<float*>(smem + L::SC_OFF + stage * L::SC);
-          // group g of 16 keys belongs to load g * per / 4
-          const int src = l0 + (lane & 3) * per / PAGES;
-          const float gk = __shfl_sync(0xffffffffu, ks, src);
-          const float gr = __shfl_sync(0xffffffffu, rv, src);
-          const float gl = __shfl_sync(0xffffffffu, lv, src);
-          const unsigned groups =
-              __ballot_sync(0xffffffffu, lane < PAGES && ((there >> ((lane & 3) * per / PAGES)) & 1));
-          if (lane < PAGES) {
-            sc[lane] = gk;
-            sc[PAGES + lane] = gr;
-            sc[2 * PAGES + lane] = gl;
-          }
-          if (lane == 0) reinterpret_cast<unsigned*>(sc)[3 * PAGES] = groups;
-          __syncwarp();
-          if (lane == 0) mbar_arrive(&full[stage]);
-          ++issued;
+      count = n < LOT ? n : LOT;
+      const int key = (at + lane / GROUPS) * Q8D_BN + (lane & 3) * 16;
+      if (lane / GROUPS < count && key < Q8Work<Q8D_BN>::keys(a, w.count, w.len, w.tile)) {
+        const int page = a.table[static_cast<int64_t>(w.b) * a.ld_table + (key >> a.block_shift)];
+        if (page >= 0 && page < a.num_blocks) {
+          const int unit = page * a.heads + w.head;
+          row = unit * a.block + (key & (a.block - 1));
+          // the codes stand in f16 as their value over q8_f16_unit, those of K and of V
+          ks = a.scales[0][unit] * a.scale_log2 * q8_f16_unit<FMT>();
+          const float vs = a.scales[1][unit];
+          const float v = vs <= Q8_LEAST_V ? Q8_LEAST_V : vs;
+          rv = 1.0f / (v * q8_f16_unit<FMT>());
+          lv = log2f(v);
+        } else {
+          q8_flag(1);
         }
       }
-      left -= n;
-      at = 0;
-      if (left > 0) w.next();
+      left -= count;
+      at += count;
+      if (at == w.units) {
+        at = 0;
+        if (left > 0) w.next();
+      }
+    };
+    int issued = 0;
+    bool ok = true;
+    look();
+    while (count > 0) {
+      const int row_now = row, units = count;
+      const float ks_now = ks, rv_now = rv, lv_now = lv;
+      look();
+      const int mine = lane / GROUPS;
+      const int unit = issued + mine, stage = unit % L::STAGES;
+      for (int u = 0; u < units && ok; u += STEP) {
+        const bool active = mine >= u && mine < u + STEP && mine < units;
+        // (the whole warp goes on or gives up together)
+        ok = __all_sync(0xffffffffu,
+                        !active || mbar_wait(&empty[stage], ((unit / L::STAGES) & 1) ^ 1u, abort_flag));
+        if (!ok) break;
+        const unsigned groups =
+            (__ballot_sync(0xffffffffu, active && row_now >= 0) >> (lane & ~3)) & 15u;
+        // the copies first: the scales may still be on their way
+        if (active && (lane & 3) == 0)
+          mbar_expect_tx(&full[stage],
+                         static_cast<uint32_t>(__popc(groups & lead_groups) * box * D * 2));
+        __syncwarp();
+        if (active && row_now >= 0 && leads) {
+          uint8_t* dst = smem + stage * L::STAGE + (lane & 3) * 16 * D;
+          tma_load_2d(dst, &map_k, &full[stage], 0, row_now);
+          tma_load_2d(dst + L::HALF, &map_v, &full[stage], 0, row_now);
+        }
+        if (active) {
+          float* sc = reinterpret_cast<float*>(smem + L::SC_OFF + stage * L::SC);
+          sc[lane & 3] = ks_now;
+          sc[GROUPS + (lane & 3)] = rv_now;
+          sc[2 * GROUPS + (lane & 3)] = lv_now;
+          if ((lane & 3) == 0) reinterpret_cast<unsigned*>(sc)[3 * GROUPS] = groups;
+        }
+        __syncwarp();
+        if (active && (lane & 3) == 0) mbar_arrive(&full[stage]);
+      }
+      if (!ok) break;
+      issued += units;
     }
     if (*abort_flag && lane == 0) {  // copies in flight land before the CTA retires (bounded)
       for (int j = issued - 1; j >= 0 && j >= issued - L::STAGES; --j) {
@@ -359,11 +360,11 @@ __global__ void __launch_bounds__(32 * (q8d_warps(NT) + 1), 1)
     // ---- products and softmax
     const int g = lane >> 2, t = lane & 3;
     const int part = warp & 3;   // 16 keys of the unit
-    const int turn = warp >> 2;  // which of WARPS / 4 units
+    const int turn = warp >> 2;  // which of two units
     constexpr int KS = D / 16;   // steps of the first product, row tiles of the second
     float* merge = reinterpret_cast<float*>(smem + L::MERGE_OFF);
     float* ml = reinterpret_cast<float*>(smem + L::ML_OFF);
-    int used = 0, mine = 0;  // units so far, and of WARPS / 4 the one that is next
+    int used = 0;
     int piece = 0;
     bool ok = true;
     while (left > 0) {
@@ -433,9 +434,7 @@ __global__ void __launch_bounds__(32 * (q8d_warps(NT) + 1), 1)
         }
       }
       for (int u = 0; u < n; ++u, ++used) {
-        const bool take = mine == turn;
-        mine = mine + 1 == WARPS / 4 ? 0 : mine + 1;
-        if (!take) continue;
+        if ((used & 1) != turn) continue;
         const int stage = used % L::STAGES;
         ok = ok && __all_sync(0xffffffffu,
                               mbar_wait(&full[stage], (used / L::STAGES) & 1, abort_flag));
@@ -572,20 +571,20 @@ __global__ void __launch_bounds__(32 * (q8d_warps(NT) + 1), 1)
           for (int i = 0; i < KS; ++i)
             *reinterpret_cast<float2*>(dst + 2 * i) = make_float2(o[j][i][e], o[j][i][2 + e]);
         }
-      asm volatile("bar.sync 1, %0;" ::"n"(32 * WARPS) : "memory");
+      asm volatile("bar.sync 1, %0;" ::"n"(32 * Q8D_WARPS) : "memory");
       const int slot = 2 * static_cast<int>(blockIdx.x) + (piece > 0 ? 1 : 0);
-      for (int e = threadIdx.x; e < 8 * NT * (D / 4); e += 32 * WARPS) {
+      for (int e = threadIdx.x; e < 8 * NT * (D / 4); e += 32 * Q8D_WARPS) {
         const int r = e / (D / 4), c = (e % (D / 4)) * 4;
         const int tok = tok0 + r / a.group;
         if (r >= a.tile_tokens * a.group || tok >= w.count) continue;
         float top = -INFINITY;
 #pragma unroll
-        for (int k = 0; k < WARPS; ++k) top = fmaxf(top, ml[(k * 8 * NT + r) * 2]);
+        for (int k = 0; k < Q8D_WARPS; ++k) top = fmaxf(top, ml[(k * 8 * NT + r) * 2]);
         const float ref = top > -INFINITY ? top : 0.0f;
         float sum = 0.0f;
         float4 y = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
 #pragma unroll
-        for (int k = 0; k < WARPS; ++k) {
+        for (int k = 0; k < Q8D_WARPS; ++k) {
           const float wt = ex2_approx(ml[(k * 8 * NT + r) * 2] - ref);
           sum += wt * ml[(k * 8 * NT + r) * 2 + 1];
           const float4 x = *reinterpret_cast<const float4*>(merge + (k * 8 * NT + r) * L::LDO + c);
@@ -608,7 +607,7 @@ __global__ void __launch_bounds__(32 * (q8d_warps(NT) + 1), 1)
           }
         }
       }
-      asm volatile("bar.sync 1, %0;" ::"n"(32 * WARPS) : "memory");
+      asm volatile("bar.sync 1, %0;" ::"n"(32 * Q8D_WARPS) : "memory");
       left -= n;
       at = 0;
       ++piece;
