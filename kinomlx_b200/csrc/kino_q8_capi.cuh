@@ -41,10 +41,10 @@ kino_status q8_smem(int bytes) {
 
 template <int FMT>
 void launch_q8_rows(const kino::Q8RowArgs& a, int64_t rows, cudaStream_t stream) {
-  // two 16-byte vectors a thread up to 512 threads: enough loads in flight with several rows on
-  // an SM; wider rows take four
-  const int nvec = a.dim / 8;
-  int threads = ((nvec + 1) / 2 + 31) / 32 * 32;
+  // Four 16-byte vectors a thread where there are rows enough for many CTAs on an SM (9216 x 4096:
+  // 48.0 us, 52.8 with two, 80.5 with one), two for few rows, whose latency counts.
+  const int nvec = a.dim / 8, each = rows >= 8 * device_sms() ? 4 : 2;
+  int threads = ((nvec + each - 1) / each + 31) / 32 * 32;
   if (threads > kino::Q8_ROW_MAX_THREADS) threads = kino::Q8_ROW_MAX_THREADS;
   const int nv = (nvec + threads - 1) / threads;
   auto run = [&](auto kernel) {
@@ -56,23 +56,25 @@ void launch_q8_rows(const kino::Q8RowArgs& a, int64_t rows, cudaStream_t stream)
     run(kino::q8_rows_kernel<FMT, 4>);
 }
 
+int log2_block(int64_t block) { return block == 16 ? 4 : block == 32 ? 5 : block == 64 ? 6 : 7; }
+
 template <int FMT>
 void launch_q8_write(const kino::Q8WriteArgs& a, int64_t items, cudaStream_t stream) {
-  const dim3 grid(static_cast<unsigned>(items), static_cast<unsigned>(a.heads), 2);
-  auto run = [&](auto kernel) {
-    launch_pdl(kernel, grid, dim3(kino::Q8_WRITE_THREADS), 0, stream, a);
+  auto run = [&](auto kernel, unsigned parts) {
+    launch_pdl(kernel, dim3(static_cast<unsigned>(items * a.heads), parts),
+               dim3(kino::Q8_WRITE_THREADS), 0, stream, a);
   };
   switch (a.block * a.dim / 1024) {
     case 1:
-      return run(kino::q8_cache_write_kernel<FMT, 1>);
+      return run(kino::q8_cache_write_kernel<FMT, 1, 2>, 1);
     case 2:
-      return run(kino::q8_cache_write_kernel<FMT, 2>);
+      return run(kino::q8_cache_write_kernel<FMT, 2, 2>, 1);
     case 4:
-      return run(kino::q8_cache_write_kernel<FMT, 4>);
+      return run(kino::q8_cache_write_kernel<FMT, 4, 2>, 1);
     case 8:
-      return run(kino::q8_cache_write_kernel<FMT, 8>);
+      return run(kino::q8_cache_write_kernel<FMT, 8, 2>, 1);
     default:
-      return run(kino::q8_cache_write_kernel<FMT, 16>);
+      return run(kino::q8_cache_write_kernel<FMT, 16, 1>, 2);
   }
 }
 
@@ -275,15 +277,34 @@ kino_status kino_q8_linear(const void* x, int64_t ldx, const float* x_scales, co
                              static_cast<uint64_t>(ldw), 128, 128);
   if (st != KINO_OK) return st;
   const cudaStream_t s = static_cast<cudaStream_t>(stream);
+  // Which form (device times at k = 4096 unless said, one SM count of 148):
+  //  - the wide form with the least token tile that needs no more CTAs than fit at once (two on an
+  //    SM, not quite filled): many small tiles read the weight from L2 again but finish sooner
+  //    than few large ones (126 x 8192, k 2048: 8.6 us with 32 tokens a tile, 14.0 with 128;
+  //    512 x 4096: 14.9 with 64, 17.6 in pairs); K cut only up to one CTA an SM (1 x 4096: 9.9
+  //    whole, 7.0 cut by four; 64 x 4096 with 32 tokens: 9.0 cut by two, 9.2 by four);
+  //  - CTA pairs once 256 x 256 tiles occupy two thirds of them (1024 x 4096: 18.3 us, wide 20.1;
+  //    256 x 16384: 21.1, wide 21.9; 512 x 4096, 32 tiles on 74 pairs: 17.6, wide 14.9);
+  //  - neither (few tokens, a very wide weight): one token tile, the weight read once.
   const int64_t sms = device_sms();
-  if (m > 256) {
+  const int64_t tiles_n = (n + 127) / 128;
+  const int64_t pair_tiles = ((m + 255) / 256) * ((n + 255) / 256);
+  int nt = 0;
+  if (m <= 128 || 3 * pair_tiles < sms)
+    for (nt = 16; nt <= 128; nt *= 2)
+      if (4 * tiles_n * ((m + nt - 1) / nt) <= 7 * sms) break;
+  if (nt > 128 && m <= 128)
+    for (nt = 16; nt < m; nt *= 2) {
+    }
+  if (nt == 0 || nt > 128) {
     CUtensorMap mx;
     st = make_map8(&mx, x, static_cast<uint64_t>(k), static_cast<uint64_t>(m),
                    static_cast<uint64_t>(ldx), 128, 128);
     if (st != KINO_OK) return st;
     a.tiles_m = static_cast<int>((m + 255) / 256);
     a.tiles_n = static_cast<int>((n + 255) / 256);
-    a.num_tiles = a.tiles_m * a.tiles_n;
+    if (pair_tiles > 0x3fffffffLL) return fail(KINO_ENOTSUPPORTED, "kino_q8_linear: shape too large");
+    a.num_tiles = static_cast<int>(pair_tiles);
     using L = kino::Gemm2SmSmem<kino::Q8G_STAGES>;
     constexpr auto kernel = kino::q8_gemm_pair_kernel;
     st = q8_smem<kernel>(L::TOTAL);
@@ -292,11 +313,9 @@ kino_status kino_q8_linear(const void* x, int64_t ldx, const float* x_scales, co
     launch_ex(kernel, dim3(2 * pairs), dim3(kino::GEMM_THREADS), L::TOTAL, s, 2, mx, mw, a);
     return check_launch("kino_q8_linear");
   }
-  // token tile: the least that holds the tokens; K cut until the tiles fill the GPU
-  const int nt = m <= 16 ? 16 : m <= 32 ? 32 : m <= 64 ? 64 : m <= 128 ? 128 : 256;
-  const int64_t tiles = (n + 127) / 128;
+  const int64_t tiles = tiles_n * ((m + nt - 1) / nt);
   int splits = 1;
-  while (splits < 8 && tiles * splits * 2 <= 2 * sms && a.kblocks >= 4 * splits) splits *= 2;
+  while (splits < 8 && tiles * splits * 2 <= sms && a.kblocks >= 8 * splits) splits *= 2;
   switch (nt) {
     case 16:
       return launch_q8_wide<16>(mw, x, ldx, k, a, splits, s);
@@ -304,10 +323,8 @@ kino_status kino_q8_linear(const void* x, int64_t ldx, const float* x_scales, co
       return launch_q8_wide<32>(mw, x, ldx, k, a, splits, s);
     case 64:
       return launch_q8_wide<64>(mw, x, ldx, k, a, splits, s);
-    case 128:
-      return launch_q8_wide<128>(mw, x, ldx, k, a, splits, s);
     default:
-      return launch_q8_wide<256>(mw, x, ldx, k, a, splits, s);
+      return launch_q8_wide<128>(mw, x, ldx, k, a, splits, s);
   }
 }
 
@@ -347,12 +364,14 @@ kino_status kino_q8_cache_write(const kino_q8_cache* cache, const void* k, int64
   a.dim = static_cast<int>(cache->dim);
   a.block = static_cast<int>(cache->block);
   a.num_blocks = static_cast<int>(cache->num_blocks);
+  a.block_shift = log2_block(cache->block);
   // n tokens fall into at most (n - 1) / block + 2 blocks (n >= 1)
   const int64_t block = cache->block, batch = cache->batch;
   const int64_t items = token_starts == nullptr
                             ? batch * ((rows / batch + block - 2) / block + 1)
                             : rows / block + 2 * std::min(batch, rows);
-  if (items > 0x7fffffffLL) return fail(KINO_ENOTSUPPORTED, "kino_q8_cache_write: too many blocks");
+  if (items * cache->heads > 0x7fffffffLL)
+    return fail(KINO_ENOTSUPPORTED, "kino_q8_cache_write: too many blocks");
   if (cache->format == KINO_Q8_INT8)
     launch_q8_write<kino::Q8_INT8>(a, items, static_cast<cudaStream_t>(stream));
   else
@@ -384,8 +403,9 @@ kino_status kino_q8_cache_read(const kino_q8_cache* cache, void* k_out, void* v_
   a.dim = static_cast<int>(cache->dim);
   a.block = static_cast<int>(cache->block);
   a.num_blocks = static_cast<int>(cache->num_blocks);
+  a.block_shift = log2_block(cache->block);
   const int64_t per_token = cache->heads * (cache->dim / 16);
-  if (tokens > (0x7fffffffLL * 256) / per_token)
+  if (tokens > (0x7fffffffLL - 256) / per_token)
     return fail(KINO_ENOTSUPPORTED, "kino_q8_cache_read: shape too large");
   const dim3 grid(static_cast<unsigned>((tokens * per_token + 255) / 256),
                   static_cast<unsigned>(cache->batch));
@@ -443,7 +463,7 @@ kino_status kino_q8_attention(const kino_q8_cache* cache, const kino_q8_attentio
   a.group = static_cast<int>(args->q_heads / cache->heads);
   a.block = static_cast<int>(cache->block);
   a.num_blocks = static_cast<int>(cache->num_blocks);
-  a.block_shift = a.block == 16 ? 4 : a.block == 32 ? 5 : a.block == 64 ? 6 : 7;
+  a.block_shift = log2_block(cache->block);
   a.scale_log2 = args->scale * 1.4426950408889634f;
   a.causal = args->causal != 0;
   a.tile_tokens = p.tile_tokens;

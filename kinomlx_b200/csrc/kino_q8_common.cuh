@@ -54,20 +54,17 @@ __device__ __forceinline__ Q8Factor q8_quotient(float a, float b) {
 
 __device__ __forceinline__ uint32_t abs_bits(float x) { return __float_as_uint(x) & 0x7FFFFFFFu; }
 
-// Four codes, lowest byte first, of already scaled values. A NaN becomes 0 in both formats: int8
-// through the conversion to integer, e4m3 by the comparison.
+// Four codes, lowest byte first, of quotients within the code range (a group with scale 0 or NaN
+// gets zeros from the caller). int8: 1.5 * 2^23 + x has the integer nearest to x, ties to even, in
+// its low bits, two's complement (a conversion to integer runs at a quarter of an addition's rate).
 template <int FMT>
 __device__ __forceinline__ uint32_t q8_encode4(float a, float b, float c, float d) {
   if constexpr (FMT == Q8_INT8) {
-    // the low bytes of four integers that are within [-127, 127] after the clamp
-    const int ia = max(-127, min(127, __float2int_rn(a))), ib = max(-127, min(127, __float2int_rn(b)));
-    const int ic = max(-127, min(127, __float2int_rn(c))), id = max(-127, min(127, __float2int_rn(d)));
+    constexpr float kShift = 12582912.0f;
+    const uint32_t ia = __float_as_uint(a + kShift), ib = __float_as_uint(b + kShift);
+    const uint32_t ic = __float_as_uint(c + kShift), id = __float_as_uint(d + kShift);
     return __byte_perm(__byte_perm(ia, ib, 0x0040), __byte_perm(ic, id, 0x0040), 0x5410);
   } else {
-    a = a == a ? a : 0.0f;
-    b = b == b ? b : 0.0f;
-    c = c == c ? c : 0.0f;
-    d = d == d ? d : 0.0f;
     const uint32_t lo = __nv_cvt_float2_to_fp8x2(make_float2(a, b), __NV_SATFINITE, __NV_E4M3);
     const uint32_t hi = __nv_cvt_float2_to_fp8x2(make_float2(c, d), __NV_SATFINITE, __NV_E4M3);
     return lo | (hi << 16);

@@ -264,8 +264,8 @@ struct Q8WideSmem {
   static constexpr int A_BYTES = 128 * Q8G_BK;  // weight rows
   static constexpr int B_BYTES = NT * Q8G_BK;   // token rows
   static constexpr int STAGE_BYTES = A_BYTES + B_BYTES;
-  // about 100 KB of loads in flight with room for two CTAs on an SM; 144 KB with 256 tokens
-  static constexpr int STAGES = NT <= 32 ? 5 : NT <= 64 ? 4 : NT <= 128 ? 3 : 4;
+  // about 100 KB of loads in flight, and room for two CTAs on an SM
+  static constexpr int STAGES = NT <= 32 ? 5 : NT <= 64 ? 4 : 3;
   static constexpr int PARTIAL_BYTES = NT * 128 * 4;
   static constexpr int TILE_BYTES =
       STAGES * STAGE_BYTES > PARTIAL_BYTES ? STAGES * STAGE_BYTES : PARTIAL_BYTES;

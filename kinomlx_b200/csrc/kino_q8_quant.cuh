@@ -121,10 +121,12 @@ __global__ void __launch_bounds__(Q8_ROW_MAX_THREADS) q8_rows_kernel(const Q8Row
   for (int i = 0; i < NV; ++i) {
     const int c = threadIdx.x + i * blockDim.x;
     if (c < nvec)
-      cr[c] = make_uint2(q8_encode4<FMT>(f.times(v[i][0]), f.times(v[i][1]), f.times(v[i][2]),
-                                         f.times(v[i][3])),
-                         q8_encode4<FMT>(f.times(v[i][4]), f.times(v[i][5]), f.times(v[i][6]),
-                                         f.times(v[i][7])));
+      cr[c] = !(scale > 0.0f)
+                  ? make_uint2(0u, 0u)
+                  : make_uint2(q8_encode4<FMT>(f.times(v[i][0]), f.times(v[i][1]),
+                                               f.times(v[i][2]), f.times(v[i][3])),
+                               q8_encode4<FMT>(f.times(v[i][4]), f.times(v[i][5]),
+                                               f.times(v[i][6]), f.times(v[i][7])));
   }
 }
 
@@ -132,8 +134,10 @@ __global__ void __launch_bounds__(Q8_ROW_MAX_THREADS) q8_rows_kernel(const Q8Row
 // Codes live as (block, head, slot, dim): the tokens of one block and head are contiguous, which
 // is the unit every kernel here reads. Sequence b's new tokens take positions lengths[b] on.
 //
-// One CTA per (cache block that gets new tokens, head, K or V). The new tokens' values stay in
-// registers between the maximum and the rounding. A block that holds earlier tokens keeps the
+// One CTA per (cache block that gets new tokens, head), K and V together (blocks of 128 tokens of
+// 128-wide heads: one of them). The new tokens' values stay in registers between the maximum and
+// the rounding. Finding the block takes two dependent reads before the first value is asked for,
+// which K and V share; several heads in turn in a CTA were slower (fewer loads in flight). A block that holds earlier tokens keeps the
 // larger of its scale and the new tokens': where it grows, the earlier codes are rounded again to
 // the new scale (at most a half step of the new scale each time).
 constexpr int Q8_WRITE_THREADS = 128;
@@ -149,6 +153,7 @@ struct Q8WriteArgs {
   const int32_t* lengths;  // tokens held before this call
   Q8Rows rows;
   int batch, heads, dim, block, num_blocks;
+  int block_shift;  // log2(block)
 };
 
 // The item-th cache block that gets new tokens, in order of sequences; false past the last one.
@@ -165,7 +170,10 @@ __device__ __forceinline__ bool q8_write_item(const Q8WriteArgs& a, int item, in
       a.rows.of(mine, f, c);
       const int len = a.lengths[mine];
       if (len < 0) q8_flag(1);
-      if (c > 0 && len >= 0) n = static_cast<int>((static_cast<int64_t>(len) + c - 1) / a.block - len / a.block + 1);
+      if (c > 0 && len >= 0) {
+        const int last = static_cast<int>((static_cast<int64_t>(len) + c - 1) >> a.block_shift);
+        n = last - (len >> a.block_shift) + 1;
+      }
     }
     int upto = n;
 #pragma unroll
@@ -180,7 +188,7 @@ __device__ __forceinline__ bool q8_write_item(const Q8WriteArgs& a, int item, in
       const int skipped = before + __shfl_sync(0xffffffffu, upto - n, l);
       held = a.lengths[b];
       a.rows.of(b, first, count);
-      index = held / a.block + (item - skipped);
+      index = (held >> a.block_shift) + (item - skipped);
       return true;
     }
     before += __shfl_sync(0xffffffffu, upto, 31);
@@ -188,90 +196,105 @@ __device__ __forceinline__ bool q8_write_item(const Q8WriteArgs& a, int item, in
   return false;
 }
 
-template <int FMT, int NV>
+template <int FMT, int NV, int KV>
 __global__ void __launch_bounds__(Q8_WRITE_THREADS) q8_cache_write_kernel(const Q8WriteArgs a) {
   griddep_wait();
   griddep_launch();
-  __shared__ uint32_t s_max[Q8_WRITE_THREADS / 32];
+  __shared__ uint32_t s_max[KV][Q8_WRITE_THREADS / 32];
   int b, index, held, count;
   int64_t first;
-  if (!q8_write_item(a, blockIdx.x, b, index, held, first, count)) return;
+  // (heads are neighbours in the grid as they are in a token's row)
+  const int head = blockIdx.x % a.heads, kv0 = KV == 2 ? 0 : blockIdx.y;
+  if (!q8_write_item(a, blockIdx.x / a.heads, b, index, held, first, count)) return;
   const int page = index < a.table_blocks ? a.table[b * a.ld_table + index] : -1;
   if (page < 0 || page >= a.num_blocks) {  // past the table, or no block of this cache
     if (threadIdx.x == 0) q8_flag(1);
     return;
   }
-  const int head = blockIdx.y, kv = blockIdx.z;
   const int64_t unit = static_cast<int64_t>(page) * a.heads + head;
-  uint8_t* codes = a.codes[kv] + unit * a.block * a.dim;
-  const int chunks = a.dim >> 3;  // 8-value chunks of a token: 8 or 16
-  const int64_t at0 = static_cast<int64_t>(index) * a.block;  // position of slot 0
-  const __nv_bfloat16* src = a.x[kv] + head * a.head_stride[kv];
-  uint4 raw[NV];
-  bool fresh[NV];
-  uint32_t top = 0;
-#pragma unroll
-  for (int i = 0; i < NV; ++i) {
-    const int e = threadIdx.x + i * Q8_WRITE_THREADS;
-    const int slot = e / chunks, c = e % chunks;
-    const int64_t t = at0 + slot - held;
-    fresh[i] = t >= 0 && t < count;
-    raw[i] = make_uint4(0, 0, 0, 0);
-    if (fresh[i]) raw[i] = __ldcs(reinterpret_cast<const uint4*>(src + (first + t) * a.ld[kv]) + c);
-  }
-#pragma unroll
-  for (int i = 0; i < NV; ++i) {
-    const uint32_t w[4] = {raw[i].x, raw[i].y, raw[i].z, raw[i].w};
-#pragma unroll
-    for (int j = 0; j < 4; ++j)
-      top = max(top, max((w[j] & 0x7FFFu) << 16, w[j] & 0x7FFF0000u));
-  }
-  top = __reduce_max_sync(0xffffffffu, top);
-  if ((threadIdx.x & 31) == 0) s_max[threadIdx.x >> 5] = top;
+  const int chunk_bits = a.dim == 128 ? 4 : 3;  // 8-value chunks of a token: 8 or 16
+  const int64_t at0 = static_cast<int64_t>(index) << a.block_shift;  // position of slot 0
   const bool earlier = held > at0;
-  const float before = earlier ? a.scales[kv][unit] : 0.0f;
-  __syncthreads();  // every thread has read the old scale
+  // slots [fresh0, fresh1) get new tokens, those before fresh0 hold earlier ones
+  const int fresh0 = earlier ? static_cast<int>(held - at0) : 0;
+  const int fresh1 = static_cast<int>(min(static_cast<int64_t>(a.block), held + static_cast<int64_t>(count) - at0));
+  const int64_t row0 = first + at0 - held;  // of slot 0
+  uint4 raw[KV][NV];
 #pragma unroll
-  for (int i = 0; i < Q8_WRITE_THREADS / 32; ++i) top = max(top, s_max[i]);
-  const float own = q8_scale<FMT>(top);
-  // the larger of the two; NaN wins
-  const float scale = before > own ? before : before == before ? own : before;
-  Q8Factor f = {0.0f, 0.0f}, again = {0.0f, 0.0f};
-  if (scale > 0.0f) {
-    if (scale > before) {  // the new tokens' own
-      f = q8_quotient(q8_top<FMT>(), __uint_as_float(top));
-      again.hi = before * f.hi;  // what the earlier codes are multiplied by
-      again.lo = fmaf(before, f.hi, -again.hi) + before * f.lo;
-    } else {
-      f = q8_quotient(1.0f, before);
+  for (int kv = 0; kv < KV; ++kv) {
+    const __nv_bfloat16* src = a.x[kv0 + kv] + head * a.head_stride[kv0 + kv];
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+      const int e = threadIdx.x + i * Q8_WRITE_THREADS;
+      const int slot = e >> chunk_bits, c = e & ((1 << chunk_bits) - 1);
+      raw[kv][i] = make_uint4(0, 0, 0, 0);
+      if (slot >= fresh0 && slot < fresh1)
+        raw[kv][i] = __ldcs(reinterpret_cast<const uint4*>(src + (row0 + slot) * a.ld[kv0 + kv]) + c);
     }
   }
-  if (threadIdx.x == 0) a.scales[kv][unit] = scale;
-  const bool grown = earlier && scale > before;
+  float before[KV];
 #pragma unroll
-  for (int i = 0; i < NV; ++i) {
-    const int e = threadIdx.x + i * Q8_WRITE_THREADS;
-    uint2* dst = reinterpret_cast<uint2*>(codes) + e;
-    float v[8];
-    if (fresh[i]) {
-      q8_unpack8(raw[i], v);
+  for (int kv = 0; kv < KV; ++kv) {
+    before[kv] = earlier ? a.scales[kv0 + kv][unit] : 0.0f;
+    uint32_t top = 0;
 #pragma unroll
-      for (int j = 0; j < 8; ++j) v[j] = f.times(v[j]);
-    } else if (grown && at0 + e / chunks < held) {
-      const uint2 old = *dst;
-      float lo[4], hi[4];
-      q8_decode4<FMT>(old.x, lo);
-      q8_decode4<FMT>(old.y, hi);
+    for (int i = 0; i < NV; ++i) {
+      const uint32_t w[4] = {raw[kv][i].x, raw[kv][i].y, raw[kv][i].z, raw[kv][i].w};
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        v[j] = again.times(lo[j]);
-        v[4 + j] = again.times(hi[j]);
-      }
-    } else {
-      continue;
+      for (int j = 0; j < 4; ++j)
+        top = max(top, max((w[j] & 0x7FFFu) << 16, w[j] & 0x7FFF0000u));
     }
-    *dst = make_uint2(q8_encode4<FMT>(v[0], v[1], v[2], v[3]),
-                      q8_encode4<FMT>(v[4], v[5], v[6], v[7]));
+    top = __reduce_max_sync(0xffffffffu, top);
+    if ((threadIdx.x & 31) == 0) s_max[kv][threadIdx.x >> 5] = top;
+  }
+  __syncthreads();  // (every thread has read the old scales too)
+#pragma unroll
+  for (int kv = 0; kv < KV; ++kv) {
+    uint32_t top = 0;
+#pragma unroll
+    for (int i = 0; i < Q8_WRITE_THREADS / 32; ++i) top = max(top, s_max[kv][i]);
+    const float own = q8_scale<FMT>(top), old_scale = before[kv];
+    // the larger of the two; NaN wins
+    const float scale = old_scale > own ? old_scale : old_scale == old_scale ? own : old_scale;
+    Q8Factor f = {0.0f, 0.0f}, again = {0.0f, 0.0f};
+    if (scale > 0.0f) {
+      if (scale > old_scale) {  // the new tokens' own
+        f = q8_quotient(q8_top<FMT>(), __uint_as_float(top));
+        again.hi = old_scale * f.hi;  // what the earlier codes are multiplied by
+        again.lo = fmaf(old_scale, f.hi, -again.hi) + old_scale * f.lo;
+      } else {
+        f = q8_quotient(1.0f, old_scale);
+      }
+    }
+    if (threadIdx.x == 0) a.scales[kv0 + kv][unit] = scale;
+    const bool grown = scale > old_scale;
+    uint2* codes = reinterpret_cast<uint2*>(a.codes[kv0 + kv] + unit * a.block * a.dim);
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+      const int e = threadIdx.x + i * Q8_WRITE_THREADS;
+      const int slot = e >> chunk_bits;
+      float v[8];
+      if (slot >= fresh0 && slot < fresh1) {
+        q8_unpack8(raw[kv][i], v);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) v[j] = f.times(v[j]);
+      } else if (grown && slot < fresh0) {
+        const uint2 old = codes[e];
+        float lo[4], hi[4];
+        q8_decode4<FMT>(old.x, lo);
+        q8_decode4<FMT>(old.y, hi);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          v[j] = again.times(lo[j]);
+          v[4 + j] = again.times(hi[j]);
+        }
+      } else {
+        continue;
+      }
+      codes[e] = !(scale > 0.0f) ? make_uint2(0u, 0u)
+                                 : make_uint2(q8_encode4<FMT>(v[0], v[1], v[2], v[3]),
+                                              q8_encode4<FMT>(v[4], v[5], v[6], v[7]));
+    }
   }
 }
 
@@ -290,6 +313,7 @@ struct Q8ReadArgs {
   const int32_t* lengths;
   int64_t tokens;
   int heads, dim, block, num_blocks;
+  int block_shift;  // log2(block)
 };
 
 template <int FMT>
@@ -297,20 +321,21 @@ __global__ void __launch_bounds__(256) q8_cache_read_kernel(const Q8ReadArgs a) 
   griddep_wait();
   griddep_launch();
   const int b = blockIdx.y;
-  const int chunks = a.dim >> 4;
-  const int64_t per_token = static_cast<int64_t>(a.heads) * chunks;
-  const int64_t total = a.tokens * per_token;
-  const int64_t e = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x;
-  if (e >= total) return;
-  const int64_t t = e / per_token;
-  const int rest = static_cast<int>(e - t * per_token);
-  const int head = rest / chunks, c = rest % chunks;
+  // (tokens * heads * dim / 16 fits 31 bits: 64-bit divisions would cost more than the copy)
+  const int chunk_bits = a.dim == 128 ? 3 : 2;
+  const uint32_t e = blockIdx.x * 256u + threadIdx.x;
+  const uint32_t per_token = static_cast<uint32_t>(a.heads) << chunk_bits;
+  const uint32_t token = e / per_token;
+  if (token >= a.tokens) return;
+  const int64_t t = token;
+  const int rest = static_cast<int>(e - token * per_token);
+  const int head = rest >> chunk_bits, c = rest & ((1 << chunk_bits) - 1);
   const int64_t capacity = static_cast<int64_t>(a.table_blocks) * a.block;
   const int64_t length = a.lengths[b];
   if (length < 0 || length > capacity) q8_flag(1);
   int page = -1;
   if (t < length && t < capacity) {
-    page = a.table[b * a.ld_table + t / a.block];
+    page = a.table[b * a.ld_table + (t >> a.block_shift)];
     if (page < 0 || page >= a.num_blocks) {
       q8_flag(1);
       page = -1;
@@ -321,7 +346,7 @@ __global__ void __launch_bounds__(256) q8_cache_read_kernel(const Q8ReadArgs a) 
   float scale[2] = {0.0f, 0.0f};
   if (page >= 0) {
     const int64_t unit = static_cast<int64_t>(page) * a.heads + head;
-    const int64_t src = (unit * a.block + t % a.block) * a.dim + c * 16;
+    const int64_t src = (unit * a.block + (t & (a.block - 1))) * a.dim + c * 16;
 #pragma unroll
     for (int kv = 0; kv < 2; ++kv) {
       raw[kv] = __ldcs(reinterpret_cast<const uint4*>(a.codes[kv] + src));

@@ -127,6 +127,7 @@ def _check_product(out, exact, bias):
     (1, 8, 16), (1, 4096, 4096), (2, 136, 128), (7, 1000, 272), (16, 640, 2064), (17, 384, 1040),
     (33, 256, 512), (64, 128, 144), (65, 264, 384), (126, 520, 1024), (129, 128, 256),
     (256, 512, 768), (257, 256, 128), (300, 1000, 400), (513, 264, 2048), (1025, 768, 640),
+    (100, 33800, 64), (300, 6400, 144), (1025, 2600, 640),
 ])
 @pytest.mark.parametrize("bias", [False, True])
 def test_linear_int8(cuda_device, m, n, k, bias):
