@@ -344,3 +344,324 @@ def test_attention_many_rows(cuda_device, case, dtype, dim, block, causal):
     held, new, heads, group = case
     _check_attention(*_attend(cuda_device, held, new, heads, group, dim, block, dtype,
                               causal=causal, seed=dim + block))
+
+
+# ---------------------------------------------------------------- edges of attention
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize(("held", "new", "group"), [([90, 200, 33], [1, 1, 1], 4), ([300, 140], [40, 90], 4)])
+def test_attention_scales_of_any_size(cuda_device, dtype, held, new, group):
+    # V scales that differ by factors of 1000 between blocks, either way
+    got = _attend(cuda_device, held, new, 2, group, 128, 16, dtype, spread=1000.0, seed=3)
+    _check_attention(*got)
+    # scale and no mask
+    _check_attention(*_attend(cuda_device, held, new, 2, group, 64, 32, dtype, causal=False, scale=0.3))
+    # a scale of 0 averages the keys
+    _check_attention(*_attend(cuda_device, held, new, 2, group, 128, 64, dtype, scale=0.0))
+
+
+@pytest.mark.parametrize("rows", [1, 40])
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_attention_not_finite_in_masked_places(cuda_device, dtype, rows):
+    """Blocks that no query sees, the rest of the last block and keys behind a causal mask hold NaN
+    scales and every code pattern; rows that do not see them are as without them."""
+    heads, group, dim, block, held = 2, 2, 128, 16, 16 * 7 + 5
+    cpu, cache, table = _cache(1, 16 * 9, heads, dim, block, dtype, 5, cuda_device)
+    q = _normal((rows, heads * group, dim), 6)
+    lengths = torch.tensor([held], dtype=torch.int32)
+    for t in (cpu, cache):
+        unseen = table[0, 8:].long().to(t.k_codes.device)
+        for x in t[2:]:
+            x[unseen] = math.nan
+        last = int(table[0, 7])
+        for x in t[:2]:
+            x.view(torch.uint8)[last, :, 5:] = 0x7F  # past the length: NaN patterns in e4m3
+    args = (table.to(cuda_device), lengths.to(cuda_device))
+    got = ops_q8.kv_cache_attention(q.to(cuda_device), cache, *args)
+    _check_attention(got.cpu(), *ref.attention(q, *cpu, table, lengths))
+    # a NaN block in sight spoils the rows that see it and no other
+    bad = int(table[0, 6])  # keys 96 .. 111
+    cache.v_scales[bad, 1] = math.nan
+    spoiled = ops_q8.kv_cache_attention(q.to(cuda_device), cache, *args).cpu()
+    for i in range(rows):
+        sees = held - rows + i >= 96
+        assert torch.equal(spoiled[i, :group], got[i, :group].cpu())
+        assert bool(spoiled[i, group:].isnan().all()) == sees
+        if not sees:
+            assert torch.equal(spoiled[i, group:], got[i, group:].cpu())
+
+
+@pytest.mark.parametrize("rows", [1, 50])
+def test_attention_zero_values_and_empty(cuda_device, rows):
+    cpu, cache, table = _cache(3, 200, 2, 128, 64, INT8, 8, cuda_device)
+    for t in (cpu, cache):
+        first = table[0].long().to(t.k_codes.device)
+        t.v_codes[first] = 0
+        t.v_scales[first] = 0.0
+    lengths = torch.tensor([200, 0, 130], dtype=torch.int32)
+    q = _normal((3 * rows, 2, 128), 9)
+    got = ops_q8.kv_cache_attention(q.to(cuda_device), cache, table.to(cuda_device),
+                                    lengths.to(cuda_device))
+    assert not got[: 2 * rows].any()
+    _check_attention(got.cpu(), *ref.attention(q, *cpu, table, lengths))
+    ops.device_status()
+
+
+@pytest.mark.parametrize("rows", [1, 30])
+def test_attention_strides_and_in_place(cuda_device, rows):
+    cpu, cache, table = _cache(2, 150, 2, 64, 32, E4M3, 12, cuda_device)
+    lengths = torch.tensor([150, 77], dtype=torch.int32)
+    qkv = _normal((2 * rows, 3, 6, 64), 10).to(cuda_device)
+    args = (table.to(cuda_device), lengths.to(cuda_device))
+    want = ops_q8.kv_cache_attention(qkv[:, 1].contiguous(), cache, *args)
+    before = qkv.clone()
+    out = torch.zeros((2 * rows, 6, 3, 64), dtype=BF16, device=cuda_device)
+    got = ops_q8.kv_cache_attention(qkv[:, 1], cache, *args, out=out[:, :, 2])
+    assert torch.equal(got, want) and not out[:, :, :2].any()
+    ops_q8.kv_cache_attention(qkv[:, 1], cache, *args, out=qkv[:, 1])
+    assert torch.equal(qkv[:, 1], want)
+    assert torch.equal(qkv[:, 0], before[:, 0]) and torch.equal(qkv[:, 2], before[:, 2])
+    _check_attention(want.cpu(), *ref.attention(before[:, 1].cpu(), *cpu, table, lengths))
+
+
+@pytest.mark.parametrize(("held", "new"), [([5000], [1]), ([3000, 40], [33, 20])])
+def test_attention_long_and_repeatable(cuda_device, held, new):
+    got = _attend(cuda_device, held, new, 1, 2, 128, 128, INT8, seed=2)
+    _check_attention(*got)
+    again = _attend(cuda_device, held, new, 1, 2, 128, 128, INT8, seed=2)
+    assert torch.equal(got[0], again[0])
+
+
+def test_many_sequences(cuda_device):
+    """More sequences than a warp scans at once, most of them short or empty."""
+    held = [(7 * b) % 90 for b in range(75)]
+    new = [min(h, b % 3) for b, h in enumerate(held)]
+    _check_attention(*_attend(cuda_device, held, new, 1, 2, 64, 16, INT8, packed=True))
+    new = [min(h, (11 * b) % 40) for b, h in enumerate(held)]
+    _check_attention(*_attend(cuda_device, held, new, 1, 4, 64, 16, E4M3, packed=True))
+    cpu, cache, table = _cache(75, 130, 1, 64, 16, INT8, 1, cuda_device)
+    x = _normal((sum(new), 1, 64), 4)
+    starts = torch.tensor([0] + [sum(new[: i + 1]) for i in range(75)], dtype=torch.int32)
+    lengths = torch.tensor(held, dtype=torch.int32)
+    dev = x.to(cuda_device)
+    ops_q8.kv_cache_write(cache, dev, dev, table.to(cuda_device), lengths.to(cuda_device),
+                          starts.to(cuda_device))
+    codes, scales = ref.cache_write(cpu.k_codes, cpu.k_scales, x, table, lengths, starts)
+    assert torch.equal(cache.k_scales.cpu(), scales) and _same(cache.k_codes, codes)
+
+
+# ---------------------------------------------------------------- device-side sizes that do not fit
+@pytest.mark.parametrize("rows", [1, 40])
+def test_sizes_that_do_not_fit_are_skipped_and_reported(cuda_device, rows):
+    cpu, cache, table = _cache(2, 100, 2, 64, 16, INT8, 3, cuda_device)
+    lengths = torch.tensor([100, 60], dtype=torch.int32)
+    q = _normal((2 * rows, 2, 64), 1).to(cuda_device)
+    good = ops_q8.kv_cache_attention(q, cache, table.to(cuda_device), lengths.to(cuda_device))
+    ops.device_status()
+    before = [t.clone() for t in cache]
+
+    def reported():
+        with pytest.raises(RuntimeError, match="EINVAL"):
+            ops.device_status()
+        ops.device_status()  # and forgotten
+
+    for page in (-1, 1 << 20, cache.k_codes.shape[0]):  # a block that the cache does not have
+        bad = table.clone()
+        bad[0, 2] = page
+        got = ops_q8.kv_cache_attention(q, cache, bad.to(cuda_device), lengths.to(cuda_device))
+        assert torch.equal(got[rows:], good[rows:]) and got.isfinite().all()
+        reported()
+        ops_q8.kv_cache_read(cache, bad.to(cuda_device), lengths.to(cuda_device), 100)
+        reported()
+        x = _normal((2 * rows, 2, 64), 2).to(cuda_device)
+        at = torch.tensor([32, 60], dtype=torch.int32, device=cuda_device)
+        ops_q8.kv_cache_write(cache, x, x, bad.to(cuda_device), at)
+        reported()
+        for t, b in zip(cache, before):
+            t.copy_(b)
+    # a skipped block's keys do not count: as if the sequence had a table without it
+    bad = table.clone()
+    bad[0, 6] = -1  # keys 96 .. 99, the last block
+    got = ops_q8.kv_cache_attention(q[:rows], cache, bad[:1].to(cuda_device),
+                                    lengths[:1].to(cuda_device), causal=False)
+    reported()
+    want = ref.attention(q[:rows].cpu(), *cpu, table[:1], torch.tensor([96]), causal=False)
+    _check_attention(got.cpu(), *want)
+    # lengths and starts outside the table and the rows
+    for wrong in ([-1, 60], [100, 2000]):
+        got = ops_q8.kv_cache_attention(q, cache, table.to(cuda_device),
+                                        torch.tensor(wrong, dtype=torch.int32, device=cuda_device))
+        keep = slice(rows, None) if wrong[0] < 0 else slice(0, rows)
+        assert torch.equal(got[keep], good[keep])
+        reported()
+    full = torch.tensor([111, 60], dtype=torch.int32, device=cuda_device)  # 112 slots
+    x = _normal((2 * rows, 2, 64), 2).to(cuda_device)
+    ops_q8.kv_cache_write(cache, x, x, table.to(cuda_device), full)
+    if rows > 1:
+        reported()
+    starts = torch.tensor([0, 2 * rows + 1, 2 * rows], dtype=torch.int32, device=cuda_device)
+    out = torch.full_like(q, 3.0)
+    ops_q8.kv_cache_attention(q, cache, table.to(cuda_device), lengths.to(cuda_device), starts, out=out)
+    assert bool((out == 3).all())
+    reported()
+
+
+# ---------------------------------------------------------------- streams, graphs, the whole run
+def _layer(dtype, seed, device, batch, tokens, held, width=256, heads=2, group=2, dim=64):
+    g = _gen(seed)
+    qkv_width = (heads * group + 2 * heads) * dim
+    w1 = (torch.randn((qkv_width, width), generator=g) / width**0.5).to(BF16)
+    w2 = (torch.randn((width, heads * group * dim), generator=g) / width**0.5).to(BF16)
+    s = dict(x=_normal((batch * tokens, width), seed), residual=_normal((batch * tokens, width), seed + 1),
+             norm=(1 + _normal((width,), seed + 2, 0.1).float()).to(BF16), w1=w1, w2=w2)
+    s = {k: v.to(device) for k, v in s.items()}
+    s["q1"], s["q2"] = ops_q8.quantize_tokens(s["w1"]), ops_q8.quantize_tokens(s["w2"])
+    _, cache, table = _cache(batch, held + tokens, heads, dim, 32, dtype, seed, device)
+    s |= dict(cache=cache, table=table.to(device), heads=heads, group=group, dim=dim,
+              lengths=torch.full((batch,), held, dtype=torch.int32, device=device),
+              after=torch.full((batch,), held + tokens, dtype=torch.int32, device=device))
+    return s
+
+
+def _run_layer(s):
+    """One attention layer in 8 bits: norm, product, cache, attention, quantising, product."""
+    codes, scales, hidden = ops_q8.rms_norm_quantize(s["x"], s["norm"], residual=s["residual"])
+    qkv = ops_q8.linear_int8(codes, scales, *s["q1"])
+    heads, group, dim = s["heads"], s["group"], s["dim"]
+    qkv = qkv.view(qkv.shape[0], -1, dim)
+    q, k, v = qkv.split([heads * group, heads, heads], 1)
+    ops_q8.kv_cache_write(s["cache"], k, v, s["table"], s["lengths"])
+    y = ops_q8.kv_cache_attention(q, s["cache"], s["table"], s["after"])
+    return hidden, ops_q8.linear_int8(*ops_q8.quantize_tokens(y.flatten(1)), *s["q2"])
+
+
+@pytest.mark.parametrize(("tokens", "held"), [(1, 70), (1, 0), (45, 20)])
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_a_layer_follows_its_64_bit_form(cuda_device, dtype, tokens, held):
+    batch = 3
+    s = _layer(dtype, 11, cuda_device, batch, tokens, held)
+    cache0 = [t.cpu().clone() for t in s["cache"]]
+    hidden, out = _run_layer(s)
+    ops.device_status()
+    c = {k: v.cpu() for k, v in s.items() if isinstance(v, torch.Tensor)}
+    h, y = ref.rms_norm(c["x"], c["norm"], 1e-6, c["residual"])
+    assert torch.equal(hidden.cpu(), h)
+    # the same run without any rounding to 8 bits but the cache's earlier tokens
+    heads, group, dim = s["heads"], s["group"], s["dim"]
+    qkv = (y @ c["w1"].double().T).view(batch, tokens, -1, dim)
+    q, k, v = qkv.split([heads * group, heads, heads], 2)
+    att = torch.zeros((batch, tokens, heads * group, dim), dtype=torch.float64)
+    for b in range(batch):
+        old = [ref.cached(cache0[i], cache0[2 + i], c["table"][b], held) for i in range(2)]
+        kk = torch.cat([old[0], k[b].transpose(0, 1)], 1)
+        vv = torch.cat([old[1], v[b].transpose(0, 1)], 1)
+        for i in range(tokens):
+            for hd in range(heads * group):
+                p = torch.softmax(kk[hd // group, : held + i + 1] @ q[b, i, hd] * dim**-0.5, 0)
+                att[b, i, hd] = p @ vv[hd // group, : held + i + 1]
+    want = att.flatten(2).flatten(0, 1) @ c["w2"].double().T
+    # Three roundings to codes on the way (activations twice, the new keys and values) and two of
+    # weights; a normal row's code error is about 0.29 steps of amax / 127, amax 3 to 4 rms: 1% of
+    # the rms each in int8, 3% in e4m3 (2^-4 / sqrt 12 of each value); the sum of five, doubled.
+    limit = 0.08 if dtype == INT8 else 0.12
+    rel = float((out.cpu().double() - want).norm() / want.norm())
+    assert rel < limit, rel
+
+
+def test_streams_and_graphs(cuda_device):
+    s = _layer(INT8, 21, cuda_device, 4, 1, 90)
+    start = [t.clone() for t in s["cache"]]
+    want = [t.clone() for t in _run_layer(s)]
+    kept = [t.clone() for t in s["cache"]]
+    for t, b in zip(s["cache"], start):
+        t.copy_(b)
+    torch.cuda.synchronize()
+    stream = torch.cuda.Stream()
+    with torch.cuda.stream(stream):  # another stream than the default
+        got = _run_layer(s)
+    stream.synchronize()
+    assert all(torch.equal(a, b) for a, b in zip(got, want))
+    graphs = []
+    for _ in range(2):  # two graphs of the same run, replayed in turn
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g, stream=stream):
+            res = _run_layer(s)
+        graphs.append((g, res))
+    for _ in range(3):
+        for g, res in graphs:
+            for t, b in zip(s["cache"], start):
+                t.copy_(b)
+            for r in res:
+                r.fill_(-1)
+            g.replay()
+            torch.cuda.synchronize()
+            assert all(torch.equal(a, b) for a, b in zip(res, want))
+            assert all(torch.equal(a, b) for a, b in zip(s["cache"], kept))
+    # two at once on two streams
+    other = torch.cuda.Stream()
+    t = _layer(INT8, 22, cuda_device, 4, 30, 10)
+    base = [x.clone() for x in t["cache"]]
+    alone = [x.clone() for x in _run_layer(t)]
+    torch.cuda.synchronize()
+    for _ in range(5):
+        for x, b in zip((*s["cache"], *t["cache"]), (*start, *base)):
+            x.copy_(b)
+        torch.cuda.synchronize()
+        with torch.cuda.stream(stream):
+            one = _run_layer(s)
+        with torch.cuda.stream(other):
+            two = _run_layer(t)
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(one, want))
+        assert all(torch.equal(a, b) for a, b in zip(two, alone))
+    ops.device_status()
+
+
+def test_front_end_refusals(cuda_device):
+    x = torch.zeros((4, 64), dtype=BF16, device=cuda_device)
+    codes, scales = ops_q8.quantize_tokens(x)
+    with pytest.raises(ValueError, match="bfloat16"):
+        ops_q8.quantize_tokens(x.float())
+    with pytest.raises(ValueError, match="unit stride"):
+        ops_q8.quantize_tokens(x.t())
+    with pytest.raises(ValueError, match="residual"):
+        ops_q8.rms_norm_quantize(x, residual=x[:2])
+    with pytest.raises(ValueError, match="give one"):
+        ops_q8.rms_norm_quantize(x, hidden=x)
+    with pytest.raises(ValueError, match="weight"):
+        ops_q8.rms_norm_quantize(x, x[0, :32])
+    with pytest.raises(RuntimeError, match="dim"):
+        ops_q8.quantize_tokens(x[:, :60].contiguous())
+    with pytest.raises(ValueError, match="int8"):
+        ops_q8.linear_int8(codes.view(torch.float8_e4m3fn), scales, codes, scales)
+    with pytest.raises(ValueError, match="input width"):
+        ops_q8.linear_int8(codes, scales, codes[:, :32], scales)
+    with pytest.raises(ValueError, match="scales"):
+        ops_q8.linear_int8(codes, scales[:3].contiguous(), codes, scales)
+    with pytest.raises(ValueError, match="out"):
+        ops_q8.linear_int8(codes, scales, codes[:, :], scales, out=x)
+    cache = ops_q8.new_kv_cache(4, 2, 64, block_tokens=16)
+    table = torch.zeros((2, 2), dtype=torch.int32, device=cuda_device)
+    lengths = torch.zeros(2, dtype=torch.int32, device=cuda_device)
+    k = torch.zeros((4, 2, 64), dtype=BF16, device=cuda_device)
+    with pytest.raises(ValueError, match="divide"):
+        ops_q8.kv_cache_write(cache, k[:3], k[:3], table, lengths)
+    with pytest.raises(ValueError, match="int32"):
+        ops_q8.kv_cache_write(cache, k, k, table.long(), lengths)
+    with pytest.raises(ValueError, match="heads"):
+        ops_q8.kv_cache_write(cache, k[:, :, :32], k[:, :, :32], table, lengths)
+    with pytest.raises(ValueError, match="rows"):
+        ops_q8.kv_cache_write(cache, k[:, :1], k[:, :1], table, lengths)
+    with pytest.raises(ValueError, match="token_starts"):
+        ops_q8.kv_cache_attention(k, cache, table, lengths, lengths)
+    with pytest.raises(ValueError, match="query heads"):
+        ops_q8.kv_cache_attention(k[:, :1].repeat(1, 3, 1), cache, table, lengths)
+    with pytest.raises(RuntimeError, match="scale"):
+        ops_q8.kv_cache_attention(k, cache, table, lengths, scale=-1.0)
+    # nothing to do is done
+    assert ops_q8.quantize_tokens(x[:0])[0].shape == (0, 64)
+    assert ops_q8.linear_int8(codes[:0], scales[:0], codes, scales).shape == (0, 4)
+    assert ops_q8.kv_cache_attention(k[:0], cache, table, lengths).shape == (0, 2, 64)
+    ops_q8.kv_cache_write(cache, k[:0], k[:0], table, lengths)
+    assert ops_q8.kv_cache_read(cache, table, lengths, 0)[0].shape == (2, 0, 2, 64)
+    assert not ops_q8.kv_cache_attention(k, cache, table, lengths).any()
+    ops.device_status()
