@@ -42,7 +42,6 @@ struct Q8Attn {
   int causal;
   int tile_tokens;  // query tokens of an item
   int tile_rows;    // rows of its partial results (tile_tokens * group, padded)
-  int least_units;  // units of a run, at least
   int runs;         // CTAs (or CTA pairs)
   float* part_o;    // [2 * runs][tile_rows][D]
   float* part_ml;   // [2 * runs][tile_rows][2]: row maximum (log2 units), row sum
@@ -154,10 +153,9 @@ struct Q8Work {
 
 constexpr float Q8_LEAST_V = 8.0779356694631609e-28f;  // 2^-90
 
-// Units of a run.
+// Units of a run. (Runs of at least two to eight units for short caches were no faster.)
 __device__ __forceinline__ int64_t q8_run_units(const Q8Attn& a, int64_t total) {
-  const int64_t even = (total + a.runs - 1) / a.runs;
-  return even > a.least_units ? even : a.least_units;
+  return (total + a.runs - 1) / a.runs;
 }
 
 // ---------------------------------------------------------------- few query rows
@@ -1296,13 +1294,18 @@ __global__ void __launch_bounds__(Q8P_THREADS, 1)
 // CTA c looks at the border between the runs c and c + 1. Where it is the first border inside an
 // item, it adds that item's pieces: the last piece of run c, then the first piece of each run up
 // to the item's end. (A run's pieces but its first and last are whole items; a piece that is both
-// first and last is in slot 0.) gridDim.y CTAs share the rows.
+// first and last is in slot 0.) gridDim.y CTAs share the rows, D / 4 threads a row. One sequence on
+// one head may be in as many pieces as there are CTAs: then all groups of D / 4 threads of a CTA
+// share a row's pieces (32000 keys on one head: 14 us, 46 with one group a row).
 template <int D, int BN>
 __global__ void __launch_bounds__(256) attention_q8_combine_kernel(const Q8Attn a) {
   // This kernel may start when every CTA of the attention has passed its own wait for what ran
   // before it, so lengths and starts are there and the items can be found while it still runs.
   __shared__ int s_item[4];      // b, tile, head, pieces (0: nothing to do)
   __shared__ int s_slot0;
+  constexpr int LANES = D / 4, GROUPS = 256 / LANES;
+  __shared__ float4 s_y[GROUPS][LANES];
+  __shared__ float2 s_ml[GROUPS];
   Q8Work<BN> w(a);
   if (threadIdx.x < 32) {
     const int64_t total = w.total();
@@ -1333,24 +1336,52 @@ __global__ void __launch_bounds__(256) attention_q8_combine_kernel(const Q8Attn 
   w.enter(s_item[0]);
   const int tok0 = s_item[1] * a.tile_tokens, head = s_item[2];
   const int live = min(a.tile_tokens, w.count - tok0) * a.group;
-  for (int e = blockIdx.y * 256 + threadIdx.x; e < live * (D / 4); e += gridDim.y * 256) {
-    const int r = e / (D / 4), c = (e % (D / 4)) * 4;
-    float top = -INFINITY, sum = 0.0f;
-    float4 y = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-    for (int k = 0; k < pieces; ++k) {
+  const int group = threadIdx.x / LANES, c = threadIdx.x % LANES * 4;
+  const bool share = pieces >= 2 * GROUPS;
+  const int first = share ? group : 0, stride = share ? GROUPS : 1;
+  for (int r = share ? blockIdx.y : blockIdx.y * GROUPS + group; r < live;
+       r += gridDim.y * (share ? 1 : GROUPS)) {
+    auto place = [&](int k) {
       const int slot = k == 0 ? s_slot0 : 2 * (static_cast<int>(blockIdx.x) + k);
-      const int64_t at = static_cast<int64_t>(slot) * a.tile_rows + r;
-      const float pm = a.part_ml[at * 2], pl = a.part_ml[at * 2 + 1];
-      const float4 x = *reinterpret_cast<const float4*>(a.part_o + at * D + c);
-      const float now = fmaxf(top, pm);
-      const float ref = now > -INFINITY ? now : 0.0f;
-      const float wo = ex2_approx(top - ref), wn = ex2_approx(pm - ref);
-      sum = sum * wo + pl * wn;
-      y.x = y.x * wo + x.x * wn;
-      y.y = y.y * wo + x.y * wn;
-      y.z = y.z * wo + x.z * wn;
-      y.w = y.w * wo + x.w * wn;
-      top = now;
+      return static_cast<int64_t>(slot) * a.tile_rows + r;
+    };
+    float top = -INFINITY, sum = 0.0f;
+#pragma unroll 4
+    for (int k = first; k < pieces; k += stride) top = fmaxf(top, a.part_ml[place(k) * 2]);
+    float ref = top > -INFINITY ? top : 0.0f;
+    float4 y = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+    auto add = [&](const float2 ml, const float4 x) {
+      const float wt = ex2_approx(ml.x - ref);
+      sum = fmaf(ml.y, wt, sum);
+      y.x = fmaf(x.x, wt, y.x);
+      y.y = fmaf(x.y, wt, y.y);
+      y.z = fmaf(x.z, wt, y.z);
+      y.w = fmaf(x.w, wt, y.w);
+    };
+#pragma unroll 4
+    for (int k = first; k < pieces; k += stride) {
+      const int64_t at = place(k);
+      add(*reinterpret_cast<const float2*>(a.part_ml + at * 2),
+          *reinterpret_cast<const float4*>(a.part_o + at * D + c));
+    }
+    if (share) {
+      s_y[group][c / 4] = y;
+      if (c == 0) s_ml[group] = make_float2(top, sum);
+      __syncthreads();
+      if (group == 0) {
+        const float4 mine = y;
+        const float2 own = make_float2(top, sum);
+#pragma unroll
+        for (int g = 1; g < GROUPS; ++g) top = fmaxf(top, s_ml[g].x);
+        ref = top > -INFINITY ? top : 0.0f;
+        sum = 0.0f;
+        y = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+        add(own, mine);
+#pragma unroll
+        for (int g = 1; g < GROUPS; ++g) add(s_ml[g], s_y[g][c / 4]);
+      }
+      __syncthreads();
+      if (group != 0) continue;
     }
     // rows that see no key: zeros
     const float inv = top > -INFINITY ? 1.0f / sum : 1.0f;

@@ -94,7 +94,7 @@ kino_status check_q8_cache(const kino_q8_cache* c, const char* what) {
     return fail(KINO_EINVAL, "%s: empty cache, batch or table", what);
   if (c->heads > 65535 || c->batch > 65535 ||
       c->num_blocks > 0x7fffffffLL / (c->heads * c->block) ||
-      c->table_blocks > 0x7fffffffLL / c->block)
+      c->table_blocks > 0x3fffffffLL / c->block)
     return fail(KINO_ENOTSUPPORTED, "%s: cache too large", what);
   if (!aligned16(c->k_codes) || !aligned16(c->v_codes))
     return fail(KINO_EINVAL, "%s: codes not 16-byte aligned", what);
@@ -144,9 +144,11 @@ kino_status plan_q8_attention(const kino_q8_cache* c, const kino_q8_attention_ar
   if (group > 128)
     return fail(KINO_ENOTSUPPORTED, "%s: at most 128 query heads on a cache head", what);
   // Query rows of a sequence on one cache head, on average (the lengths are on the device; both
-  // kernels take any).
+  // kernels take any). Up to 64 rows the kernel for few rows is the faster one although it reads
+  // the cache again for each 16 of them (16 sequences of 8192 tokens, 8 heads of 128: 32 rows
+  // 131 us, with tcgen05 287; 64 rows 247 and 287; 8 sequences of 2000 with 128 rows 84 and 48).
   const int64_t rows = (g->rows + c->batch - 1) / c->batch * group;
-  p->decode_tiles = rows <= 8 ? 1 : rows <= 16 ? 2 : 0;
+  p->decode_tiles = rows <= 8 ? 1 : rows <= 64 && group <= 16 ? 2 : 0;
   const int64_t tile = p->decode_tiles ? 8 * p->decode_tiles : 512;
   p->tile_tokens = static_cast<int>(p->decode_tiles ? tile / group : 4 * (128 / group));
   p->tile_rows = static_cast<int>(tile);
@@ -170,8 +172,8 @@ kino_status launch_q8_decode(const kino_q8_cache* c, const kino::Q8Attn& a, cuda
   if (st != KINO_OK) return st;
   launch_pdl(kernel, dim3(a.runs), dim3(kino::Q8D_THREADS), L::TOTAL, stream, mk, mv, a);
   if (a.runs > 1)
-    launch_pdl(kino::attention_q8_combine_kernel<D, kino::Q8D_BN>, dim3(a.runs - 1, NT), dim3(256),
-               0, stream, a);
+    launch_pdl(kino::attention_q8_combine_kernel<D, kino::Q8D_BN>, dim3(a.runs - 1, 2),
+               dim3(256), 0, stream, a);
   return check_launch("kino_q8_attention");
 }
 
@@ -468,7 +470,6 @@ kino_status kino_q8_attention(const kino_q8_cache* cache, const kino_q8_attentio
   a.causal = args->causal != 0;
   a.tile_tokens = p.tile_tokens;
   a.tile_rows = p.tile_rows;
-  a.least_units = 4;
   a.runs = p.runs;
   a.part_o = static_cast<float*>(args->workspace);
   a.part_ml = a.part_o + 2LL * p.runs * p.tile_rows * cache->dim;

@@ -308,6 +308,8 @@ SMALL = [  # held (with the new tokens), new, cache heads, group
     ([40, 0, 513], [1, 0, 2], 2, 7),
     ([700], [1], 1, 16),
     ([2, 90], [4, 4], 2, 2),
+    ([130, 61], [9, 20], 2, 3),
+    ([200], [4], 1, 16),
 ]
 
 
@@ -332,6 +334,8 @@ MANY = [  # held (with the new tokens), new, cache heads, group
     ([64, 200], [70, 20], 1, 5),  # more queries than keys: the first see none
     ([350], [3], 1, 100),
     ([300], [270], 3, 1),
+    ([333], [12], 2, 12),
+    ([900, 20], [30, 12], 1, 16),
 ]
 
 
