@@ -52,8 +52,10 @@ void launch_q8_rows(const kino::Q8RowArgs& a, int64_t rows, cudaStream_t stream)
   };
   if (nv <= 2)
     run(kino::q8_rows_kernel<FMT, 2>);
-  else
+  else if (nv <= 4)
     run(kino::q8_rows_kernel<FMT, 4>);
+  else
+    run(kino::q8_wide_rows_kernel<FMT>);
 }
 
 int log2_block(int64_t block) { return block == 16 ? 4 : block == 32 ? 5 : block == 64 ? 6 : 7; }
@@ -186,7 +188,9 @@ kino_status launch_q8_attention(const kino_q8_cache* c, kino::Q8Attn& a, int dec
   CUtensorMap mq;
   const uint64_t dims[3] = {D, static_cast<uint64_t>(a.heads) * a.group,
                             static_cast<uint64_t>(a.rows.rows)};
-  const uint64_t strides[2] = {static_cast<uint64_t>(a.hs_q), static_cast<uint64_t>(a.ld_q)};
+  // (the stride of a dimension of one counts for nothing but the map's own checks)
+  const uint64_t strides[2] = {dims[1] > 1 ? static_cast<uint64_t>(a.hs_q) : D,
+                               dims[2] > 1 ? static_cast<uint64_t>(a.ld_q) : D * dims[1]};
   const uint32_t box[3] = {64, static_cast<uint32_t>(a.group),
                            static_cast<uint32_t>(a.tile_tokens / 4)};
   kino_status st = make_map(&mq, a.q, 3, dims, strides, box);
@@ -216,8 +220,8 @@ kino_status kino_q8_rows(const void* x, int64_t ldx, const void* residual, int64
     return fail(KINO_EINVAL, "kino_q8_rows: null");
   if (!q8_format(format)) return fail(KINO_EINVAL, "kino_q8_rows: format %d", format);
   if (rows < 1 || rows > 0x7fffffffLL) return fail(KINO_EINVAL, "kino_q8_rows: rows");
-  if (dim < 8 || dim % 8 || dim > 16384)
-    return fail(KINO_ENOTSUPPORTED, "kino_q8_rows: dim %% 8 == 0 and dim <= 16384, not %lld",
+  if (dim < 8 || dim % 8 || dim > 131072)
+    return fail(KINO_ENOTSUPPORTED, "kino_q8_rows: dim %% 8 == 0 and dim <= 131072, not %lld",
                 (long long)dim);
   if (!aligned16(x) || !aligned16(residual) || !aligned16(weight) || !aligned16(hidden) ||
       (reinterpret_cast<uintptr_t>(codes) & 7u))

@@ -130,6 +130,78 @@ __global__ void __launch_bounds__(Q8_ROW_MAX_THREADS) q8_rows_kernel(const Q8Row
   }
 }
 
+// The same for rows that do not fit the registers of a CTA: two passes over the row, the second
+// from the sum that the first one stored (each thread reads back what it wrote) or from x again.
+template <int FMT>
+__global__ void __launch_bounds__(Q8_ROW_MAX_THREADS) q8_wide_rows_kernel(const Q8RowArgs a) {
+  griddep_wait();
+  griddep_launch();
+  __shared__ float s_sum[16];
+  __shared__ uint32_t s_max[16];
+  const int64_t row = blockIdx.x;
+  const int nvec = a.dim >> 3;
+  const uint4* xr = reinterpret_cast<const uint4*>(a.x + row * a.ldx);
+  uint4* hr = reinterpret_cast<uint4*>(a.hidden + row * a.ld_hidden);
+  auto weighted = [&](float (&v)[8], int c) {
+    if (a.weight == nullptr) return;
+    float w[8];
+    q8_unpack8(__ldg(reinterpret_cast<const uint4*>(a.weight) + c), w);
+#pragma unroll
+    for (int j = 0; j < 8; ++j) v[j] *= w[j] + a.weight_offset;
+  };
+  float sum = 0.0f;
+  uint32_t top = 0;
+  for (int c = threadIdx.x; c < nvec; c += Q8_ROW_MAX_THREADS) {
+    float v[8];
+    q8_unpack8(xr[c], v);
+    if (a.residual != nullptr) {
+      float r[8];
+      q8_unpack8(reinterpret_cast<const uint4*>(a.residual + row * a.ld_residual)[c], r);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) v[j] = bf16_round(v[j] + r[j]);
+    }
+    if (a.hidden != nullptr)
+      hr[c] = make_uint4(pack_bf16x2(v[0], v[1]), pack_bf16x2(v[2], v[3]), pack_bf16x2(v[4], v[5]),
+                         pack_bf16x2(v[6], v[7]));
+#pragma unroll
+    for (int j = 0; j < 8; ++j) sum = fmaf(v[j], v[j], sum);
+    weighted(v, c);
+#pragma unroll
+    for (int j = 0; j < 8; ++j) top = max(top, abs_bits(v[j]));
+  }
+  top = __reduce_max_sync(0xffffffffu, top);
+  sum = warp_sum_f(sum);
+  if ((threadIdx.x & 31) == 0) {
+    s_sum[threadIdx.x >> 5] = sum;
+    s_max[threadIdx.x >> 5] = top;
+  }
+  __syncthreads();
+  top = __reduce_max_sync(0xffffffffu, s_max[threadIdx.x & 15]);
+  sum = warp_sum_f((threadIdx.x & 31) < 16 ? s_sum[threadIdx.x & 15] : 0.0f);
+  float scale = q8_scale<FMT>(top);
+  Q8Factor f = {0.0f, 0.0f};
+  if (scale > 0.0f) {
+    f = q8_quotient(q8_top<FMT>(), __uint_as_float(top));
+    if (a.norm) {
+      scale *= rsqrtf(sum / static_cast<float>(a.dim) + a.eps);
+      if (scale < Q8_LEAST_SCALE) scale = 0.0f;
+    }
+  }
+  if (threadIdx.x == 0) a.scales[row] = scale;
+  const uint4* again = a.hidden != nullptr ? hr : xr;
+  uint2* cr = reinterpret_cast<uint2*>(a.codes + row * a.dim);
+  for (int c = threadIdx.x; c < nvec; c += Q8_ROW_MAX_THREADS) {
+    float v[8];
+    q8_unpack8(again[c], v);
+    weighted(v, c);
+    cr[c] = !(scale > 0.0f) ? make_uint2(0u, 0u)
+                            : make_uint2(q8_encode4<FMT>(f.times(v[0]), f.times(v[1]),
+                                                         f.times(v[2]), f.times(v[3])),
+                                         q8_encode4<FMT>(f.times(v[4]), f.times(v[5]),
+                                                         f.times(v[6]), f.times(v[7])));
+  }
+}
+
 // ---------------------------------------------------------------- cache write
 // Codes live as (block, head, slot, dim): the tokens of one block and head are contiguous, which
 // is the unit every kernel here reads. Sequence b's new tokens take positions lengths[b] on.

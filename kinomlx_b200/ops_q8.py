@@ -117,7 +117,8 @@ def _quantize_rows(x, weight, eps, residual, dtype, weight_offset, norm, hidden,
             if hidden.shape != x.shape:
                 raise ValueError(f"hidden {tuple(hidden.shape)} does not match {tuple(x.shape)}")
         r2, h2 = _rows(residual, "residual"), _rows(hidden, "hidden")
-        r_ptr, ld_r, h_ptr, ld_h = r2.data_ptr(), r2.stride(0), h2.data_ptr(), h2.stride(0)
+        r_ptr, h_ptr = r2.data_ptr(), h2.data_ptr()
+        ld_r, ld_h = (r2.stride(0), h2.stride(0)) if rows > 1 else (dim, dim)
     elif hidden is not None:
         raise ValueError("hidden is the sum with a residual: give one")
     if weight is not None:
@@ -129,14 +130,14 @@ def _quantize_rows(x, weight, eps, residual, dtype, weight_offset, norm, hidden,
     scales = x.new_empty(x.shape[:-1], dtype=F32)
     if rows and dim:
         _launch(label, 0.0, (3.0 if residual is None else 7.0) * rows * dim, device,
-                "kino_q8_rows", x2.data_ptr(), x2.stride(0), r_ptr, ld_r, w_ptr, weight_offset, eps,
+                "kino_q8_rows", x2.data_ptr(), x2.stride(0) if rows > 1 else dim, r_ptr, ld_r, w_ptr, weight_offset, eps,
                 norm, h_ptr, ld_h, codes.data_ptr(), scales.data_ptr(), fmt, rows, dim)
     return codes, scales, x if hidden is None else hidden
 
 
 def quantize_tokens(x: torch.Tensor, dtype: torch.dtype = torch.int8):
     """Codes like x and a scale for each row of x (..., dim) bf16: activations by token, or a
-    weight (out, in) by output channel. dim a multiple of 8, at most 16384."""
+    weight (out, in) by output channel. dim a multiple of 8, at most 131072."""
     codes, scales, _ = _quantize_rows(x, None, 0.0, None, dtype, 0.0, 0, None, "quantize_tokens")
     return codes, scales
 
@@ -281,6 +282,12 @@ def _heads(t: torch.Tensor, name: str, dim: int, device: torch.device) -> None:
         raise ValueError(f"{name} {tuple(t.shape)} is not (rows, heads, {dim})")
 
 
+def _strides(t: torch.Tensor) -> tuple[int, int]:
+    """Row and head strides of (rows, heads, dim); a dimension of one has any, so 0."""
+    rows, heads, _ = t.shape
+    return t.stride(0) if rows > 1 else 0, t.stride(1) if heads > 1 else 0
+
+
 def kv_cache_write(
     cache: KVCache,
     k: torch.Tensor,
@@ -309,8 +316,7 @@ def kv_cache_write(
         return
     starts = _starts(token_starts, args.batch, rows, device)
     _launch("kv_cache_write", 0.0, 6.0 * k.numel(), device, "kino_q8_cache_write", args,
-            k.data_ptr(), k.stride(0), k.stride(1), v.data_ptr(), v.stride(0), v.stride(1), starts,
-            rows)
+            k.data_ptr(), *_strides(k), v.data_ptr(), *_strides(v), starts, rows)
 
 
 def kv_cache_read(
@@ -365,7 +371,7 @@ def kv_cache_attention(
     if not rows or not heads or not args.batch:
         return out
     call = _lib.Q8AttentionArgs(
-        q.data_ptr(), q.stride(0), q.stride(1), out.data_ptr(), out.stride(0), out.stride(1),
+        q.data_ptr(), *_strides(q), out.data_ptr(), *_strides(out),
         _starts(token_starts, args.batch, rows, device), rows, heads,
         args.dim**-0.5 if scale is None else scale, causal)
     size = _entries.get("size") or _entries.setdefault(

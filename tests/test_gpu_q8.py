@@ -38,7 +38,8 @@ def _same(a, b):
 # ---------------------------------------------------------------- rows
 @pytest.mark.parametrize("dtype", DTYPES)
 @pytest.mark.parametrize(("rows", "dim"), [(1, 8), (3, 64), (5, 504), (17, 1032), (2, 4096),
-                                           (3, 8200), (2, 16384)])
+                                           (3, 8200), (2, 16384), (3, 20008),
+                                           (1300, 96), (1, 131072)])
 def test_quantize_tokens_is_exact(cuda_device, dtype, rows, dim):
     x = _normal((rows, dim), rows + dim)
     x[0] *= 1e-3
@@ -65,7 +66,8 @@ def test_quantize_tokens_special_rows(cuda_device, dtype):
 
 
 @pytest.mark.parametrize("dtype", DTYPES)
-@pytest.mark.parametrize(("rows", "dim"), [(1, 8), (3, 264), (9, 2048), (2, 5000), (2, 16384)])
+@pytest.mark.parametrize(("rows", "dim"), [(1, 8), (3, 264), (9, 2048), (2, 5000), (2, 16384),
+                                           (2, 28672), (1250, 80)])
 @pytest.mark.parametrize("residual", [False, True])
 @pytest.mark.parametrize("weight", [False, True])
 def test_rms_norm_quantize(cuda_device, dtype, rows, dim, residual, weight):
@@ -78,7 +80,7 @@ def test_rms_norm_quantize(cuda_device, dtype, rows, dim, residual, weight):
         weight_offset=1.0 if weight else 0.0)
     h, y = ref.rms_norm(x, w, 1e-5, r, 1.0)
     assert torch.equal(hidden.cpu(), h)
-    # scale: a sum of squares of up to 42 fp32 additions in a row, halved by the root; rsqrtf 2 ulp;
+    # scale: a sum of squares of up to 66 fp32 additions in a row, halved by the root; rsqrtf 2 ulp;
     # four products and quotients and the weight's sum: below 3e-6 of the value. Codes do not depend
     # on the root: the weight's sum and two products, below 4 * 2^-24
     want = y.abs().amax(-1) / ref.TOP[dtype]
@@ -99,6 +101,8 @@ def test_rms_norm_quantize_in_place_and_strided(cuda_device):
     for got, want in zip((codes, scales, hidden), expect):
         assert torch.equal(got, want)
     assert torch.equal(wide, before)
+    one = ops_q8.quantize_tokens(wide[:1, 256:500].as_strided((1, 240), (13, 1)))  # any stride of one row
+    assert torch.equal(one[0], ops_q8.quantize_tokens(wide[:1, 256:496].contiguous())[0])
     three = ops_q8.quantize_tokens(r.view(2, 3, 256))
     two = ops_q8.quantize_tokens(r)
     assert three[0].shape == (2, 3, 256) and three[1].shape == (2, 3)
@@ -335,6 +339,7 @@ MANY = [  # held (with the new tokens), new, cache heads, group
     ([350], [3], 1, 100),
     ([300], [270], 3, 1),
     ([333], [12], 2, 12),
+    ([70], [1], 1, 33),
     ([900, 20], [30, 12], 1, 16),
 ]
 

@@ -68,7 +68,7 @@ def _rows_status(**over):
 @pytest.mark.parametrize(("over", "status"), [
     (dict(x=None), EINVAL), (dict(codes=None), EINVAL), (dict(scales=None), EINVAL),
     (dict(fmt=2), EINVAL), (dict(rows=0), EINVAL), (dict(dim=60), UNSUPPORTED),
-    (dict(dim=16392, ldx=16392), UNSUPPORTED), (dict(dim=0), UNSUPPORTED),
+    (dict(dim=131080, ldx=131080), UNSUPPORTED), (dict(dim=0), UNSUPPORTED),
     (dict(x=ADDRESS + 8), EINVAL), (dict(codes=ADDRESS + 4), EINVAL), (dict(ldx=68), UNSUPPORTED),
     (dict(ldx=56), EINVAL), (dict(residual=ADDRESS, ld_r=56), EINVAL),
     (dict(residual=ADDRESS + 2, ld_r=64), EINVAL), (dict(hidden=ADDRESS, ld_h=8), EINVAL),
