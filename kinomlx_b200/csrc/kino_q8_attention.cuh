@@ -617,20 +617,29 @@ __global__ void __launch_bounds__(Q8D_THREADS, 1)
 // ---------------------------------------------------------------- many query rows
 // tcgen05 on CTA pairs (cta_group::2): an item is up to two tiles of 256 query rows, 128 of each
 // in either CTA (chunks of 128 / group tokens x group heads, so that grouped heads share the keys'
-// tile), in ping-pong over blocks of 128 keys. A pair shares a block's operands: each CTA converts
-// 64 of its keys for the first product and half of the dims of its V for the second, which halves
-// the conversion and the shared-memory traffic that bound the same kernel on single CTAs (1400 us
-// against 1100 for 4608 queries x 9216 keys x 24 heads of 128).
+// tile), over blocks of 128 keys. A pair shares a block's operands: each CTA converts 64 of its
+// keys for the first product and half of the dims of its V for the second, which halves the
+// conversion and the shared-memory traffic.
 //   warp 0        Q chunks by TMA, when the last item's first products are done
-//   warp 1        tensor memory; in the even CTA the products, in the odd one the word to the
-//                 even one that a block's converted operands are there (by a thread without loads
-//                 in flight, which a release at cluster scope would wait for)
-//   warps 2..9    softmax of the CTA's rows, four warps for each tile
+//   warp 1        tensor memory; in the even CTA the products, issued from code that the compiler
+//                 knows to be uniform (from one divergent thread they took twice as long); in the
+//                 odd CTA the word to the even one that a block's operands are there (by a thread
+//                 without loads in flight, which a release at cluster scope would wait for)
+//   warps 2..9    softmax of the CTA's rows, four warps a tile and a thread a row, 64 keys at a time
 //   warps 10..13  codes -> bf16 (K), f16 (V) in the layout TMA would write (128-byte swizzle);
 //                 each thread keeps the next block's codes in registers
-// Tensor memory as in the dense kernel: S_A, S_B, O_A, O_B. All roles of both CTAs walk the same
-// run of items; the pipelines' phases go on over items. Tile A sees a prefix of the item's keys
-// under a causal mask and leaves the blocks behind it out.
+// Tensor memory: S_A in columns [0, 128), S_B [128, 256), O_A [256, 256 + D), O_B [384, 384 + D).
+// Each S is two buffers of 64 keys, so that a tile's next scores are there while its warps work on
+// these (keys 32 h .. and 64 + 32 h .. of the block for buffer h: 32 of each CTA's 64). P of a buffer
+// overlies its scores. All roles of both CTAs walk the same run of items; the pipelines' phases go
+// on over items. Tile A sees a prefix of the item's keys under a causal mask and leaves the blocks
+// behind it out.
+//
+// 4608 queries x 9216 keys, 24 heads of 128: 600 us, 870 TFLOP/s (the dense bf16 kernel: 424 us);
+// on single CTAs with two warps a row 1400, in pairs 1100, a row a thread 810, with the issue and
+// the words between CTAs as above 655, in half blocks 600. Neither pipe is full: the tensor pipe
+// is busy for about 2400 of 5000 cycles a block, exponentials for 2048; the chain score ->
+// maximum -> P -> product of either tile is what remains, and the conversion (100 us of the 600).
 constexpr int Q8P_BN = 128;
 constexpr int Q8P_THREADS = 448;
 
