@@ -24,6 +24,14 @@
 
 namespace kino {
 
+// Where a run starts, for the kernel that adds the pieces.
+struct Q8RunStart {
+  int64_t run;    // units of a run
+  int64_t first;  // the item's first query row of its sequence
+  int tile, head, count;
+  int at, units;  // the run's first unit of the item's units (units 0: an empty run)
+};
+
 struct Q8Attn {
   const __nv_bfloat16* q;
   int64_t ld_q, hs_q;
@@ -45,6 +53,7 @@ struct Q8Attn {
   int runs;         // CTAs (or CTA pairs)
   float* part_o;    // [2 * runs][tile_rows][D]
   float* part_ml;   // [2 * runs][tile_rows][2]: row maximum (log2 units), row sum
+  Q8RunStart* starts;  // [runs]
 };
 
 // The items and their units, as every CTA sees them.
@@ -242,6 +251,9 @@ __global__ void __launch_bounds__(Q8D_THREADS, 1)
     int64_t at = 0;
     if (u0 < total) at = w.seek(u0);
     if (lane == 0) {
+      a.starts[blockIdx.x] = u0 < total ? Q8RunStart{run, w.first, w.tile, w.head, w.count,
+                                                     static_cast<int>(at), w.units}
+                                        : Q8RunStart{run, 0, 0, 0, 0, 0, 0};
       s_run[0] = u0;
       s_run[1] = u0 + run < total ? u0 + run : total;
       s_run[2] = at;
@@ -744,6 +756,10 @@ __global__ void __launch_bounds__(Q8P_THREADS, 1)
     int64_t in = 0;
     if (u0 < total) in = w.seek(u0);
     if (lane == 0) {
+      if (rank == 0)
+        a.starts[pair] = u0 < total ? Q8RunStart{run, w.first, w.tile, w.head, w.count,
+                                                 static_cast<int>(in), w.units}
+                                    : Q8RunStart{run, 0, 0, 0, 0, 0, 0};
       s_run[0] = u0;
       s_run[1] = u0 + run < total ? u0 + run : total;
       s_run[2] = in;
@@ -1306,88 +1322,79 @@ __global__ void __launch_bounds__(Q8P_THREADS, 1)
 // first and last is in slot 0.) gridDim.y CTAs share the rows, D / 4 threads a row. One sequence on
 // one head may be in as many pieces as there are CTAs: then all groups of D / 4 threads of a CTA
 // share a row's pieces (32000 keys on one head: 14 us, 46 with one group a row).
-template <int D, int BN>
+template <int D>
 __global__ void __launch_bounds__(256) attention_q8_combine_kernel(const Q8Attn a) {
-  // This kernel may start when every CTA of the attention has passed its own wait for what ran
-  // before it, so lengths and starts are there and the items can be found while it still runs.
-  __shared__ int s_item[4];      // b, tile, head, pieces (0: nothing to do)
-  __shared__ int s_slot0;
+  griddep_wait();
+  griddep_launch();
   constexpr int LANES = D / 4, GROUPS = 256 / LANES;
   __shared__ float4 s_y[GROUPS][LANES];
   __shared__ float2 s_ml[GROUPS];
-  Q8Work<BN> w(a);
-  if (threadIdx.x < 32) {
-    const int64_t total = w.total();
-    const int64_t run = q8_run_units(a, total);
-    const int64_t border = (blockIdx.x + 1) * run;
-    int pieces = 0, slot0 = 0;
-    if (border < total) {
-      const int64_t in = w.seek(border);
-      const int64_t start = border - in, end = start + w.units;
-      if (in > 0 && start >= border - run) {
-        pieces = static_cast<int>((end - 1) / run - blockIdx.x) + 1;
-        slot0 = 2 * static_cast<int>(blockIdx.x) + (start > border - run ? 1 : 0);
-      }
-    }
-    if (threadIdx.x == 0) {
-      s_item[0] = w.b;
-      s_item[1] = w.tile;
-      s_item[2] = w.head;
-      s_item[3] = pieces;
-      s_slot0 = slot0;
-    }
-  }
-  __syncthreads();
-  griddep_wait();  // the pieces
-  griddep_launch();
-  const int pieces = s_item[3];
-  if (pieces == 0) return;
-  w.enter(s_item[0]);
-  const int tok0 = s_item[1] * a.tile_tokens, head = s_item[2];
-  const int live = min(a.tile_tokens, w.count - tok0) * a.group;
+  const Q8RunStart s = a.starts[blockIdx.x + 1];
+  const int64_t border = (blockIdx.x + 1) * s.run, start = border - s.at;
+  if (s.units == 0 || s.at == 0 || start < border - s.run) return;
+  const int pieces = static_cast<int>((start + s.units - 1) / s.run - blockIdx.x) + 1;
+  const int slot0 = 2 * static_cast<int>(blockIdx.x) + (start > border - s.run ? 1 : 0);
+  const int tok0 = s.tile * a.tile_tokens;
+  const int live = min(a.tile_tokens, s.count - tok0) * a.group;
   const int group = threadIdx.x / LANES, c = threadIdx.x % LANES * 4;
   const bool share = pieces >= 2 * GROUPS;
   const int first = share ? group : 0, stride = share ? GROUPS : 1;
   for (int r = share ? blockIdx.y : blockIdx.y * GROUPS + group; r < live;
        r += gridDim.y * (share ? 1 : GROUPS)) {
     auto place = [&](int k) {
-      const int slot = k == 0 ? s_slot0 : 2 * (static_cast<int>(blockIdx.x) + k);
+      const int slot = k == 0 ? slot0 : 2 * (static_cast<int>(blockIdx.x) + k);
       return static_cast<int64_t>(slot) * a.tile_rows + r;
     };
     float top = -INFINITY, sum = 0.0f;
-#pragma unroll 4
-    for (int k = first; k < pieces; k += stride) top = fmaxf(top, a.part_ml[place(k) * 2]);
-    float ref = top > -INFINITY ? top : 0.0f;
     float4 y = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-    auto add = [&](const float2 ml, const float4 x) {
-      const float wt = ex2_approx(ml.x - ref);
-      sum = fmaf(ml.y, wt, sum);
+    auto add = [&](float wt, float l, const float4 x) {
+      sum = fmaf(l, wt, sum);
       y.x = fmaf(x.x, wt, y.x);
       y.y = fmaf(x.y, wt, y.y);
       y.z = fmaf(x.z, wt, y.z);
       y.w = fmaf(x.w, wt, y.w);
     };
-#pragma unroll 4
-    for (int k = first; k < pieces; k += stride) {
-      const int64_t at = place(k);
-      add(*reinterpret_cast<const float2*>(a.part_ml + at * 2),
-          *reinterpret_cast<const float4*>(a.part_o + at * D + c));
+    constexpr int LOT = 8;  // pieces whose reads are in flight together
+    for (int k0 = first; k0 < pieces; k0 += LOT * stride) {
+      float2 ml[LOT];
+      float4 x[LOT];
+#pragma unroll
+      for (int i = 0; i < LOT; ++i) {
+        const int k = k0 + i * stride;
+        ml[i] = make_float2(-INFINITY, 0.0f);
+        x[i] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+        if (k < pieces) {
+          const int64_t at = place(k);
+          ml[i] = *reinterpret_cast<const float2*>(a.part_ml + at * 2);
+          x[i] = *reinterpret_cast<const float4*>(a.part_o + at * D + c);
+        }
+      }
+      float now = top;
+#pragma unroll
+      for (int i = 0; i < LOT; ++i) now = fmaxf(now, ml[i].x);
+      const float ref = now > -INFINITY ? now : 0.0f;
+      const float keep = ex2_approx(top - ref);
+      sum *= keep;
+      y.x *= keep;
+      y.y *= keep;
+      y.z *= keep;
+      y.w *= keep;
+      top = now;
+#pragma unroll
+      for (int i = 0; i < LOT; ++i) add(ex2_approx(ml[i].x - ref), ml[i].y, x[i]);
     }
     if (share) {
       s_y[group][c / 4] = y;
       if (c == 0) s_ml[group] = make_float2(top, sum);
       __syncthreads();
       if (group == 0) {
-        const float4 mine = y;
-        const float2 own = make_float2(top, sum);
 #pragma unroll
         for (int g = 1; g < GROUPS; ++g) top = fmaxf(top, s_ml[g].x);
-        ref = top > -INFINITY ? top : 0.0f;
+        const float ref = top > -INFINITY ? top : 0.0f;
         sum = 0.0f;
         y = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-        add(own, mine);
 #pragma unroll
-        for (int g = 1; g < GROUPS; ++g) add(s_ml[g], s_y[g][c / 4]);
+        for (int g = 0; g < GROUPS; ++g) add(ex2_approx(s_ml[g].x - ref), s_ml[g].y, s_y[g][c / 4]);
       }
       __syncthreads();
       if (group != 0) continue;
@@ -1395,8 +1402,8 @@ __global__ void __launch_bounds__(256) attention_q8_combine_kernel(const Q8Attn 
     // rows that see no key: zeros
     const float inv = top > -INFINITY ? 1.0f / sum : 1.0f;
     const int tok = tok0 + r / a.group;
-    *reinterpret_cast<uint2*>(a.out + (w.first + tok) * a.ld_out +
-                              static_cast<int64_t>(head * a.group + r % a.group) * a.hs_out + c) =
+    *reinterpret_cast<uint2*>(a.out + (s.first + tok) * a.ld_out +
+                              static_cast<int64_t>(s.head * a.group + r % a.group) * a.hs_out + c) =
         make_uint2(pack_bf16x2(y.x * inv, y.y * inv), pack_bf16x2(y.z * inv, y.w * inv));
   }
 }

@@ -155,7 +155,8 @@ kino_status plan_q8_attention(const kino_q8_cache* c, const kino_q8_attention_ar
   p->tile_tokens = static_cast<int>(p->decode_tiles ? tile / group : 4 * (128 / group));
   p->tile_rows = static_cast<int>(tile);
   p->runs = p->decode_tiles ? device_sms() : device_sms() / 2;  // CTAs, or pairs of them
-  p->bytes = 2LL * p->runs * tile * (c->dim + 2) * 4;
+  p->bytes = 2LL * p->runs * tile * (c->dim + 2) * 4 +
+             p->runs * static_cast<int64_t>(sizeof(kino::Q8RunStart));
   return KINO_OK;
 }
 
@@ -174,7 +175,7 @@ kino_status launch_q8_decode(const kino_q8_cache* c, const kino::Q8Attn& a, cuda
   if (st != KINO_OK) return st;
   launch_pdl(kernel, dim3(a.runs), dim3(kino::Q8D_THREADS), L::TOTAL, stream, mk, mv, a);
   if (a.runs > 1)
-    launch_pdl(kino::attention_q8_combine_kernel<D, kino::Q8D_BN>, dim3(a.runs - 1, 2),
+    launch_pdl(kino::attention_q8_combine_kernel<D>, dim3(a.runs - 1, 2),
                dim3(256), 0, stream, a);
   return check_launch("kino_q8_attention");
 }
@@ -201,7 +202,7 @@ kino_status launch_q8_attention(const kino_q8_cache* c, kino::Q8Attn& a, int dec
   if (st != KINO_OK) return st;
   launch_ex(kernel, dim3(2 * a.runs), dim3(kino::Q8P_THREADS), L::TOTAL, stream, 2, mq, a);
   if (a.runs > 1)
-    launch_pdl(kino::attention_q8_combine_kernel<D, kino::Q8P_BN>, dim3(a.runs - 1, 16), dim3(256),
+    launch_pdl(kino::attention_q8_combine_kernel<D>, dim3(a.runs - 1, 32), dim3(256),
                0, stream, a);
   return check_launch("kino_q8_attention");
 }
@@ -477,6 +478,7 @@ kino_status kino_q8_attention(const kino_q8_cache* cache, const kino_q8_attentio
   a.runs = p.runs;
   a.part_o = static_cast<float*>(args->workspace);
   a.part_ml = a.part_o + 2LL * p.runs * p.tile_rows * cache->dim;
+  a.starts = reinterpret_cast<kino::Q8RunStart*>(a.part_ml + 2LL * p.runs * p.tile_rows * 2);
   const cudaStream_t s = static_cast<cudaStream_t>(stream);
   const bool i8 = cache->format == KINO_Q8_INT8;
   if (cache->dim == 128)

@@ -86,6 +86,13 @@ def _need(t: torch.Tensor, name: str, dtype: torch.dtype, device: torch.device |
         raise ValueError(f"{name} needs a unit stride in its last dimension")
 
 
+def _empty_as(t: torch.Tensor, dtype: torch.dtype) -> torch.Tensor:
+    """Contiguous, of t's shape (empty_like is the quickest of torch's ways to one)."""
+    if t.is_contiguous():
+        return torch.empty_like(t, dtype=dtype)
+    return torch.empty(t.shape, dtype=dtype, device=t.device)
+
+
 def _rows(t: torch.Tensor, name: str) -> torch.Tensor:
     """(..., dim) as (rows, dim) without a copy."""
     if t.dim() == 2:
@@ -111,7 +118,7 @@ def _quantize_rows(x, weight, eps, residual, dtype, weight_offset, norm, hidden,
         if residual.shape != x.shape:
             raise ValueError(f"residual {tuple(residual.shape)} does not match {tuple(x.shape)}")
         if hidden is None:
-            hidden = x.new_empty(x.shape)
+            hidden = _empty_as(x, BF16)
         else:
             _need(hidden, "hidden", BF16, device)
             if hidden.shape != x.shape:
@@ -126,8 +133,8 @@ def _quantize_rows(x, weight, eps, residual, dtype, weight_offset, norm, hidden,
         if weight.shape != (dim,):
             raise ValueError(f"weight {tuple(weight.shape)} does not match width {dim}")
         w_ptr = weight.data_ptr()
-    codes = x.new_empty(x.shape, dtype=dtype)
-    scales = x.new_empty(x.shape[:-1], dtype=F32)
+    codes = _empty_as(x, dtype)
+    scales = torch.empty(rows if x.dim() == 2 else x.shape[:-1], dtype=F32, device=device)
     if rows and dim:
         _launch(label, 0.0, (3.0 if residual is None else 7.0) * rows * dim, device,
                 "kino_q8_rows", x2.data_ptr(), x2.stride(0) if rows > 1 else dim, r_ptr, ld_r, w_ptr, weight_offset, eps,
@@ -192,7 +199,7 @@ def linear_int8(
         b_ptr = bias.data_ptr()
     shape = (*codes.shape[:-1], n)
     if out is None:
-        out = codes.new_empty(shape, dtype=BF16)
+        out = torch.empty(shape, dtype=BF16, device=device)
     else:
         _need(out, "out", BF16, device)
         if out.shape != shape:
@@ -363,7 +370,7 @@ def kv_cache_attention(
     if heads % args.heads:
         raise ValueError(f"{heads} query heads on {args.heads} cache heads")
     if out is None:
-        out = torch.empty_like(q, memory_format=torch.contiguous_format)
+        out = _empty_as(q, BF16)
     else:
         _heads(out, "out", args.dim, device)
         if out.shape != q.shape:
