@@ -179,8 +179,9 @@ __device__ __forceinline__ int64_t q8_run_units(const Q8Attn& a, int64_t total) 
 // a fragment's rows and columns stand for, so nothing is transposed but the 16 x 8
 // probabilities (movmatrix).
 constexpr int Q8D_BN = 64;
-constexpr int Q8D_WARPS = 8;  // that compute; one more loads
-constexpr int Q8D_THREADS = 32 * (Q8D_WARPS + 1);
+// Warps that compute (one more loads): three groups of four where the registers allow it (16 x 32768
+// tokens, one tile of rows: 184 us, 192 with two groups).
+constexpr int q8d_warps(int nt) { return nt == 1 ? 12 : 8; }
 
 template <int D, int NT>
 struct Q8DecodeSmem {
@@ -190,13 +191,14 @@ struct Q8DecodeSmem {
   // has seen each earlier phase of its barrier. (Another group could come to a stage whose last
   // load is still on its way, since loads need not arrive in order, and take the phase before that
   // for its own.)
-  static constexpr int STAGES = (NT == 1 ? 10 : 8) * (D == 128 ? 1 : 2);
-  static_assert(STAGES % (Q8D_WARPS / 4) == 0, "a stage belongs to one group of warps");
+  static constexpr int WARPS = q8d_warps(NT), TURNS = WARPS / 4;
+  static constexpr int STAGES = (NT == 1 ? 9 : 8) * (D == 128 ? 1 : 2);
+  static_assert(STAGES % TURNS == 0, "a stage belongs to one group of warps");
   static constexpr int LDO = D + 4;        // padded row of the merge buffer, in floats
   static constexpr int MERGE_OFF = STAGES * STAGE;
-  static constexpr int MERGE = Q8D_WARPS * 8 * NT * LDO * 4;
+  static constexpr int MERGE = WARPS * 8 * NT * LDO * 4;
   static constexpr int ML_OFF = MERGE_OFF + MERGE;      // [warp][8 NT][2]
-  static constexpr int SC_OFF = ML_OFF + Q8D_WARPS * 8 * NT * 8;
+  static constexpr int SC_OFF = ML_OFF + WARPS * 8 * NT * 8;
   // per stage, of the four 16-key groups: K scales (with the softmax scale), 1 / vs, log2(vs), and
   // a word of which groups are there
   static constexpr int SC = 64;
@@ -227,7 +229,7 @@ __device__ __forceinline__ uint32_t q8_chunk(int r, int c) {
 }
 
 template <int D, int NT, int FMT>
-__global__ void __launch_bounds__(Q8D_THREADS, 1)
+__global__ void __launch_bounds__(32 * (q8d_warps(NT) + 1), 1)
     attention_q8_decode_kernel(const __grid_constant__ CUtensorMap map_k,
                                const __grid_constant__ CUtensorMap map_v, const Q8Attn a) {
   using L = Q8DecodeSmem<D, NT>;
@@ -278,11 +280,12 @@ __global__ void __launch_bounds__(Q8D_THREADS, 1)
   w.head = s_item[2];
   w.units = Q8Work<Q8D_BN>::units_of(a, w.count, w.len, w.tile);
 
-  if (warp == Q8D_WARPS) {
+  constexpr int WARPS = L::WARPS;
+  if (warp == WARPS) {
     // ---- loads: the places and scales of up to eight units are looked up at once, a lane for each
     // group of 16 keys, while the eight before them are issued (a look-up is two dependent reads,
     // about a microsecond, in which two or three units arrive)
-    constexpr int GROUPS = Q8D_BN / 16, LOT = 32 / GROUPS, STEP = 2;
+    constexpr int GROUPS = Q8D_BN / 16, LOT = 32 / GROUPS, STEP = 4;
     const int box = a.block >= Q8D_BN ? Q8D_BN : a.block;
     const bool leads = (lane & 3) * 16 % box == 0;  // the copy of its group's box
     const unsigned lead_groups = box == 64 ? 1u : box == 32 ? 5u : 15u;
@@ -370,11 +373,11 @@ __global__ void __launch_bounds__(Q8D_THREADS, 1)
     // ---- products and softmax
     const int g = lane >> 2, t = lane & 3;
     const int part = warp & 3;   // 16 keys of the unit
-    const int turn = warp >> 2;  // which of two units
+    const int turn = warp >> 2;  // which of TURNS units
     constexpr int KS = D / 16;   // steps of the first product, row tiles of the second
     float* merge = reinterpret_cast<float*>(smem + L::MERGE_OFF);
     float* ml = reinterpret_cast<float*>(smem + L::ML_OFF);
-    int used = 0;
+    int used = 0, next = 0;  // units so far, and the turn of the one that is next
     int piece = 0;
     bool ok = true;
     while (left > 0) {
@@ -444,7 +447,9 @@ __global__ void __launch_bounds__(Q8D_THREADS, 1)
         }
       }
       for (int u = 0; u < n; ++u, ++used) {
-        if ((used & 1) != turn) continue;
+        const bool take = next == turn;
+        next = next + 1 == L::TURNS ? 0 : next + 1;
+        if (!take) continue;
         const int stage = used % L::STAGES;
         ok = ok && __all_sync(0xffffffffu,
                               mbar_wait(&full[stage], (used / L::STAGES) & 1, abort_flag));
@@ -581,20 +586,20 @@ __global__ void __launch_bounds__(Q8D_THREADS, 1)
           for (int i = 0; i < KS; ++i)
             *reinterpret_cast<float2*>(dst + 2 * i) = make_float2(o[j][i][e], o[j][i][2 + e]);
         }
-      asm volatile("bar.sync 1, %0;" ::"n"(32 * Q8D_WARPS) : "memory");
+      asm volatile("bar.sync 1, %0;" ::"n"(32 * WARPS) : "memory");
       const int slot = 2 * static_cast<int>(blockIdx.x) + (piece > 0 ? 1 : 0);
-      for (int e = threadIdx.x; e < 8 * NT * (D / 4); e += 32 * Q8D_WARPS) {
+      for (int e = threadIdx.x; e < 8 * NT * (D / 4); e += 32 * WARPS) {
         const int r = e / (D / 4), c = (e % (D / 4)) * 4;
         const int tok = tok0 + r / a.group;
         if (r >= a.tile_tokens * a.group || tok >= w.count) continue;
         float top = -INFINITY;
 #pragma unroll
-        for (int k = 0; k < Q8D_WARPS; ++k) top = fmaxf(top, ml[(k * 8 * NT + r) * 2]);
+        for (int k = 0; k < WARPS; ++k) top = fmaxf(top, ml[(k * 8 * NT + r) * 2]);
         const float ref = top > -INFINITY ? top : 0.0f;
         float sum = 0.0f;
         float4 y = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
 #pragma unroll
-        for (int k = 0; k < Q8D_WARPS; ++k) {
+        for (int k = 0; k < WARPS; ++k) {
           const float wt = ex2_approx(ml[(k * 8 * NT + r) * 2] - ref);
           sum += wt * ml[(k * 8 * NT + r) * 2 + 1];
           const float4 x = *reinterpret_cast<const float4*>(merge + (k * 8 * NT + r) * L::LDO + c);
@@ -617,7 +622,7 @@ __global__ void __launch_bounds__(Q8D_THREADS, 1)
           }
         }
       }
-      asm volatile("bar.sync 1, %0;" ::"n"(32 * Q8D_WARPS) : "memory");
+      asm volatile("bar.sync 1, %0;" ::"n"(32 * WARPS) : "memory");
       left -= n;
       at = 0;
       ++piece;

@@ -173,7 +173,7 @@ kino_status launch_q8_decode(const kino_q8_cache* c, const kino::Q8Attn& a, cuda
   constexpr auto kernel = kino::attention_q8_decode_kernel<D, NT, FMT>;
   st = q8_smem<kernel>(L::TOTAL);
   if (st != KINO_OK) return st;
-  launch_pdl(kernel, dim3(a.runs), dim3(kino::Q8D_THREADS), L::TOTAL, stream, mk, mv, a);
+  launch_pdl(kernel, dim3(a.runs), dim3(32 * (L::WARPS + 1)), L::TOTAL, stream, mk, mv, a);
   if (a.runs > 1)
     launch_pdl(kino::attention_q8_combine_kernel<D>, dim3(a.runs - 1, 2),
                dim3(256), 0, stream, a);
