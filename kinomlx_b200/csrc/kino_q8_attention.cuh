@@ -652,7 +652,8 @@ __global__ void __launch_bounds__(32 * (q8d_warps(NT) + 1), 1)
 // on over items. Tile A sees a prefix of the item's keys under a causal mask and leaves the blocks
 // behind it out.
 //
-// 4608 queries x 9216 keys, 24 heads of 128: 600 us, 870 TFLOP/s (the dense bf16 kernel: 424 us);
+// 4608 queries x 9216 keys, 24 heads of 128: 600 us in a short burst, 870 TFLOP/s, 630 sustained
+// (the dense bf16 kernel: 424 in a burst);
 // on single CTAs with two warps a row 1400, in pairs 1100, a row a thread 810, with the issue and
 // the words between CTAs as above 655, in half blocks 600. Neither pipe is full: the tensor pipe
 // is busy for about 2400 of 5000 cycles a block, exponentials for 2048; the chain score ->
