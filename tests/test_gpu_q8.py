@@ -674,3 +674,46 @@ def test_front_end_refusals(cuda_device):
     assert ops_q8.kv_cache_read(cache, table, lengths, 0)[0].shape == (2, 0, 2, 64)
     assert not ops_q8.kv_cache_attention(k, cache, table, lengths).any()
     ops.device_status()
+
+
+@pytest.mark.parametrize("new", [[1, 1], [40, 25]])
+def test_rows_in_front_and_a_table_of_a_wider_one(cuda_device, new):
+    held, heads, group = [120, 70], 2, 3
+    cpu, cache, table = _cache(2, 130, heads, 128, 32, E4M3, 31, cuda_device)
+    wide = torch.full((2, table.shape[1] + 5), -7, dtype=torch.int32, device=cuda_device)
+    wide[:, 2 : 2 + table.shape[1]] = table.to(cuda_device)
+    view = wide[:, 2 : 2 + table.shape[1]]
+    rows, front = sum(new), 4
+    q = _normal((front + rows + 2, heads * group, 128), 32)
+    starts = torch.tensor([front, front + new[0], front + rows], dtype=torch.int32, device=cuda_device)
+    lengths = torch.tensor(held, dtype=torch.int32, device=cuda_device)
+    out = torch.full(q.shape, 9.0, dtype=BF16, device=cuda_device)
+    ops_q8.kv_cache_attention(q.to(cuda_device), cache, view, lengths, starts, out=out)
+    ops.device_status()
+    assert bool((out[:front] == 9).all()) and bool((out[front + rows:] == 9).all())
+    _check_attention(out[front : front + rows].cpu(), *ref.attention(
+        q[front : front + rows], *cpu, table, lengths.cpu(), (starts - front).cpu()))
+    k = _normal((front + rows, heads, 128), 33)
+    at = torch.tensor([10, 3], dtype=torch.int32, device=cuda_device)
+    ops_q8.kv_cache_write(cache, k.to(cuda_device), k.to(cuda_device), view, at, starts)
+    codes, scales = ref.cache_write(cpu.k_codes, cpu.k_scales, k, table, at.cpu(), starts.cpu())
+    assert torch.equal(cache.k_scales.cpu(), scales) and _same(cache.k_codes, codes)
+    ops.device_status()
+
+
+def test_leading_dimensions_and_launch_log(cuda_device):
+    x = _normal((2, 5, 128), 41).to(cuda_device)
+    w = _normal((64, 128), 42).to(cuda_device)
+    wq = ops_q8.quantize_tokens(w)
+    log = ops.LaunchLog()
+    ops.set_launch_log(log)
+    try:
+        codes, scales, hidden = ops_q8.rms_norm_quantize(x)
+        y = ops_q8.linear_int8(codes, scales, *wq)
+    finally:
+        ops.set_launch_log(None)
+    torch.cuda.synchronize()
+    assert hidden is x and y.shape == (2, 5, 64)
+    assert [r[0] for r in log.records] == ["rms_norm_quantize", "linear_int8"]
+    flat = ops_q8.rms_norm_quantize(x.view(10, 128))
+    assert torch.equal(y.view(10, 64), ops_q8.linear_int8(*flat[:2], *wq))
