@@ -130,8 +130,23 @@ __global__ void __launch_bounds__(Q8_ROW_MAX_THREADS) q8_rows_kernel(const Q8Row
   }
 }
 
-// The same for rows that do not fit the registers of a CTA: two passes over the row, the second
-// from the sum that the first one stored (each thread reads back what it wrote) or from x again.
+// Values c of a row in a second pass: the sum that the first one stored (each thread reads back what
+// it wrote; x or the residual may be gone under it), or x, and the residual to it, once more.
+__device__ __forceinline__ void q8_row_again(const Q8RowArgs& a, int64_t row, int c, float (&v)[8]) {
+  if (a.hidden != nullptr) {
+    q8_unpack8(reinterpret_cast<const uint4*>(a.hidden + row * a.ld_hidden)[c], v);
+    return;
+  }
+  q8_unpack8(reinterpret_cast<const uint4*>(a.x + row * a.ldx)[c], v);
+  if (a.residual != nullptr) {
+    float r[8];
+    q8_unpack8(reinterpret_cast<const uint4*>(a.residual + row * a.ld_residual)[c], r);
+#pragma unroll
+    for (int j = 0; j < 8; ++j) v[j] = bf16_round(v[j] + r[j]);
+  }
+}
+
+// The same for rows that do not fit the registers of a CTA: two passes over the row.
 template <int FMT>
 __global__ void __launch_bounds__(Q8_ROW_MAX_THREADS) q8_wide_rows_kernel(const Q8RowArgs a) {
   griddep_wait();
@@ -188,11 +203,10 @@ __global__ void __launch_bounds__(Q8_ROW_MAX_THREADS) q8_wide_rows_kernel(const 
     }
   }
   if (threadIdx.x == 0) a.scales[row] = scale;
-  const uint4* again = a.hidden != nullptr ? hr : xr;
   uint2* cr = reinterpret_cast<uint2*>(a.codes + row * a.dim);
   for (int c = threadIdx.x; c < nvec; c += Q8_ROW_MAX_THREADS) {
     float v[8];
-    q8_unpack8(again[c], v);
+    q8_row_again(a, row, c, v);
     weighted(v, c);
     cr[c] = !(scale > 0.0f) ? make_uint2(0u, 0u)
                             : make_uint2(q8_encode4<FMT>(f.times(v[0]), f.times(v[1]),

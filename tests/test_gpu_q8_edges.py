@@ -1,0 +1,50 @@
+"""8-bit serving operators at the edges of their ranges: calls without a sum's buffer, rows whose
+squares leave fp32, the widest product, queries that are huge, tiny or infinite, strides of every
+order, and a cache whose offsets pass 32 bits."""
+
+from __future__ import annotations
+
+import math
+
+import pytest
+import torch
+
+from kinomlx_b200 import _lib, ops, ops_q8
+from oracle import serving_q8 as ref
+
+pytestmark = pytest.mark.gpu
+
+BF16 = torch.bfloat16
+INT8, E4M3 = torch.int8, torch.float8_e4m3fn
+DTYPES = [INT8, E4M3]
+
+
+def _normal(shape, seed, std=1.0):
+    return (torch.randn(shape, generator=torch.Generator().manual_seed(seed)) * std).to(BF16)
+
+
+def _same(a, b):
+    a, b = a.cpu().float(), b.cpu().float()
+    return bool(((a == b) | (a.isnan() & b.isnan())).all())
+
+
+# ---------------------------------------------------------------- rows
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("dim", [64, 16384, 16392, 40000])
+@pytest.mark.parametrize("norm", [0, 1])
+def test_residual_without_a_buffer_for_the_sum(cuda_device, dtype, dim, norm):
+    """The C entry point's `hidden` may be NULL: codes and scales are those of the sum all the same."""
+    x, r = _normal((3, dim), dim), _normal((3, dim), dim + 1, 5.0)
+    xd, rd = x.to(cuda_device), r.to(cuda_device)
+    codes = torch.empty((3, dim), dtype=dtype, device=cuda_device)
+    scales = torch.empty(3, device=cuda_device)
+    status = _lib.load().kino_q8_rows(
+        xd.data_ptr(), dim, rd.data_ptr(), dim, None, 0.0, 1e-6, norm, None, 0, codes.data_ptr(),
+        scales.data_ptr(), ops_q8.FORMATS[dtype], 3, dim, torch.cuda.current_stream().cuda_stream)
+    assert status == 0, _lib.last_error()
+    if norm:
+        want = ops_q8.rms_norm_quantize(xd, residual=rd, dtype=dtype)
+    else:
+        want = ref.quantize_rows((x.float() + r.float()).to(BF16), dtype)
+    assert torch.equal(scales.cpu(), want[1].cpu()) and _same(codes, want[0])
+    assert torch.equal(xd.cpu(), x) and torch.equal(rd.cpu(), r)
