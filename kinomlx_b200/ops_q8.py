@@ -18,6 +18,7 @@ device; entries that do not fit are skipped there and `ops.device_status` raises
 
 from __future__ import annotations
 
+import math
 from typing import NamedTuple
 
 import torch
@@ -100,7 +101,8 @@ def _rows(t: torch.Tensor, name: str) -> torch.Tensor:
     if t.dim() == 0:
         raise ValueError(f"{name} needs rows")
     try:
-        return t.view(-1, t.shape[-1]) if t.numel() else t.reshape(0, t.shape[-1])
+        return (t.view(-1, t.shape[-1]) if t.numel()
+                else t.reshape(math.prod(t.shape[:-1]), t.shape[-1]))
     except RuntimeError:
         raise ValueError(f"{name}: rows of {tuple(t.shape)} are not at one stride") from None
 
@@ -110,6 +112,8 @@ def _quantize_rows(x, weight, eps, residual, dtype, weight_offset, norm, hidden,
     _need(x, "x", BF16)
     x2 = _rows(x, "x")
     rows, dim = x2.shape
+    if rows and not dim:
+        raise ValueError(f"x {tuple(x.shape)} has rows of width 0")
     device = x.device
     r_ptr = h_ptr = w_ptr = None
     ld_r = ld_h = 0
@@ -135,7 +139,7 @@ def _quantize_rows(x, weight, eps, residual, dtype, weight_offset, norm, hidden,
         w_ptr = weight.data_ptr()
     codes = _empty_as(x, dtype)
     scales = torch.empty(rows if x.dim() == 2 else x.shape[:-1], dtype=F32, device=device)
-    if rows and dim:
+    if rows:
         _launch(label, 0.0, (3.0 if residual is None else 7.0) * rows * dim, device,
                 "kino_q8_rows", x2.data_ptr(), x2.stride(0) if rows > 1 else dim, r_ptr, ld_r, w_ptr, weight_offset, eps,
                 norm, h_ptr, ld_h, codes.data_ptr(), scales.data_ptr(), fmt, rows, dim)
@@ -184,6 +188,8 @@ def linear_int8(
     _need(w_scales, "w_scales", F32, device)
     x2 = _rows(codes, "codes")
     m, k = x2.shape
+    if m and not k:
+        raise ValueError(f"codes {tuple(codes.shape)} have rows of width 0")
     if w_codes.dim() != 2 or w_codes.shape[1] != k:
         raise ValueError(f"weight {tuple(w_codes.shape)} does not match input width {k}")
     n = w_codes.shape[0]

@@ -48,3 +48,23 @@ def test_residual_without_a_buffer_for_the_sum(cuda_device, dtype, dim, norm):
         want = ref.quantize_rows((x.float() + r.float()).to(BF16), dtype)
     assert torch.equal(scales.cpu(), want[1].cpu()) and _same(codes, want[0])
     assert torch.equal(xd.cpu(), x) and torch.equal(rd.cpu(), r)
+
+
+def test_rows_without_values_are_refused(cuda_device):
+    for shape in ((4, 0), (2, 3, 0)):
+        x = torch.empty(shape, dtype=BF16, device=cuda_device)
+        codes = torch.empty(shape, dtype=INT8, device=cuda_device)
+        weight = torch.empty((8, 0), dtype=INT8, device=cuda_device)
+        with pytest.raises(ValueError, match="width"):
+            ops_q8.quantize_tokens(x)
+        with pytest.raises(ValueError, match="width"):
+            ops_q8.rms_norm_quantize(x, residual=x)
+        with pytest.raises(ValueError, match="width"):
+            ops_q8.linear_int8(codes, torch.ones(shape[:-1], device=cuda_device), weight,
+                               torch.ones(8, device=cuda_device))
+    # no rows are nothing to do
+    codes, scales = ops_q8.quantize_tokens(torch.empty((2, 0, 64), dtype=BF16, device=cuda_device))
+    assert codes.shape == (2, 0, 64) and scales.shape == (2, 0)
+    y = ops_q8.linear_int8(codes, scales, *ops_q8.quantize_tokens(
+        torch.ones((8, 64), dtype=BF16, device=cuda_device)))
+    assert y.shape == (2, 0, 8)

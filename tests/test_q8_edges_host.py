@@ -1,0 +1,33 @@
+"""Refusals of the 8-bit serving operators at the edges of their shapes, without a GPU."""
+
+from __future__ import annotations
+
+import pytest
+import torch
+
+from kinomlx_b200 import ops_q8
+
+BF16 = torch.bfloat16
+
+
+@pytest.mark.parametrize("shape", [(4, 0), (2, 3, 0), (0,)])
+def test_rows_without_values_are_refused(monkeypatch, shape):
+    """Outputs would be left unwritten: rows there are, but no value that the kernels could read."""
+    monkeypatch.setattr(ops_q8, "_need", lambda *_: None)  # these tensors are on the CPU
+    x, codes = torch.empty(shape, dtype=BF16), torch.empty(shape, dtype=torch.int8)
+    for call in (lambda: ops_q8.quantize_tokens(x),
+                 lambda: ops_q8.rms_norm_quantize(x, residual=x),
+                 lambda: ops_q8.linear_int8(codes, torch.ones(shape[:-1]),
+                                            torch.empty((8, 0), dtype=torch.int8), torch.ones(8))):
+        with pytest.raises(ValueError, match="width 0"):
+            call()
+
+
+def test_no_rows_are_nothing_to_do(monkeypatch):
+    monkeypatch.setattr(ops_q8, "_need", lambda *_: None)
+    monkeypatch.setattr(ops_q8, "_launch", None)  # not called
+    for shape in ((0, 64), (2, 0, 64), (0, 0)):
+        codes, scales = ops_q8.quantize_tokens(torch.empty(shape, dtype=BF16))
+        assert codes.shape == shape and scales.shape == shape[:-1]
+        y = ops_q8.linear_int8(codes, scales, torch.empty((8, shape[-1]), dtype=torch.int8), torch.ones(8))
+        assert y.shape == (*shape[:-1], 8)
