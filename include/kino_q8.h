@@ -44,7 +44,7 @@ kino_status kino_q8_rows(const void* x, int64_t ldx, const void* residual, int64
                          int64_t rows, int64_t dim, void* stream);
 
 /* out[i, j] = bf16(float(sum_k x[i, k] * w[j, k]) * x_scales[i] * w_scales[j] + bias[j]): int8
- * codes, the sum exact in int32 (k <= 131072). x: m x k at row stride ldx, w: n x k at ldw (bytes,
+ * codes, the sum exact in int32 (k < 131072). x: m x k at row stride ldx, w: n x k at ldw (bytes,
  * multiples of 16, 16-byte aligned), out: bf16 m x n at ldo (a multiple of 8). k % 16 == 0,
  * n % 8 == 0. bias: [n] bf16 or NULL; scales and bias 16-byte aligned. */
 kino_status kino_q8_linear(const void* x, int64_t ldx, const float* x_scales, const void* w,

@@ -263,8 +263,8 @@ kino_status kino_q8_linear(const void* x, int64_t ldx, const float* x_scales, co
   if (k % 16 || n % 8 || ldx % 16 || ldw % 16 || ldo % 8)
     return fail(KINO_ENOTSUPPORTED, "kino_q8_linear: k and the code strides must be multiples of "
                 "16, n and the output stride of 8 (k=%lld n=%lld)", (long long)k, (long long)n);
-  if (k > 131072)  // 131072 * 128 * 128 = 2^31: the int32 sum
-    return fail(KINO_ENOTSUPPORTED, "kino_q8_linear: k <= 131072, not %lld", (long long)k);
+  if (k >= 131072)  // 131072 products of -128 with itself are 2^31, one more than int32 holds
+    return fail(KINO_ENOTSUPPORTED, "kino_q8_linear: k < 131072, not %lld", (long long)k);
   if (m > (1 << 28) || n > (1 << 28))
     return fail(KINO_ENOTSUPPORTED, "kino_q8_linear: shape too large");
   if (ldx < k || ldw < k || ldo < n) return fail(KINO_EINVAL, "kino_q8_linear: stride below width");

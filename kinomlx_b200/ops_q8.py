@@ -180,7 +180,7 @@ def linear_int8(
 ) -> torch.Tensor:
     """bf16(codes @ w_codes.T * scales[:, None] * w_scales + bias) for int8 codes (..., k) with a
     scale for each row and an int8 weight (n, k) with one for each channel; the sum over k is
-    exact. k a multiple of 16, n of 8."""
+    exact. k a multiple of 16 below 131072, n of 8."""
     _need(codes, "codes", torch.int8)
     device = codes.device
     _need(w_codes, "w_codes", torch.int8, device)

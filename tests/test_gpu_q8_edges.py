@@ -68,3 +68,18 @@ def test_rows_without_values_are_refused(cuda_device):
     y = ops_q8.linear_int8(codes, scales, *ops_q8.quantize_tokens(
         torch.ones((8, 64), dtype=BF16, device=cuda_device)))
     assert y.shape == (2, 0, 8)
+
+
+# ---------------------------------------------------------------- product
+@pytest.mark.parametrize(("m", "n"), [(3, 16), (300, 6400)])  # both forms
+def test_the_widest_product_of_the_lowest_codes(cuda_device, m, n):
+    k = 131056  # the widest that the int32 sum holds: 131056 * 2^14 = 2^31 - 2^18
+    x = torch.full((m, k), -128, dtype=INT8, device=cuda_device)
+    w = torch.full((n, k), -128, dtype=INT8, device=cuda_device)
+    w[1] = 127
+    ones = torch.ones(max(m, n), device=cuda_device)
+    out = ops_q8.linear_int8(x, ones[:m], w, ones[:n])
+    ops.device_status()
+    want = torch.full((n,), float(128 * 128 * k)).to(BF16)
+    want[1] = torch.tensor(-128.0 * 127 * k).to(BF16)
+    assert torch.equal(out.cpu(), want.expand(m, n))

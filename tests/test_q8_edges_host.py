@@ -5,7 +5,7 @@ from __future__ import annotations
 import pytest
 import torch
 
-from kinomlx_b200 import ops_q8
+from kinomlx_b200 import _lib, ops_q8
 
 BF16 = torch.bfloat16
 
@@ -31,3 +31,12 @@ def test_no_rows_are_nothing_to_do(monkeypatch):
         assert codes.shape == shape and scales.shape == shape[:-1]
         y = ops_q8.linear_int8(codes, scales, torch.empty((8, shape[-1]), dtype=torch.int8), torch.ones(8))
         assert y.shape == (*shape[:-1], 8)
+
+
+@pytest.mark.parametrize("k", [131072, 262144])
+def test_products_that_int32_cannot_hold_are_refused(k):
+    """131072 products of the code -128 with itself are 2^31."""
+    at = 1 << 20  # never read
+    lib = _lib.load()
+    assert lib.kino_q8_linear(at, k, at, at, k, at, None, at, 64, 4, 64, k, None) == 2
+    assert "k <" in _lib.last_error()
