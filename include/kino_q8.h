@@ -37,7 +37,8 @@ int kino_q8_abi_version(void);
  * x, residual, hidden: rows x dim bf16 at their own row strides (multiples of 8, 16-byte aligned);
  * hidden may be x or residual. weight: [dim] bf16 or NULL (then no weight and no offset). codes:
  * contiguous rows x dim bytes, 8-byte aligned; scales: [rows] fp32. dim % 8 == 0, dim <= 131072.
- * Row strides are not looked at where there is one row. */
+ * Row strides are not looked at where there is one row. Rows whose squares or weighted values leave
+ * fp32's range are normed in 64 bits, and a row of zeros has scale 0 whatever eps is. */
 kino_status kino_q8_rows(const void* x, int64_t ldx, const void* residual, int64_t ld_residual,
                          const void* weight, float weight_offset, float eps, int norm,
                          void* hidden, int64_t ld_hidden, void* codes, float* scales, int format,

@@ -42,8 +42,124 @@ struct Q8RowArgs {
   int dim;
 };
 
+// Values c of a row in a second pass: the sum that the first one stored (each thread reads back what
+// it wrote; x or the residual may be gone under it), or x, and the residual to it, once more.
+__device__ __forceinline__ void q8_row_again(const Q8RowArgs& a, int64_t row, int c, float (&v)[8]) {
+  if (a.hidden != nullptr) {
+    q8_unpack8(reinterpret_cast<const uint4*>(a.hidden + row * a.ld_hidden)[c], v);
+    return;
+  }
+  q8_unpack8(reinterpret_cast<const uint4*>(a.x + row * a.ldx)[c], v);
+  if (a.residual != nullptr) {
+    float r[8];
+    q8_unpack8(reinterpret_cast<const uint4*>(a.residual + row * a.ld_residual)[c], r);
+#pragma unroll
+    for (int j = 0; j < 8; ++j) v[j] = bf16_round(v[j] + r[j]);
+  }
+}
+
+// The scale of a normed row, and the factor of its codes, from the sum of squares and the largest
+// |p|; false where fp32 cannot give them (the same in all threads): squares or products that left
+// its range, or so small that they lost bits. (A term's error is at most 2^-126, so the mean is
+// right to 2^-26 from 2^-100 on. Products below 2^-126 have lost bits too, which counts only if the
+// root brings the scale back to 2^-126.)
+template <int FMT>
+__device__ __forceinline__ bool q8_norm_scale(const Q8RowArgs& a, float sum, uint32_t top,
+                                              float& scale, Q8Factor& f) {
+  const float mean = sum / static_cast<float>(a.dim) + a.eps;
+  if (!(mean >= 7.888609e-31f && mean < INFINITY) || top >= 0x7F800000u) return false;
+  const float root = rsqrtf(mean);
+  if (scale > 0.0f) {
+    f = q8_quotient(q8_top<FMT>(), __uint_as_float(top));
+    scale *= root;
+    if (scale < Q8_LEAST_SCALE) scale = 0.0f;
+    return true;
+  }
+  return (__uint_as_float(top) + 1.401298e-45f) * root < Q8_LEAST_SCALE;
+}
+
+// Such a row once more in 64 bits, by the whole CTA. Values of 1e20 and more (their squares pass
+// fp32's range), weights that carry h * w out of it, or values below 1e-15 with a smaller eps: no
+// path of a model in working order, so nothing here is tuned.
+template <int FMT>
+__device__ __noinline__ void q8_norm_row_far(const Q8RowArgs& a, int64_t row) {
+  __shared__ double s_sum[16], s_max[16];
+  __shared__ int s_bad;
+  const int nvec = a.dim >> 3;
+  auto both = [&](const __nv_bfloat16* at, int i) {
+    return unpack_bf16x2(*reinterpret_cast<const uint32_t*>(at + i));
+  };
+  // values i, i + 1 of the row (as in q8_row_again), and times their weights
+  auto values = [&](int i) {
+    if (a.hidden != nullptr) return both(a.hidden + row * a.ld_hidden, i);
+    float2 h = both(a.x + row * a.ldx, i);
+    if (a.residual != nullptr) {
+      const float2 r = both(a.residual + row * a.ld_residual, i);
+      h = make_float2(bf16_round(h.x + r.x), bf16_round(h.y + r.y));
+    }
+    return h;
+  };
+  auto product = [&](float h, float w) {
+    return a.weight == nullptr ? static_cast<double>(h) : static_cast<double>(h) * (w + a.weight_offset);
+  };
+  auto weights = [&](int i) { return a.weight == nullptr ? make_float2(0.0f, 0.0f) : both(a.weight, i); };
+  double sum = 0.0, top = 0.0;
+  bool bad = false;
+#pragma unroll 1
+  for (int c = threadIdx.x; c < nvec; c += blockDim.x)
+#pragma unroll 1
+    for (int i = 8 * c; i < 8 * c + 8; i += 2) {
+      const float2 h = values(i), w = weights(i);
+      const double p = product(h.x, w.x), q = product(h.y, w.y);
+      sum += static_cast<double>(h.x) * h.x + static_cast<double>(h.y) * h.y;
+      bad = bad || !isfinite(p) || !isfinite(q);
+      top = fmax(top, fmax(fabs(p), fabs(q)));
+    }
+#pragma unroll 1
+  for (int o = 16; o > 0; o >>= 1) {
+    sum += __shfl_xor_sync(0xffffffffu, sum, o);
+    top = fmax(top, __shfl_xor_sync(0xffffffffu, top, o));
+  }
+  if (threadIdx.x == 0) s_bad = 0;
+  __syncthreads();
+  if ((threadIdx.x & 31) == 0) {
+    s_sum[threadIdx.x >> 5] = sum;
+    s_max[threadIdx.x >> 5] = top;
+  }
+  if (bad) s_bad = 1;
+  __syncthreads();
+  sum = top = 0.0;
+#pragma unroll 1
+  for (int i = 0; i < static_cast<int>(blockDim.x >> 5); ++i) {
+    sum += s_sum[i];
+    top = fmax(top, s_max[i]);
+  }
+  float scale = 0.0f;
+  if (s_bad) {
+    scale = __uint_as_float(0x7FC00000u);
+  } else if (top > 0.0) {
+    scale = static_cast<float>(top / (q8_top<FMT>() * sqrt(sum / a.dim + a.eps)));
+    if (scale < Q8_LEAST_SCALE) scale = 0.0f;
+    if (isinf(scale)) scale = __uint_as_float(0x7FC00000u);  // so is the row's largest value
+  }
+  if (threadIdx.x == 0) a.scales[row] = scale;
+  const double factor = scale > 0.0f ? q8_top<FMT>() / top : 0.0;
+#pragma unroll 1
+  for (int c = threadIdx.x; c < nvec; c += blockDim.x)
+#pragma unroll 1
+    for (int i = 8 * c; i < 8 * c + 8; i += 2) {
+      uint32_t codes = 0;
+      if (scale > 0.0f) {
+        const float2 h = values(i), w = weights(i);
+        codes = q8_encode4<FMT>(static_cast<float>(product(h.x, w.x) * factor),
+                                static_cast<float>(product(h.y, w.y) * factor), 0.0f, 0.0f);
+      }
+      *reinterpret_cast<uint16_t*>(a.codes + row * a.dim + i) = static_cast<uint16_t>(codes);
+    }
+}
+
 template <int FMT, int NV>
-__global__ void __launch_bounds__(Q8_ROW_MAX_THREADS) q8_rows_kernel(const Q8RowArgs a) {
+__global__ void __launch_bounds__(Q8_ROW_MAX_THREADS) q8_rows_kernel(const __grid_constant__ Q8RowArgs a) {
   griddep_wait();
   griddep_launch();
   __shared__ float s_sum[16];
@@ -108,12 +224,13 @@ __global__ void __launch_bounds__(Q8_ROW_MAX_THREADS) q8_rows_kernel(const Q8Row
   }
   float scale = q8_scale<FMT>(top);
   Q8Factor f = {0.0f, 0.0f};
-  if (scale > 0.0f) {
-    f = q8_quotient(q8_top<FMT>(), __uint_as_float(top));
-    if (a.norm) {
-      scale *= rsqrtf(sum / static_cast<float>(a.dim) + a.eps);
-      if (scale < Q8_LEAST_SCALE) scale = f.hi = f.lo = 0.0f;
+  if (a.norm) {
+    if (__builtin_expect(!q8_norm_scale<FMT>(a, sum, top, scale, f), 0)) {
+      q8_norm_row_far<FMT>(a, row);
+      return;
     }
+  } else if (scale > 0.0f) {
+    f = q8_quotient(q8_top<FMT>(), __uint_as_float(top));
   }
   if (threadIdx.x == 0) a.scales[row] = scale;
   uint2* cr = reinterpret_cast<uint2*>(a.codes + row * a.dim);
@@ -130,25 +247,11 @@ __global__ void __launch_bounds__(Q8_ROW_MAX_THREADS) q8_rows_kernel(const Q8Row
   }
 }
 
-// Values c of a row in a second pass: the sum that the first one stored (each thread reads back what
-// it wrote; x or the residual may be gone under it), or x, and the residual to it, once more.
-__device__ __forceinline__ void q8_row_again(const Q8RowArgs& a, int64_t row, int c, float (&v)[8]) {
-  if (a.hidden != nullptr) {
-    q8_unpack8(reinterpret_cast<const uint4*>(a.hidden + row * a.ld_hidden)[c], v);
-    return;
-  }
-  q8_unpack8(reinterpret_cast<const uint4*>(a.x + row * a.ldx)[c], v);
-  if (a.residual != nullptr) {
-    float r[8];
-    q8_unpack8(reinterpret_cast<const uint4*>(a.residual + row * a.ld_residual)[c], r);
-#pragma unroll
-    for (int j = 0; j < 8; ++j) v[j] = bf16_round(v[j] + r[j]);
-  }
-}
-
-// The same for rows that do not fit the registers of a CTA: two passes over the row.
+// The same for rows that do not fit the registers of a CTA: two passes over the row. (Four CTAs on
+// an SM: 2048 x 28672 with a residual 82 us, with three, as the registers of the rare 64-bit rows
+// would have it, 88.)
 template <int FMT>
-__global__ void __launch_bounds__(Q8_ROW_MAX_THREADS) q8_wide_rows_kernel(const Q8RowArgs a) {
+__global__ void __launch_bounds__(Q8_ROW_MAX_THREADS, 4) q8_wide_rows_kernel(const __grid_constant__ Q8RowArgs a) {
   griddep_wait();
   griddep_launch();
   __shared__ float s_sum[16];
@@ -195,12 +298,13 @@ __global__ void __launch_bounds__(Q8_ROW_MAX_THREADS) q8_wide_rows_kernel(const 
   sum = warp_sum_f((threadIdx.x & 31) < 16 ? s_sum[threadIdx.x & 15] : 0.0f);
   float scale = q8_scale<FMT>(top);
   Q8Factor f = {0.0f, 0.0f};
-  if (scale > 0.0f) {
-    f = q8_quotient(q8_top<FMT>(), __uint_as_float(top));
-    if (a.norm) {
-      scale *= rsqrtf(sum / static_cast<float>(a.dim) + a.eps);
-      if (scale < Q8_LEAST_SCALE) scale = 0.0f;
+  if (a.norm) {
+    if (__builtin_expect(!q8_norm_scale<FMT>(a, sum, top, scale, f), 0)) {
+      q8_norm_row_far<FMT>(a, row);
+      return;
     }
+  } else if (scale > 0.0f) {
+    f = q8_quotient(q8_top<FMT>(), __uint_as_float(top));
   }
   if (threadIdx.x == 0) a.scales[row] = scale;
   uint2* cr = reinterpret_cast<uint2*>(a.codes + row * a.dim);

@@ -50,6 +50,67 @@ def test_residual_without_a_buffer_for_the_sum(cuda_device, dtype, dim, norm):
     assert torch.equal(xd.cpu(), x) and torch.equal(rd.cpu(), r)
 
 
+def _far_rows(dim):
+    """(x, eps) whose squares, products or their sum leave fp32, each beside an ordinary row."""
+    base = _normal((6, dim), dim, 1.0).float()
+    base[:, 0] = 3.0
+    out = []
+    for factor, eps in ((1e20, 1e-6), (2.0**126, 1e-6), (1e-30, 0.0), (1e-39, 0.0), (1e-37, 1e-6),
+                        (1e-37, 1e-12), (1e-25, 1e-35), (1e19, 0.0)):
+        x = base.clone()
+        x[1:4] *= factor
+        x[2, 1:] *= 1e-3 if factor > 1 else 1.0  # one large value
+        x[4] = 0
+        out.append((x.clamp(-3.3e38, 3.3e38).to(BF16), eps))
+    return out
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("dim", [8, 128, 5000, 20008])
+@pytest.mark.parametrize("form", ["plain", "residual", "weight"])
+def test_norm_of_rows_whose_squares_leave_fp32(cuda_device, dtype, dim, form):
+    for i, (x, eps) in enumerate(_far_rows(dim)):
+        r = (x.float() * -0.5).to(BF16) if form == "residual" else None
+        w = None
+        if form == "weight":  # products that overflow or vanish before the root is taken
+            w = (_normal((dim,), i, 0.5).float() * (1e25 if i % 2 else 1e-10)).to(BF16)
+        args = [t if t is None else t.to(cuda_device) for t in (x, w)]
+        rd = None if r is None else r.to(cuda_device)
+        codes, scales, hidden = ops_q8.rms_norm_quantize(
+            *args, eps, residual=rd, dtype=dtype, hidden=rd)  # the sum over the residual
+        h, y = ref.rms_norm(x, w, eps, r)
+        y = torch.where(h == 0, torch.zeros_like(y), y)  # a row of zeros without eps is 0 / 0
+        assert torch.equal(hidden.cpu(), h)
+        want = y.abs().amax(-1) / ref.TOP[dtype]
+        none = want < 2.0**-126
+        assert bool(((want < 0.99 * 2.0**-126) | (want > 1.01 * 2.0**-126)).all())  # no border case
+        got = scales.cpu().double()
+        # as for ordinary rows: a sum of squares and its root in fp32 below 3e-6, codes below
+        # 4 * 2^-24 in front of their own rounding; longer sums only where fp64 is used
+        assert not got[none].any() and not codes.cpu().double()[none].any()
+        assert bool(((got - want).abs() <= 3e-6 * want)[~none].all()), (i, got, want)
+        c = codes.cpu().double()[~none]
+        q = y[~none] / want[~none, None]
+        half = 0.5 if dtype == INT8 else torch.clamp(q.abs() * 2.0**-4, min=2.0**-10)
+        assert bool(((c - q).abs() <= half + 4 * 2.0**-24 * (c.abs() + 1)).all()), i
+
+
+@pytest.mark.parametrize("dim", [128, 20008])
+def test_norm_of_rows_that_are_not_finite(cuda_device, dim):
+    x = _normal((5, dim), 3)
+    x[0, 5], x[1, 6], x[2, 7], x[3] = math.inf, -math.inf, math.nan, 1e25
+    x[3, 9] = math.nan
+    w = torch.ones(dim, dtype=BF16)
+    w[5] = 0  # infinity times 0
+    for weight in (None, w):
+        codes, scales, _ = ops_q8.rms_norm_quantize(
+            x.to(cuda_device), None if weight is None else weight.to(cuda_device))
+        assert scales[:4].isnan().all() and not codes[:4].any()
+        alone = ops_q8.rms_norm_quantize(x[4:].to(cuda_device),
+                                         None if weight is None else weight.to(cuda_device))
+        assert torch.equal(codes[4:], alone[0]) and torch.equal(scales[4:], alone[1])
+
+
 def test_rows_without_values_are_refused(cuda_device):
     for shape in ((4, 0), (2, 3, 0)):
         x = torch.empty(shape, dtype=BF16, device=cuda_device)
