@@ -412,10 +412,9 @@ __global__ void __launch_bounds__(32 * (q8d_warps(NT) + 1), 1)
           top = max(top, max((qf[j][i] & 0x7FFFu) << 16, qf[j][i] & 0x7FFF0000u));
         top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
         top = max(top, __shfl_xor_sync(0xffffffffu, top, 2));
-        const uint32_t ex = top >> 23;
-        const bool plain = ex == 0 || ex >= 254;  // zeros and subnormals, or not finite: as they are
-        const float down = plain ? 1.0f : __uint_as_float((254u - ex) << 23);
-        const float up = plain ? 1.0f : __uint_as_float(ex << 23);
+        // (the factors of zeros, subnormals and the largest values are the nearest normal ones)
+        const uint32_t ex = min(max(top >> 23, 1u), 253u);
+        const float down = __uint_as_float((254u - ex) << 23), up = __uint_as_float(ex << 23);
 #pragma unroll
         for (int i = 0; i < 2 * KS; ++i) {
           const float2 f = unpack_bf16x2(qf[j][i]);

@@ -144,3 +144,64 @@ def test_the_widest_product_of_the_lowest_codes(cuda_device, m, n):
     want = torch.full((n,), float(128 * 128 * k)).to(BF16)
     want[1] = torch.tensor(-128.0 * 127 * k).to(BF16)
     assert torch.equal(out.cpu(), want.expand(m, n))
+
+
+# ---------------------------------------------------------------- attention
+def _cache(batch, most, heads, dim, block, dtype, seed, device, codes=127):
+    g = torch.Generator().manual_seed(seed)
+    per = max(1, -(-most // block))
+    table = torch.randperm(batch * per, generator=g).view(batch, per).to(torch.int32)
+    cc = [torch.randint(-codes, codes + 1, (batch * per, heads, block, dim), generator=g)
+          for _ in range(2)]
+    scales = [(torch.rand((batch * per, heads), generator=g) + 0.5) * 0.02 for _ in range(2)]
+    cpu = ops_q8.KVCache(*((c if dtype == INT8 else c.float()).to(dtype) for c in cc), *scales)
+    return cpu, ops_q8.KVCache(*(t.to(device) for t in cpu)), table
+
+
+def _check(got, want, weight, reach, crowd, keys):
+    # f16 weights 2^-11 (2^-25 below 2^-14, against a largest of at least 1: `crowd`), scores by
+    # at most (dim + 4) * 2^-24 of their sum of magnitudes and exponentials 2^-20 (numerator and
+    # denominator), sums over the keys 2^-24 an addition (the tensor cores 2^-23), bf16 2^-8
+    dim = want.shape[-1]
+    inner = ((2.0**-11 + 2 * ((dim + 4) * 2.0**-24 * reach + 2.0**-20) + 3 * keys * 2.0**-24)
+             * weight + 2.0**-25 * crowd)
+    limit = inner + 2.0**-8 * (want.abs() + inner) + 1e-30
+    assert got.isfinite().all()
+    assert bool(((got.double() - want).abs() <= limit).all())
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize(("rows", "group"), [(1, 2), (6, 2), (70, 2)])
+@pytest.mark.parametrize("held", [100, 300])
+def test_attention_of_the_largest_queries(cuda_device, dtype, rows, group, held):
+    """Finite queries up to the largest bf16 values, with keys whose products stay in fp32."""
+    dim, heads = 128, 2
+    cpu, cache, table = _cache(1, held, heads, dim, 32, dtype, 3, cuda_device, codes=1)
+    for t in (cpu, cache):
+        t.k_scales.fill_(2.0**-120)
+    q = torch.zeros((rows, heads * group, dim))
+    g = torch.Generator().manual_seed(4)
+    at = torch.randint(0, dim, (rows, heads * group, 1), generator=g)
+    q.scatter_(2, at, 2.0**127 * (1 + torch.rand(at.shape, generator=g) * 0.98))
+    q = q.to(BF16)
+    assert q.isfinite().all()
+    lengths = torch.tensor([held], dtype=torch.int32)
+    got = ops_q8.kv_cache_attention(q.to(cuda_device), cache, table.to(cuda_device),
+                                    lengths.to(cuda_device), scale=0.02)
+    _check(got.cpu(), *ref.attention(q, *cpu, table, lengths, scale=0.02), held)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize(("rows", "group"), [(1, 2), (6, 2)])
+def test_attention_of_subnormal_queries(cuda_device, dtype, rows, group):
+    dim, heads, held = 128, 2, 150
+    cpu, cache, table = _cache(1, held, heads, dim, 32, dtype, 5, cuda_device)
+    for t in (cpu, cache):
+        t.k_scales.fill_(2.0**112)
+    q = (_normal((rows, heads * group, dim), 6).float() * 2.0**-128).to(BF16)
+    q[q.abs() >= 2.0**-126] = 2.0**-127
+    assert q.any() and bool((q.abs() < 2.0**-126).all())
+    lengths = torch.tensor([held], dtype=torch.int32)
+    got = ops_q8.kv_cache_attention(q.to(cuda_device), cache, table.to(cuda_device),
+                                    lengths.to(cuda_device), scale=32.0)
+    _check(got.cpu(), *ref.attention(q, *cpu, table, lengths, scale=32.0), held)
