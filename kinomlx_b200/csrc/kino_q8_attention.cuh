@@ -16,6 +16,7 @@
 // unnormalised partial result with its row maxima and sums; attention_q8_combine adds the pieces
 // of each cut item in a fixed order.
 #pragma once
+#include <cfloat>
 #include <type_traits>
 
 #include "kino_attention.cuh"
@@ -414,7 +415,10 @@ __global__ void __launch_bounds__(32 * (q8d_warps(NT) + 1), 1)
         top = max(top, __shfl_xor_sync(0xffffffffu, top, 2));
         // (the factors of zeros, subnormals and the largest values are the nearest normal ones)
         const uint32_t ex = min(max(top >> 23, 1u), 253u);
-        const float down = __uint_as_float((254u - ex) << 23), up = __uint_as_float(ex << 23);
+        const float down = __uint_as_float((254u - ex) << 23);
+        // (a row that is not finite has only infinite and NaN scores, whose softmax is NaN also
+        // where all of them are -infinity: its factor makes them NaN)
+        const float up = __uint_as_float(top < 0x7F800000u ? ex << 23 : 0x7FC00000u);
 #pragma unroll
         for (int i = 0; i < 2 * KS; ++i) {
           const float2 f = unpack_bf16x2(qf[j][i]);
@@ -1177,14 +1181,23 @@ __global__ void __launch_bounds__(Q8P_THREADS, 1)
             best[g] = max3f(max3f(x, y, z), max3f(u, f(12), f(13)), fmaxf(f(14), f(15)));
           }
         }
-        float mine = -INFINITY;
+        float y[4];
 #pragma unroll
         for (int g = 0; g < 4; ++g) {
           const float4 s4 = sc2[g >> 1];
-          const float y = fmaf(best[g], g & 1 ? s4.z : s4.x, g & 1 ? s4.w : s4.y);
-          // a masked group stays at -inf whatever its scales are
-          mine = fmaxf(mine, masked && ((g & 1) * 16 >= valid[g >> 1] || !((groups >> g) & 1))
-                                 ? -INFINITY : y);
+          y[g] = fmaf(best[g], g & 1 ? s4.z : s4.x, g & 1 ? s4.w : s4.y);
+        }
+        // A masked group stays at -inf whatever its scales are. One in sight counts as the lowest
+        // finite value at least: a row whose scores are all -inf then ends as 0 / 0, and not as
+        // one that sees no key.
+        float mine = -INFINITY;
+        if (masked) {
+#pragma unroll
+          for (int g = 0; g < 4; ++g)
+            if ((g & 1) * 16 < valid[g >> 1] && ((groups >> g) & 1))
+              mine = max3f(mine, y[g], -FLT_MAX);
+        } else {
+          mine = max3f(max3f(y[0], y[1], y[2]), y[3], -FLT_MAX);
         }
         // The reference moves only when it is exceeded by 2^8 (the stale one cancels in the
         // division).

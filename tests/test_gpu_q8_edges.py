@@ -205,3 +205,31 @@ def test_attention_of_subnormal_queries(cuda_device, dtype, rows, group):
     got = ops_q8.kv_cache_attention(q.to(cuda_device), cache, table.to(cuda_device),
                                     lengths.to(cuda_device), scale=32.0)
     _check(got.cpu(), *ref.attention(q, *cpu, table, lengths, scale=32.0), held)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize(("rows", "group"), [(2, 2), (7, 2), (140, 1)])
+@pytest.mark.parametrize("held", [60, 300])
+@pytest.mark.parametrize("value", [math.inf, -math.inf, math.nan])
+def test_attention_of_infinite_queries(cuda_device, dtype, rows, group, held, value):
+    """Every score of such a row is infinite or NaN, so its softmax is NaN, also where all of them
+    are minus infinity; no other row changes, and a row that sees no key stays 0."""
+    dim, heads = 64, 2
+    cpu, cache, table = _cache(1, held, heads, dim, 16, dtype, 7, cuda_device)
+    for t in (cpu, cache):  # all keys on one side: the code of 5
+        t.k_codes.view(torch.uint8)[..., 7] = 5 if dtype == INT8 else 0x4A
+    q = _normal((rows, heads * group, dim), 8)
+    lengths = torch.tensor([held], dtype=torch.int32)
+    want = ref.attention(q, *cpu, table, lengths)
+    bad = torch.zeros((rows, heads * group), dtype=torch.bool)
+    bad[0, 0] = bad[rows - 1, heads * group - 1] = True
+    qb = q.clone()
+    qb[..., 7][bad] = value
+    got = ops_q8.kv_cache_attention(qb.to(cuda_device), cache, table.to(cuda_device),
+                                    lengths.to(cuda_device)).cpu()
+    ops.device_status()
+    if held < rows:
+        assert not got[0].any()
+        bad[0, 0] = False
+    assert got[bad].isnan().all()
+    _check(got[~bad], *(t[~bad] for t in want), held)
