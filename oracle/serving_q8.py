@@ -139,3 +139,38 @@ def attention(q, k_codes, v_codes, k_scales, v_scales, table, lengths, starts=No
                 crowd[first + i, h] = (seen * TOP[v_codes.dtype]
                                        * v_scales[blocks, h // group].to(F64).max())
     return out, weight, reach, crowd
+
+
+def attention_by_products(q, k_codes, v_codes, k_scales, v_scales, table, lengths, starts=None, *,
+                          causal=True, scale=None):
+    """What `attention` gives, for long sequences: matrix products on the tensors' device."""
+    rows, heads, dim = q.shape
+    cache_heads, block = k_codes.shape[1:3]
+    group = heads // cache_heads
+    scale = dim**-0.5 if scale is None else scale
+    like = dict(dtype=F64, device=q.device)
+    out, weight = (torch.zeros(q.shape, **like) for _ in range(2))
+    reach, crowd = (torch.zeros((rows, heads, 1), **like) for _ in range(2))
+    for b, (first, n) in enumerate(rows_of(starts, len(lengths), rows)):
+        length = int(lengths[b])
+        if not length or not n:
+            continue
+        k = cached(k_codes, k_scales, table[b], length)
+        v = cached(v_codes, v_scales, table[b], length)
+        pages = table[b, : -(-length // block)].long().to(q.device)
+        tops = v_scales[pages].to(F64).cummax(0).values  # (pages, heads): the largest so far
+        for i0 in range(0, n, 128):
+            i = torch.arange(i0, min(n, i0 + 128), device=q.device)
+            seen = (length - n + i + 1).clamp(0, length) if causal else torch.full_like(i, length)
+            hidden = (torch.arange(length, device=q.device)[None] >= seen[:, None])[:, None]
+            last = ((seen - 1).clamp(min=0) // block)
+            for h in range(cache_heads):
+                at = (slice(first + i0, first + i0 + len(i)), slice(h * group, (h + 1) * group))
+                x = q[at].to(F64)
+                s = (x @ k[h].T * scale).masked_fill(hidden, -math.inf)
+                p = torch.softmax(s, -1).masked_fill((seen == 0)[:, None, None], 0.0)
+                out[at], weight[at] = p @ v[h], p @ v[h].abs()
+                reach[at] = ((x.abs() @ k[h].abs().T).masked_fill(hidden, 0.0)
+                             .amax(-1, keepdim=True) * scale)
+                crowd[at] = (seen * TOP[v_codes.dtype] * tops[last, h])[:, None, None]
+    return out, weight, reach, crowd

@@ -6,6 +6,7 @@ import pytest
 import torch
 
 from kinomlx_b200 import _lib, ops_q8
+from oracle import serving_q8 as ref
 
 BF16 = torch.bfloat16
 
@@ -40,3 +41,16 @@ def test_products_that_int32_cannot_hold_are_refused(k):
     lib = _lib.load()
     assert lib.kino_q8_linear(at, k, at, at, k, at, None, at, 64, 4, 64, k, None) == 2
     assert "k <" in _lib.last_error()
+
+
+@pytest.mark.parametrize("causal", [True, False])
+def test_oracle_attention_by_products(causal):
+    g = torch.Generator().manual_seed(3)
+    codes = [torch.randint(-127, 128, (12, 2, 16, 64), generator=g, dtype=torch.int8) for _ in range(2)]
+    scales = [torch.rand((12, 2), generator=g) * 0.02 for _ in range(2)]
+    table = torch.randperm(12, generator=g).view(2, 6).to(torch.int32)
+    q = torch.randn((150, 6, 64), generator=g).to(BF16)
+    lengths, starts = torch.tensor([90, 20]), torch.tensor([0, 120, 148])  # queries in front of the keys
+    args = (q, *codes, *scales, table, lengths, starts)
+    for a, b in zip(ref.attention(*args, causal=causal), ref.attention_by_products(*args, causal=causal)):
+        assert torch.allclose(a, b, rtol=1e-12, atol=1e-12)
