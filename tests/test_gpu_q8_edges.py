@@ -233,3 +233,43 @@ def test_attention_of_infinite_queries(cuda_device, dtype, rows, group, held, va
         bad[0, 0] = False
     assert got[bad].isnan().all()
     _check(got[~bad], *(t[~bad] for t in want), held)
+
+
+@pytest.mark.parametrize("rows", [4, 90])
+def test_attention_takes_rows_and_heads_in_any_order(cuda_device, rows):
+    dim, heads, group = 64, 2, 3
+    _, cache, table = _cache(2, 200, heads, dim, 32, INT8, 9, cuda_device)
+    lengths = torch.tensor([200, 130], dtype=torch.int32, device=cuda_device)
+    args = (cache, table.to(cuda_device), lengths)
+    q = _normal((2 * rows, heads * group, dim), 10).to(cuda_device)
+    want = ops_q8.kv_cache_attention(q, *args)
+    turned = q.transpose(0, 1).contiguous().transpose(0, 1)  # heads outside
+    assert torch.equal(ops_q8.kv_cache_attention(turned, *args), want)
+    out = torch.empty((heads * group, 2 * rows, dim), dtype=BF16, device=cuda_device).transpose(0, 1)
+    ops_q8.kv_cache_attention(turned, *args, out=out)
+    assert torch.equal(out, want)
+    # one head, and one row, for all of them
+    for same in (q[:, :1].expand(-1, heads * group, -1), q[:1].expand(2 * rows, -1, -1)):
+        assert torch.equal(ops_q8.kv_cache_attention(same, *args),
+                           ops_q8.kv_cache_attention(same.contiguous(), *args))
+
+
+def test_a_cache_whose_offsets_pass_32_bits(cuda_device):
+    heads, block, dim, blocks = 8, 128, 128, 32776  # 2^32 + 2^20 bytes of codes, K and V each
+    big = ops_q8.new_kv_cache(blocks, heads, dim, block_tokens=block, device=cuda_device)
+    small = ops_q8.new_kv_cache(8, heads, dim, block_tokens=block, device=cuda_device)
+    pages = torch.tensor([[32775, 3, 16390], [8200, 32769, 32770]], dtype=torch.int32, device=cuda_device)
+    near = torch.tensor([[0, 1, 2], [3, 4, 5]], dtype=torch.int32, device=cuda_device)
+    k, v = _normal((2 * 330, heads, dim), 1).to(cuda_device), _normal((2 * 330, heads, dim), 2).to(cuda_device)
+    zero = torch.zeros(2, dtype=torch.int32, device=cuda_device)
+    after = zero + 330
+    for cache, table in ((big, pages), (small, near)):
+        ops_q8.kv_cache_write(cache, k, v, table, zero)
+    for a, b in zip(ops_q8.kv_cache_read(big, pages, after, 333),
+                    ops_q8.kv_cache_read(small, near, after, 333)):
+        assert torch.equal(a, b) and a[:, :330].any()
+    for rows in (1, 9, 120):
+        q = _normal((2 * rows, heads, dim), rows).to(cuda_device)
+        assert torch.equal(ops_q8.kv_cache_attention(q, big, pages, after),
+                           ops_q8.kv_cache_attention(q, small, near, after))
+    ops.device_status()
