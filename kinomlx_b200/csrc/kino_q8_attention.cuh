@@ -682,7 +682,11 @@ struct Q8PrefillSmem {
   // q_full, q_empty, kv_full[S], kv_empty[S], kv_peer[S], s_full[4], p_full[4], pv_done[2], o_full,
   // o_empty, drain
   static constexpr int NBAR = 2 + 3 * STAGES + 4 + 4 + 2 + 3;
-  static constexpr int TOTAL = BAR_OFF + NBAR * 8 + 64 + 1024;
+  static constexpr int USED = BAR_OFF + NBAR * 8 + 64 + 1024;
+  // No CTA of another kernel that holds tensor memory while it waits for its cluster may share an SM
+  // (each could wait for columns that the other holds on the cluster's other SM): heads of 64 ask
+  // for more than they use.
+  static constexpr int TOTAL = USED > 140 * 1024 ? USED : 140 * 1024;
 };
 
 // sdesc_mn128 for 32 elements a row: 64-byte rows along K with the 64-byte swizzle, 8-row groups

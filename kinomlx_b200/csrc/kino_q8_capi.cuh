@@ -180,6 +180,10 @@ kino_status launch_q8_decode(const kino_q8_cache* c, const kino::Q8Attn& a, cuda
   return check_launch("kino_q8_attention");
 }
 
+// (see Q8PrefillSmem; 228 KB an SM, 1 KB of them for each CTA)
+static_assert(kino::Q8PrefillSmem<64>::TOTAL + kino::Q8WideSmem<16>::TOTAL + 2048 > 228 * 1024,
+              "the product's cluster form does not fit beside the attention");
+
 template <int D, int FMT>
 kino_status launch_q8_attention(const kino_q8_cache* c, kino::Q8Attn& a, int decode_tiles,
                                 cudaStream_t stream) {
