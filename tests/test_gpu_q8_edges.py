@@ -273,3 +273,92 @@ def test_a_cache_whose_offsets_pass_32_bits(cuda_device):
         assert torch.equal(ops_q8.kv_cache_attention(q, big, pages, after),
                            ops_q8.kv_cache_attention(q, small, near, after))
     ops.device_status()
+
+
+# ---------------------------------------------------------------- as a program uses them
+@pytest.mark.parametrize(("batch", "rows"), [(3, 3), (3, 12), (2, 200)])
+def test_graphs_replayed_with_other_lengths_starts_and_tables(cuda_device, batch, rows):
+    """Write, read and attention captured once; every replay finds other sizes on the device."""
+    dim, heads, group, block, most = 64, 2, 2, 16, 320
+    cpu, cache, table = _cache(batch, most, heads, dim, block, E4M3, 21, cuda_device)
+    first = [t.clone() for t in cache]
+    dev_table = table.to(cuda_device)
+    lengths, after, starts = (torch.zeros(n, dtype=torch.int32, device=cuda_device)
+                              for n in (batch, batch, batch + 1))
+    q = _normal((rows, heads * group, dim), 22).to(cuda_device)
+    k, v = (_normal((rows, heads, dim), s).to(cuda_device) for s in (23, 24))
+    out = torch.empty_like(q)
+
+    def run():
+        ops_q8.kv_cache_write(cache, k, v, dev_table, lengths, starts)
+        read = ops_q8.kv_cache_read(cache, dev_table, after, most)
+        ops_q8.kv_cache_attention(q, cache, dev_table, after, starts, out=out)
+        return read
+
+    stream, graph = torch.cuda.Stream(), torch.cuda.CUDAGraph()
+    with torch.cuda.stream(stream):
+        run()
+    stream.synchronize()
+    with torch.cuda.graph(graph, stream=stream):
+        read = run()
+    g = torch.Generator().manual_seed(25)
+    for step in range(6):
+        cut = torch.sort(torch.randint(0, rows + 1, (batch - 1,), generator=g)).values
+        s = torch.cat([torch.zeros(1, dtype=torch.long), cut, torch.tensor([rows if step % 2 else max(cut)])])
+        held = torch.randint(0, 100 if step < 5 else 1, (batch,), generator=g).to(torch.int32)
+        n = (s[1:] - s[:-1]).to(torch.int32)
+        page = table[torch.randperm(batch, generator=g)]
+        for t, value in ((starts, s), (lengths, held), (after, held + n), (dev_table, page)):
+            t.copy_(value)
+        for t, b in zip(cache, first):
+            t.copy_(b)
+        out.fill_(7)
+        torch.cuda.synchronize()
+        graph.replay()
+        torch.cuda.synchronize()
+        ops.device_status()
+        want = [ref.cache_write(cpu[i], cpu[2 + i], x.cpu()[: int(s[-1])], page, held, s)
+                for i, x in enumerate((k, v))]
+        for i in range(2):
+            assert torch.equal(cache[2 + i].cpu(), want[i][1]) and _same(cache[i], want[i][0])
+            for b in range(batch):
+                length = int(held[b] + n[b])
+                y = ref.cached(*want[i], page[b], length).transpose(0, 1)
+                assert torch.equal(read[i][b, :length].cpu(), y.float().to(BF16))
+                assert not read[i][b, length:].any()
+        parts = ref.attention(q.cpu()[: int(s[-1])], want[0][0], want[1][0], want[0][1], want[1][1],
+                              page, held + n, s)
+        _check(out[: int(s[-1])].cpu(), *parts, most)
+        assert bool((out[int(s[-1]):] == 7).all())
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_decoding_token_by_token_behind_a_shared_prefix(cuda_device, dtype):
+    """Sequences that share the blocks of a prefix and write behind it, a token at a time: the cache
+    holds the oracle's codes after every step, and each step's attention reads it all."""
+    dim, heads, group, block, batch, prefix, steps = 128, 2, 4, 32, 3, 64, 40
+    cpu = ops_q8.new_kv_cache(2 + 2 * batch, heads, dim, block_tokens=block, dtype=dtype, device="cpu")
+    cache = ops_q8.KVCache(*(t.to(cuda_device) for t in cpu))
+    table = torch.tensor([[0, 1, 2 + 2 * b, 3 + 2 * b] for b in range(batch)], dtype=torch.int32)
+    dev = table.to(cuda_device)
+    x = [_normal((prefix, heads, dim), s) for s in (31, 32)]
+    zero = torch.zeros(1, dtype=torch.int32)
+    ops_q8.kv_cache_write(cache, *(t.to(cuda_device) for t in x), dev[:1], zero.to(cuda_device))
+    state = [ref.cache_write(cpu[i], cpu[2 + i], x[i], table[:1], zero) for i in range(2)]
+    for step in range(steps):
+        held = torch.full((batch,), prefix + step, dtype=torch.int32)
+        size = 4.0 if step % 7 == 3 else 1.0  # now and then the blocks' scales grow
+        new = [_normal((batch, 1, dim), 100 + step, size), _normal((batch, heads, dim), 200 + step, size)]
+        new[0] = new[0].expand(batch, heads, dim)  # one key for all heads, a stride of 0
+        ops_q8.kv_cache_write(cache, new[0].to(cuda_device)[:, :1].expand(batch, heads, dim),
+                              new[1].to(cuda_device), dev, held.to(cuda_device))
+        state = [ref.cache_write(*state[i], new[i], table, held) for i in range(2)]
+        for i in range(2):
+            assert torch.equal(cache[2 + i].cpu(), state[i][1]), step
+            assert _same(cache[i], state[i][0]), step
+        if step % 13 == 0:
+            q = _normal((batch, heads * group, dim), 300 + step)
+            got = ops_q8.kv_cache_attention(q.to(cuda_device), cache, dev, (held + 1).to(cuda_device))
+            _check(got.cpu(), *ref.attention(q, state[0][0], state[1][0], state[0][1], state[1][1],
+                                             table, held + 1), prefix + step + 1)
+    ops.device_status()
