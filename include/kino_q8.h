@@ -111,8 +111,9 @@ int64_t kino_q8_attention_workspace_size(const kino_q8_cache* cache,
 
 /* softmax(q k^T * scale) v over a sequence's cached tokens [0, lengths[b]), query head h on cache
  * head h / group. The n query tokens of a sequence are its last n tokens: with `causal` query i
- * sees keys up to position lengths[b] - n + i. A query that sees no key gives zeros. Rows in front
- * of the first start and behind the last are neither read nor written. */
+ * sees keys up to position lengths[b] - n + i. A query that sees no key gives zeros; one with an
+ * infinity or a NaN gives NaN where it sees a key. Rows in front of the first start and behind the
+ * last are not written, and nothing comes of their values. */
 kino_status kino_q8_attention(const kino_q8_cache* cache, const kino_q8_attention_args* args,
                               void* stream);
 

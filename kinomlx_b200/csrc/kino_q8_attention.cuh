@@ -181,7 +181,7 @@ __device__ __forceinline__ int64_t q8_run_units(const Q8Attn& a, int64_t total) 
 // probabilities (movmatrix).
 constexpr int Q8D_BN = 64;
 // Warps that compute (one more loads): three groups of four where the registers allow it (16 x 32768
-// tokens, one tile of rows: 184 us, 192 with two groups).
+// tokens, one tile of rows, in a graph: 180 us, 188 with two groups).
 constexpr int q8d_warps(int nt) { return nt == 1 ? 12 : 8; }
 
 template <int D, int NT>
@@ -655,10 +655,11 @@ __global__ void __launch_bounds__(32 * (q8d_warps(NT) + 1), 1)
 // on over items. Tile A sees a prefix of the item's keys under a causal mask and leaves the blocks
 // behind it out.
 //
-// 4608 queries x 9216 keys, 24 heads of 128: 600 us in a short burst, 870 TFLOP/s, 630 sustained
-// (the dense bf16 kernel: 424 in a burst);
+// 4608 queries x 9216 keys, 24 heads of 128: 600 us in a graph, 870 TFLOP/s, 620 in calls one after
+// another (the cache read to bf16 and the dense bf16 kernel, two calls: 455);
 // on single CTAs with two warps a row 1400, in pairs 1100, a row a thread 810, with the issue and
-// the words between CTAs as above 655, in half blocks 600. Neither pipe is full: the tensor pipe
+// the words between CTAs as above 655, in half blocks 608, with maxima that select nothing in
+// unmasked blocks 600. Neither pipe is full: the tensor pipe
 // is busy for about 2400 of 5000 cycles a block, exponentials for 2048; the chain score ->
 // maximum -> P -> product of either tile is what remains, and the conversion (100 us of the 600).
 constexpr int Q8P_BN = 128;

@@ -149,6 +149,7 @@ kino_status plan_q8_attention(const kino_q8_cache* c, const kino_q8_attention_ar
   // kernels take any). Up to 64 rows the kernel for few rows is the faster one although it reads
   // the cache again for each 16 of them (16 sequences of 8192 tokens, 8 heads of 128: 32 rows
   // 131 us, with tcgen05 287; 64 rows 247 and 287; 8 sequences of 2000 with 128 rows 84 and 48).
+  // One kernel for the call: a prompt's chunk beside decoded tokens is better a call of its own.
   const int64_t rows = (g->rows + c->batch - 1) / c->batch * group;
   p->decode_tiles = rows <= 8 ? 1 : rows <= 64 && group <= 16 ? 2 : 0;
   const int64_t tile = p->decode_tiles ? 8 * p->decode_tiles : 512;

@@ -326,10 +326,11 @@ __global__ void __launch_bounds__(Q8_ROW_MAX_THREADS, 4) q8_wide_rows_kernel(con
 //
 // One CTA per (cache block that gets new tokens, head), K and V together (blocks of 128 tokens of
 // 128-wide heads: one of them). The new tokens' values stay in registers between the maximum and
-// the rounding. Finding the block takes two dependent reads before the first value is asked for,
-// which K and V share; several heads in turn in a CTA were slower (fewer loads in flight). A block that holds earlier tokens keeps the
-// larger of its scale and the new tokens': where it grows, the earlier codes are rounded again to
-// the new scale (at most a half step of the new scale each time).
+// the rounding. The values are asked for once the block is known, after two dependent reads (lengths
+// and starts, then the table) that K and V share; several heads in turn in a CTA were slower (fewer
+// loads in flight). A block that holds earlier tokens keeps the larger of its scale and the new
+// tokens': where it grows, the earlier codes are rounded again to the new scale (at most a half
+// step of the new scale each time).
 constexpr int Q8_WRITE_THREADS = 128;
 
 struct Q8WriteArgs {

@@ -367,7 +367,8 @@ def kv_cache_attention(
     dim) bf16, query heads a multiple of the cache's heads (head h reads cache head h // group);
     lengths (batch,) int32, the tokens in the cache, among them the sequence's queries, which are
     its last tokens: with `causal` query i of n sees keys up to position lengths - n + i. Rows go
-    to sequences as in `kv_cache_write`. A query that sees no key gives zeros. Rows of `out`
+    to sequences as in `kv_cache_write`. A query that sees no key gives zeros, an infinite one that
+    sees some NaN. Decoded tokens and prompts are faster as calls of their own. Rows of `out`
     outside every sequence are left as they were (uninitialised where `out` is not given)."""
     args = _cache_args(cache, block_table, lengths)
     device = cache[0].device
@@ -398,5 +399,6 @@ def kv_cache_attention(
         raise RuntimeError(f"kino_q8_attention: {_lib.last_error()}")
     space = torch.empty(nbytes, device=device, dtype=torch.uint8)
     call.workspace, call.workspace_bytes = space.data_ptr(), nbytes
+    # (its work goes by lengths that only the device knows: none is logged)
     _launch("kv_cache_attention", 0.0, 0.0, device, "kino_q8_attention", args, call)
     return out
